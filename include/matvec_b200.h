@@ -184,6 +184,71 @@ int mvb_gemm4(const void *w, const void *ws, const void *xq, const float *xs, fl
  * internal wait that gave up (the kernel then wrote no output), and clears it; -1 if the stream failed. */
 int mvb_gemm_status(void *stream);
 
+/* ---- Serving operators: rotary positions, a paged 8- or 4-bit cache, attention over it, log probabilities ----
+ * No counterpart in the reference, whose cache is fp32 inside its forward pass. Device pointers, asynchronous on
+ * `stream`, on the current device; 0, or -1 with the reason in mvb_last_error(). No call keeps state or needs a workspace, so
+ * calls on several streams or in several graphs do not meet. Strides are in elements.
+ *
+ * dtype of queries, keys, values, outputs and logits: MVB_F32, MVB_BF16 or MVB_F16.
+ * Cache: kq, vq hold pages x kv_heads x page rows of head integers (bits 8: int8; bits 4: two's complement nibbles, element
+ * 2i in the low half of byte i), ks, vs pages x kv_heads x page fp32 scales; value = integer * scale. page: a power of two
+ * in 16 .. 1024; head: a multiple of 16 in 16 .. 128; all four 16-byte aligned.
+ * Batch: rows cu[b] .. cu[b + 1] - 1 belong to sequence b and stand at its positions lens[b] and on; position p is slot
+ * p % page of page table[b * table_cols + p / page]. `rows` is the room of the row arrays; rows at or behind cu[batch]
+ * are left as they are. cu, lens and table are read on the device; what is out of range there is skipped and reported by
+ * mvb_serve_status. */
+#define MVB_F32 0
+#define MVB_BF16 1
+#define MVB_F16 2
+
+/* table (positions x 2 * half fp32): row p holds factor * cos of the angles (start + p) * freq[i] (freq: half fp64 on the
+ * device), then factor * sin; angles and functions in fp64, rounded once. */
+int mvb_rope_table(const double *freq, float *table, int half, int positions, int start, double factor, void *stream);
+
+/* out[t] = x[t] (heads x head, contiguous; strides from one token to the next multiples of 4) with the first rot elements
+ * of each head turned by table row pos[t] (table_rows x rot): pair (a, b) becomes (a cos - b sin, b cos + a sin). layout 0:
+ * pairs (i, i + rot / 2); 1: (2i, 2i + 1). head and rot multiples of 8, rot <= head <= 128. out may be x. A token whose
+ * position is outside the table is left out and reported. */
+int mvb_rope(const void *x, const int *pos, const float *table, void *out, int dtype, int tokens, int heads, int head,
+             int rot, int table_rows, int layout, long long x_stride, long long out_stride, void *stream);
+
+/* The batch's keys and values (rows x kv_heads x head) into the cache: scale = fl(max |x| / 127) (bits 4: / 7), integer =
+ * rint(x / scale). rope (may be NULL): keys are turned first, in fp64 (each element rounded once), by the table row pos[row]
+ * (pos NULL: the position in the cache); then q (may be NULL; rows x heads x head) is turned into q_out, which may be q.
+ * A row with an infinity or a NaN gets the scale NaN. Two sequences must not share a page that the call writes. */
+int mvb_kv_append(void *kq, float *ks, void *vq, float *vs, int pages, int page, int kv_heads, int head, int bits,
+                  const int *table, int table_cols, const int *cu, const int *lens, int batch, int rows, const void *k,
+                  long long k_stride, const void *v, long long v_stride, int dtype, const float *rope, const int *pos,
+                  int rot, int table_rows, int layout, const void *q, long long q_stride, void *q_out,
+                  long long q_out_stride, int heads, void *stream);
+
+/* The cached rows back as k_out and v_out (rows x kv_heads x head; 16-byte aligned, strides multiples of 16 bytes). */
+int mvb_kv_read(const void *kq, const float *ks, const void *vq, const float *vs, int pages, int page, int kv_heads,
+                int head, int bits, const int *table, int table_cols, const int *cu, const int *lens, int batch, int rows,
+                void *k_out, long long k_stride, void *v_out, long long v_stride, int dtype, void *stream);
+
+/* Attention of the batch's new tokens, whose keys and values are in the cache: out = softmax(scale * q k) v over positions
+ * below lens[b] and, of the new ones, those that `tree` allows: rows x words 64-bit words, bit j for the sequence's j-th new
+ * token (NULL: each sees those before it and itself). heads is a multiple of kv_heads. max_new: at least the most new
+ * tokens of a sequence (sequences with more are left out and reported); max_len: about the longest lens[b] + new tokens,
+ * which only decides how the work is split. lse (may be NULL): rows x heads, the natural log of the sum of exponentials. A
+ * row that sees nothing gives zeros and -inf. fp32 inputs give fp32-accurate results; the same call gives the same bits. */
+int mvb_tree_attention(const void *q, long long q_stride, const void *kq, const float *ks, const void *vq, const float *vs,
+                       int pages, int page, int kv_heads, int head, int bits, const int *table, int table_cols,
+                       const int *cu, const int *lens, int batch, int rows, int heads, int dtype, const void *tree,
+                       int words, float scale, int max_new, int max_len, void *out, long long out_stride, float *lse,
+                       void *stream);
+
+/* Rows of logits (vocab <= 2^21, any stride): logp[r * nids + i] = log softmax at ids[r * nids + i] (-1: 0; outside the
+ * vocabulary: NaN, reported), entropy[r] (may be NULL) in nats, and the `top` (<= 64) largest logits' ids and log
+ * probabilities, equal logits by the lowest id, NaN last. A row with a NaN, +inf or no finite logit gives NaN. */
+int mvb_logprobs(const void *x, long long stride, int dtype, int rows, int vocab, const int *ids, int nids, float *logp,
+                 float *entropy, int top, int *top_ids, float *top_logp, void *stream);
+
+/* Synchronizes `stream`; 0, or what the serving operators found out of range since the last call, and clears it: 1 a page
+ * number, 2 a length or row range, 3 a rotary position, 4 a token id; -1 if the stream failed. */
+int mvb_serve_status(void *stream);
+
 /* ---- Row-sharded matvec with the all-gather fused into the kernel (one process per GPU, NVLink peers) ----
  * No counterpart in the reference, which drives one board: this is fpga_matvec4 (driver/matvec_fpga.h:29-33)
  * for a matrix whose rows are split across `world` GPUs, rank r owning rows [r * rows, (r + 1) * rows). Each

@@ -124,6 +124,23 @@ def lib():
         L.mvb_gather_error.argtypes = [vp, vp]
         L.mvb_gather_destroy.restype = None
         L.mvb_gather_destroy.argtypes = [vp]
+        ll, f, d = C.c_longlong, C.c_float, C.c_double
+        L.mvb_rope_table.restype = i
+        L.mvb_rope_table.argtypes = [vp, vp, i, i, i, d, vp]
+        L.mvb_rope.restype = i
+        L.mvb_rope.argtypes = [vp] * 4 + [i] * 7 + [ll, ll, vp]
+        L.mvb_kv_append.restype = i
+        L.mvb_kv_append.argtypes = ([vp] * 4 + [i] * 5 + [vp, i, vp, vp, i, i, vp, ll, vp, ll, i, vp, vp, i, i, i, vp, ll,
+                                                          vp, ll, i, vp])
+        L.mvb_kv_read.restype = i
+        L.mvb_kv_read.argtypes = [vp] * 4 + [i] * 5 + [vp, i, vp, vp, i, i, vp, ll, vp, ll, i, vp]
+        L.mvb_tree_attention.restype = i
+        L.mvb_tree_attention.argtypes = ([vp, ll] + [vp] * 4 + [i] * 5 + [vp, i, vp, vp] + [i] * 4 +
+                                         [vp, i, f, i, i, vp, ll, vp, vp])
+        L.mvb_logprobs.restype = i
+        L.mvb_logprobs.argtypes = [vp, ll, i, i, i, vp, i, vp, vp, i, vp, vp, vp]
+        L.mvb_serve_status.restype = i
+        L.mvb_serve_status.argtypes = [vp]
         _bind_extra(L)
         _lib = L
     return _lib
@@ -261,6 +278,12 @@ def gemm4(w, ws, xq, xs, out, n, d, m, ldx, wbits, stream=None):
 def gemm_status(stream=None):
     """Synchronizes and returns the GEMM kernels' error word (0 = every internal wait completed)."""
     return lib().mvb_gemm_status(_stream(stream))
+
+
+# ---- serving operators over a paged quantized cache (serving.py; include/matvec_b200.h, mvb_rope .. mvb_logprobs) ----
+
+from .serving import (KvCache, LogProbs, kv_append, kv_read, logprobs, rope, rope_frequencies,  # noqa: E402,F401
+                      rope_table, serve_status, tree_attention, tree_mask)
 
 
 # ---- row-sharded matvec with the all-gather in the kernel (include/matvec_b200.h, mvb_gather_*) ----

@@ -6,6 +6,7 @@ usage: python build.py [--verbose]     (--verbose adds -Xptxas -v: registers, sp
 -ffp-contract=off), so neither does any kernel here. The CUDA runtime is linked statically so that hosts built
 from the reference's C (-lmatvec_b200) need nothing else.
 """
+import concurrent.futures
 import glob
 import os
 import subprocess
@@ -13,9 +14,10 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB = os.path.join(HERE, "libmatvec_b200.so")
+OBJ = os.path.join(HERE, "build")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-fmad=false", "-Xcompiler", "-fPIC,-O2", "-shared", "-cudart", "static",
+FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-fmad=false", "-Xcompiler", "-fPIC,-O2", "-cudart", "static",
          "--expt-relaxed-constexpr"]
 
 
@@ -35,12 +37,23 @@ def up_to_date():
 def build(verbose=False, force=False):
     if not force and not verbose and up_to_date():
         return LIB
-    cmd = [NVCC, *ARCH, *FLAGS, *(["-Xptxas", "-v"] if verbose else []), "-o", LIB + ".tmp", *sources()]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + r.stdout + r.stderr)
+    os.makedirs(OBJ, exist_ok=True)
+
+    def run(cmd):
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + r.stdout + r.stderr)
+        return r.stdout + r.stderr
+
+    def compile_one(src):  # each source on its own, side by side
+        obj = os.path.join(OBJ, os.path.basename(src) + ".o")
+        return obj, run([NVCC, *ARCH, *FLAGS, *(["-Xptxas", "-v"] if verbose else []), "-c", "-o", obj, src])
+
+    with concurrent.futures.ThreadPoolExecutor(os.cpu_count()) as pool:
+        objs, logs = zip(*pool.map(compile_one, sources()))
     if verbose:
-        sys.stdout.write(r.stdout + r.stderr)
+        sys.stdout.write("".join(logs))
+    run([NVCC, *ARCH, "-shared", "-cudart", "static", "-o", LIB + ".tmp", *objs])
     os.replace(LIB + ".tmp", LIB)
     return LIB
 

@@ -1,0 +1,94 @@
+// Shared by the two kernels of mvb_tree_attention (tree_attention.cu: few query rows; tree_attention_tc.cu: many).
+#pragma once
+#include "rows.cuh"
+
+namespace mvb {
+namespace attn {
+
+struct AttnParams {
+    const void *q;
+    void *out;
+    float *lse;  // or null
+    const uint8_t *kq, *vq;
+    const float *ks, *vs;
+    rows::Batch bt;
+    const unsigned long long *tree;  // or null: each new token sees those before it and itself
+    long long q_stride, out_stride;
+    float scale_log2;  // the softmax scale times log2(e)
+    int words, rows, heads, kv_heads, group, head, max_new, qtiles, splits;
+};
+
+// One sequence of the batch, its index arrays checked (a value out of range is noted and clamped: no access leaves
+// the arrays, and mvb_serve_status tells).
+struct Sequence {
+    int row0, n, ctx, len;  // first row, new tokens, cached positions before them, ctx + n
+};
+
+__device__ __forceinline__ Sequence sequence_at(const AttnParams &p, int b, int *error) {
+    Sequence s;
+    s.row0 = p.bt.cu[b];
+    const int end = p.bt.cu[b + 1];
+    s.ctx = p.bt.lens[b];
+    bool ok = s.row0 >= 0 && end >= s.row0 && end <= p.rows && end - s.row0 <= p.max_new && s.ctx >= 0;
+    s.n = ok ? end - s.row0 : 0;
+    const long long most = (long long)p.bt.table_cols << p.bt.page_log2;
+    if (ok && (long long)s.ctx + s.n > most) ok = false, s.n = 0;
+    if (!ok) rows::note(error, rows::kBadLength);
+    s.len = s.ctx + s.n;
+    return s;
+}
+
+// The page of position pos (in range of the table): page 0 with the error noted where the table names none.
+__device__ __forceinline__ int page_of(const AttnParams &p, int b, int pos, int *error) {
+    const int pg = p.bt.table[(size_t)b * p.bt.table_cols + (pos >> p.bt.page_log2)];
+    if ((unsigned)pg < (unsigned)p.bt.pages) return pg;
+    rows::note(error, rows::kBadPage);
+    return 0;
+}
+
+// Whether new token i of the sequence may see position t.
+__device__ __forceinline__ bool allowed(const AttnParams &p, const Sequence &s, int i, int t) {
+    if (t < s.ctx) return true;
+    const int j = t - s.ctx;
+    if (j >= s.n || i >= s.n) return false;
+    if (!p.tree) return j <= i;
+    if ((j >> 6) >= p.words) return false;
+    return (p.tree[(size_t)(s.row0 + i) * p.words + (j >> 6)] >> (j & 63)) & 1;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {  // 2 ulp; exp2(-inf) = 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// 2^k as fp32 for k in [-126, 127].
+__device__ __forceinline__ float pow2(int k) { return __int_as_float((k + 127) << 23); }
+
+// Biased exponent of |x| (0 for zero and subnormals, 255 for infinities and NaN).
+__device__ __forceinline__ int exponent_of(float x) { return (__float_as_int(x) >> 23) & 255; }
+
+// Four int8 of a word, with the sign bits flipped by the caller (x ^ 0x80808080), as two exact half2: the byte in the
+// low mantissa of 1024 gives 1024 + (v + 128).
+__device__ __forceinline__ uint32_t bytes_to_half2(uint32_t x, uint32_t selector) {
+    uint32_t h;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(h) : "r"(x), "r"(0x64646464u), "r"(selector));
+    const uint32_t bias = 0x64806480u;  // 1152
+    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(h) : "r"(bias));
+    return h;
+}
+
+// Nibbles k and k + 4 of a word, sign bits flipped (x ^ 0x88888888), as an exact half2: 1024 + (v + 8).
+__device__ __forceinline__ uint32_t nibbles_to_half2(uint32_t x, int k) {
+    uint32_t h = ((x >> (4 * k)) & 0x000F000Fu) | 0x64006400u;
+    const uint32_t bias = 0x64086408u;  // 1032
+    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(h) : "r"(bias));
+    return h;
+}
+
+int tc_take_error(cudaStream_t s);
+// The kernel for many query rows; returns the CUDA error of its launch.
+cudaError_t launch_tc(const AttnParams &p, int dtype, int bits, int max_len, cudaStream_t s);
+
+}  // namespace attn
+}  // namespace mvb

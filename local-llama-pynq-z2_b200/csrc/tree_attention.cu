@@ -7,17 +7,20 @@
 // with k and v the cached integers, which fp16 holds exactly: the products take them as they are, the keys' scales
 // multiply S and the values' scales multiply P. q is put in fp16 after a power of two of its row's largest element was
 // taken out (2 ^ e; a bf16 or fp16 q keeps every bit that is above 2^-33 of the row's largest); an fp32 q goes in two
-// parts, high and low (22 bits), and its P too, so that fp32 callers get fp32 results: two products each instead of one.
-// Else P is rounded to fp16 once (2^-12), less than the output's own rounding. max, sum and O are fp32.
+// parts, high and low (22 bits). P is rounded to fp16 once for bf16 callers (2^-12, an eighth of the output's own half
+// step); for fp16 and fp32 callers it goes in two parts too (22 bits), since one rounding would be as large as an fp16
+// output's own. max, sum and O are fp32.
 //
-// This kernel: up to 16 * MT query rows (new tokens x the query heads of one kv head) at a time; a handful of rows does
-// little arithmetic per cached byte, so the work is to stream the cache. One warp owns 16-key slices (HDP = 128; 32
-// keys for HDP = 64): cp.async into its own ring of three stages, no barrier with the other warps; keys go from bytes
-// to fp16 fragments of mma.m16n8k16 in registers. The order of the head's elements inside a product is free as long as
-// q and k agree, and so is the order of the keys in P v: both are chosen so that a lane reads whole 4- to 16-byte
-// pieces. Keys of a sequence are split over the warps of a CTA and over the CTAs of a cluster (up to 16), whose partial
-// (max, sum, O) are joined in distributed shared memory in a fixed order: one launch, no workspace, the same bits on
-// every run.
+// This kernel: 8 * NT query rows (new tokens x the query heads of one kv head) at a time; a handful of rows does little
+// arithmetic per cached byte, so the work is to stream the cache with few instructions a byte. One warp owns slices of 16
+// keys (HDP = 128) or 32 (HDP = 64): cp.async into its own ring of three stages, no barrier with the other warps. The
+// products are mma.m16n8k16 with the cache as the 16-row operand (S^T = K Q^T, O^T = V^T P^T): eight query rows cost
+// eight columns, and a slice's fragments, converted from bytes in registers, serve all NT column tiles. S^T leaves a lane
+// with (key, two rows); movmatrix turns that into the operand of the second product. The order of the head's elements
+// inside a product is free as long as q and k agree, and so is the order of the keys in P v: both are chosen so that a
+// lane reads whole 4- to 16-byte pieces. Keys of a sequence are split over the warps of a CTA and over the CTAs of a
+// cluster (up to 16), whose partial (max, sum, O) are joined in distributed shared memory in a fixed order: one launch,
+// no workspace, the same bits on every run.
 #include <cooperative_groups.h>
 #include <limits.h>
 #include <math.h>
@@ -66,31 +69,46 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint4 &a, uint32_t
         : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ void cp_async(uint32_t dst, const void *src, int bytes) {
-    if (bytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+template <int BYTES>
+__device__ __forceinline__ void cp_async(uint32_t dst, const void *src) {
+    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
     else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
 
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {  // of an 8 x 8 tile of 16-bit elements
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
 // The head element that element e (0 .. 3: k = 2c, 2c + 1, 2c + 8, 2c + 9) of lane column c holds in k-step ks: a lane
-// reads 16 elements (64 * (ks / 4) + 16 c ..) at once and spreads them over four k-steps, in byte order for 8 bits, as
-// (o, o + 4), (o + 1, o + 5) of each 8 for 4 bits.
+// reads 16 elements (64 * (ks / 4) + 16 c ..) at once and spreads them over four k-steps as the conversions leave them:
+// bytes (0, 2) and (1, 3) of a word, nibbles (o, o + 4) and (o + 1, o + 5).
 template <int BITS>
 __device__ __forceinline__ int element_of(int ks, int c, int e) {
     const int base = 64 * (ks >> 2) + 16 * c, w = ks & 3;
-    if (BITS == 8) return base + 4 * w + e;
+    if (BITS == 8) return base + 4 * w + (e >> 1) + 2 * (e & 1);
     return base + 8 * (w >> 1) + 2 * (w & 1) + (e >> 1) + 4 * (e & 1);
 }
 
-template <typename T, int BITS, int HDP, int MT>
-__global__ void __launch_bounds__(kWarps * 32, MT == 1 ? 2 : 1) tree_attention_kernel(const AttnParams p) {
+// Parts of q and of P for each caller's type.
+template <typename T> struct Parts { static constexpr int kQ = 1, kP = 1; };
+template <> struct Parts<__half> { static constexpr int kQ = 1, kP = 2; };
+template <> struct Parts<float> { static constexpr int kQ = 2, kP = 2; };
+
+template <typename T, int BITS, int HDP, int NT>
+__global__ void __launch_bounds__(kWarps * 32, NT <= 2 ? 2 : 1) tree_attention_kernel(const AttnParams p) {
     using S = Slice<HDP, BITS>;
-    constexpr int KS = HDP / 16, NT = HDP / 8;   // k-steps of q.k; 8-column tiles of O (tile j: elements NT * n + j)
-    constexpr int NP = sizeof(T) == 4 ? 2 : 1;   // parts of q and of P
-    constexpr int ROWS = 16 * MT;
+    constexpr int KS = HDP / 16;                 // k-steps of q.k, and 16-element tiles of O
+    constexpr int RUN = HDP / 8;                 // a lane's elements of a value row: RUN * r ..
+    constexpr int QP = Parts<T>::kQ, PP = Parts<T>::kP;
+    constexpr int ROWS = 8 * NT;
+    constexpr bool QREG = NT * QP * KS <= (NT == 1 ? 16 : 8);  // q's fragments in registers, else read again for every slice
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float row_factor[ROWS], warp_m[kWarps][ROWS], warp_l[kWarps][ROWS], cta_m[ROWS], cta_l[ROWS];
-    uint4 *qfrag = reinterpret_cast<uint4 *>(smem);  // [NP][MT][KS][32 lanes]
-    uint8_t *pipe = smem + NP * MT * KS * 512;
+    __shared__ float all_m[16][ROWS], all_l[16][ROWS];
+    uint2 *qfrag = reinterpret_cast<uint2 *>(smem);  // [QP][NT][KS][32 lanes]
+    uint8_t *pipe = smem + QP * NT * KS * 256;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
     const int b = blockIdx.z, kvh = blockIdx.y / p.qtiles, qt = blockIdx.y - kvh * p.qtiles, split = blockIdx.x;
@@ -119,15 +137,25 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 1 ? 2 : 1) tree_attention_k
             const size_t row = (((size_t)pg * p.kv_heads + kvh) << p.bt.page_log2) + (key & ((1 << p.bt.page_log2) - 1));
             const uint8_t *kp = p.kq + row * row_bytes + lane * piece, *vp = p.vq + row * row_bytes + lane * piece;
             const uint32_t d = mine_u + stage * S::kStage + sub * 16 * S::kRow;
+            if (piece == 16) {
 #pragma unroll
-            for (int i = 0; i < S::kPieces; i++)
-                if (doff[i] >= 0) {
-                    cp_async(d + doff[i], kp + 32 * i * piece, piece);
-                    cp_async(d + S::kKeys * S::kRow + doff[i], vp + 32 * i * piece, piece);
-                }
-            const uint32_t ds = mine_u + stage * S::kStage + S::kScales + sub * 64;
-            if (lane < 4) cp_async(ds + 16 * lane, p.ks + row + 4 * lane, 16);
-            else if (lane < 8) cp_async(ds + S::kKeys * 4 + 16 * (lane - 4), p.vs + row + 4 * (lane - 4), 16);
+                for (int i = 0; i < S::kPieces; i++)
+                    if (doff[i] >= 0) {
+                        cp_async<16>(d + doff[i], kp + 512 * i);
+                        cp_async<16>(d + S::kKeys * S::kRow + doff[i], vp + 512 * i);
+                    }
+            } else {
+#pragma unroll
+                for (int i = 0; i < S::kPieces; i++)
+                    if (doff[i] >= 0) {
+                        cp_async<8>(d + doff[i], kp + 256 * i);
+                        cp_async<8>(d + S::kKeys * S::kRow + doff[i], vp + 256 * i);
+                    }
+            }
+            // the scales: lanes 0 .. 3 the keys', 4 .. 7 the values'
+            if (lane < 8)
+                cp_async<16>(mine_u + stage * S::kStage + S::kScales + sub * 64 + (lane >> 2) * S::kKeys * 4 + 16 * c,
+                             (lane < 4 ? p.ks : p.vs) + row + 4 * c);
         }
     };
     int sl_next = s0 + warp;
@@ -157,45 +185,49 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 1 ? 2 : 1) tree_attention_k
         if (lane == 0) row_factor[i] = pow2(k);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < MT * KS * 32; i += kWarps * 32) {
-        const int ln = i & 31, ks = (i >> 5) % KS, mt = (i >> 5) / KS;
-        const float *a = qrow + (mt * 16 + (ln >> 2)) * HDP, *bq = a + 8 * HDP;
-        float f[8];
+    for (int i = threadIdx.x; i < NT * KS * 32; i += kWarps * 32) {
+        const int ln = i & 31, ks = (i >> 5) % KS, nt = (i >> 5) / KS;
+        const float *a = qrow + (nt * 8 + (ln >> 2)) * HDP;
+        float f[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int d = element_of<BITS>(ks, ln & 3, e);
-            f[e] = a[d];
-            f[4 + e] = bq[d];
-        }
-        const uint4 hi = make_uint4(pack2<__half>(f[0], f[1]), pack2<__half>(f[4], f[5]), pack2<__half>(f[2], f[3]),
-                                    pack2<__half>(f[6], f[7]));
-        qfrag[i] = hi;
-        if (NP == 2) {
+        for (int e = 0; e < 4; e++) f[e] = a[element_of<BITS>(ks, ln & 3, e)];
+        qfrag[i] = make_uint2(pack2<__half>(f[0], f[1]), pack2<__half>(f[2], f[3]));
+        if (QP == 2) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) f[e] = f[e] - __half2float(__float2half_rn(f[e]));
-            qfrag[MT * KS * 32 + i] = make_uint4(pack2<__half>(f[0], f[1]), pack2<__half>(f[4], f[5]),
-                                                 pack2<__half>(f[2], f[3]), pack2<__half>(f[6], f[7]));
+            for (int e = 0; e < 4; e++) f[e] = f[e] - __half2float(__float2half_rn(f[e]));
+            qfrag[NT * KS * 32 + i] = make_uint2(pack2<__half>(f[0], f[1]), pack2<__half>(f[2], f[3]));
         }
     }
     __syncthreads();
+    uint2 qreg[QREG ? QP * NT * KS : 1];
+    if (QREG) {
+#pragma unroll
+        for (int i = 0; i < QP * NT * KS; i++) qreg[i] = qfrag[i * 32 + lane];
+    }
 
-    float O[MT][NT][4], m[MT][2], l[MT][2], rf[MT][2];
-    int draft[MT][2];
+    // this lane's rows of column tile nt: 8 nt + 2c, + 1
+    float O[NT][KS][4], m[NT][2], l[NT][2], rf[NT][2];
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++) {
+    for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-        for (int j = 0; j < NT; j++)
+        for (int j = 0; j < KS; j++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) O[mt][j][e] = 0.0f;
+            for (int e = 0; e < 4; e++) O[nt][j][e] = 0.0f;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            m[mt][h] = -INFINITY;
-            l[mt][h] = 0.0f;
-            rf[mt][h] = row_factor[mt * 16 + r + 8 * h];
-            draft[mt][h] = (R0 + mt * 16 + r + 8 * h) / p.group;
+            m[nt][h] = -INFINITY;
+            l[nt][h] = 0.0f;
+            rf[nt][h] = row_factor[nt * 8 + 2 * c + h];
         }
     }
-    float W = pow2(-100);  // at or above every |vs| so far, a power of two
+    float W = pow2(-100);  // at or above every finite |vs| so far, a power of two
+
+    // where this lane's fragments lie in a stage (+ 16 * kRow * sub; the rows 8 further lie 8 * kRow further)
+    const int k_at = place<S::kRow>(r, BITS == 8 ? 16 * c : 8 * c);
+    const int k_at1 = HDP == 128 ? place<S::kRow>(r, BITS == 8 ? 64 + 16 * c : 32 + 8 * c) : 0;
+    constexpr int WORDS = RUN * BITS / 32;  // 32-bit words of a key's elements: 4, 2 (8 bits), 2, 1 (4 bits)
+    const int v_at = S::kKeys * S::kRow + place<S::kRow>(2 * c, r * WORDS * 4);
+    const int v_at1 = S::kKeys * S::kRow + place<S::kRow>(2 * c + 1, r * WORDS * 4);
 
     int stage = 0;
     for (int sl = s0 + warp; sl < s1; sl += kWarps) {
@@ -207,36 +239,34 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 1 ? 2 : 1) tree_attention_k
         }
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
         __syncwarp();
-        const uint8_t *kt = mine + stage * S::kStage, *vt = kt + S::kKeys * S::kRow;
+        const uint8_t *kt = mine + stage * S::kStage;
         const float *ksc = reinterpret_cast<const float *>(kt + S::kScales), *vsc = ksc + S::kKeys;
         const int key0 = sl * S::kKeys;
 
-        float sc[MT][S::kSub][2][4];
+        float sc[NT][S::kSub][4];  // (key r, row 2c), (key r, row 2c + 1), (key r + 8, ..), ..
 #pragma unroll
         for (int sub = 0; sub < S::kSub; sub++) {
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
+            for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int n = 0; n < 2; n++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) sc[mt][sub][n][e] = 0.0f;
+                for (int e = 0; e < 4; e++) sc[nt][sub][e] = 0.0f;
 #pragma unroll
             for (int ch = 0; ch < HDP / 64; ch++) {
-                uint32_t kb[2][4][2];  // [8-key tile][k-step of this chunk][b0, b1]
+                uint32_t kb[2][4][2];  // [key r, r + 8][k-step of this chunk][low, high k]
 #pragma unroll
                 for (int n = 0; n < 2; n++) {
-                    const int row = sub * 16 + n * 8 + r;
+                    const uint8_t *src = kt + (ch ? k_at1 : k_at) + (sub * 16 + n * 8) * S::kRow;
                     if (BITS == 8) {
-                        const uint4 u = *reinterpret_cast<const uint4 *>(kt + place<S::kRow>(row, 64 * ch + 16 * c));
-                        const uint32_t w[4] = {u.x ^ 0x80808080u, u.y ^ 0x80808080u, u.z ^ 0x80808080u, u.w ^ 0x80808080u};
+                        const uint4 u = *reinterpret_cast<const uint4 *>(src);
+                        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
-                            kb[n][k][0] = bytes_to_half2(w[k], 0x4140u);
-                            kb[n][k][1] = bytes_to_half2(w[k], 0x4342u);
+                            kb[n][k][0] = bytes_to_half2(w[k]);
+                            kb[n][k][1] = bytes_to_half2(w[k] >> 8);
                         }
                     } else {
-                        const uint2 u = *reinterpret_cast<const uint2 *>(kt + place<S::kRow>(row, 32 * ch + 8 * c));
-                        const uint32_t w[2] = {u.x ^ 0x88888888u, u.y ^ 0x88888888u};
+                        const uint2 u = *reinterpret_cast<const uint2 *>(src);
+                        const uint32_t w[2] = {u.x, u.y};
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
                             kb[n][k][0] = nibbles_to_half2(w[k >> 1], 2 * (k & 1));
@@ -245,119 +275,130 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 1 ? 2 : 1) tree_attention_k
                     }
                 }
 #pragma unroll
-                for (int k = 0; k < 4; k++)
+                for (int k = 0; k < 4; k++) {
+                    const uint4 a = make_uint4(kb[0][k][0], kb[1][k][0], kb[0][k][1], kb[1][k][1]);
 #pragma unroll
-                    for (int mt = 0; mt < MT; mt++)
+                    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                        for (int part = 0; part < NP; part++) {
-                            const uint4 a = qfrag[((part * MT + mt) * KS + 4 * ch + k) * 32 + lane];
-#pragma unroll
-                            for (int n = 0; n < 2; n++) mma16816(sc[mt][sub][n], a, kb[n][k][0], kb[n][k][1]);
+                        for (int part = 0; part < QP; part++) {
+                            const int i = (part * NT + nt) * KS + 4 * ch + k;
+                            const uint2 q = QREG ? qreg[QREG ? i : 0] : qfrag[i * 32 + lane];
+                            mma16816(sc[nt][sub], a, q.x, q.y);
                         }
+                }
             }
         }
-        // scales of this lane's keys, the mask, and the values' scales
-        const bool tail = key0 + S::kKeys > s.ctx;  // some key is a new token's, or none
-        float vv[S::kSub][2][2], mv = 0.0f;
+        // the scales of this lane's keys; S in units of the row's factor; the mask where some key is new or none
+        float vv[S::kSub][2];
+        const bool tail = key0 + S::kKeys > s.ctx;
+        bool move = false;
 #pragma unroll
         for (int sub = 0; sub < S::kSub; sub++)
 #pragma unroll
             for (int n = 0; n < 2; n++) {
-                const int i = sub * 16 + n * 8 + 2 * c;
-                const float2 k2 = *reinterpret_cast<const float2 *>(ksc + i);
-                const float2 v2 = *reinterpret_cast<const float2 *>(vsc + i);
-                const float kk[2] = {k2.x * p.scale_log2, k2.y * p.scale_log2};
-                vv[sub][n][0] = key0 + i < s.len ? v2.x : 0.0f;
-                vv[sub][n][1] = key0 + i + 1 < s.len ? v2.y : 0.0f;
-                // (an infinite scale makes the rows that see it infinite; it must not set W for the others)
+                const float kk = ksc[sub * 16 + n * 8 + r] * p.scale_log2;
+                vv[sub][n] = vsc[sub * 16 + n * 8 + r];
 #pragma unroll
-                for (int e = 0; e < 2; e++)
-                    if (fabsf(vv[sub][n][e]) < INFINITY) mv = fmaxf(mv, fabsf(vv[sub][n][e]));
-#pragma unroll
-                for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        float u = sc[mt][sub][n][e] * kk[e & 1];
-                        if (tail && !allowed(p, s, draft[mt][e >> 1], key0 + i + (e & 1))) u = -INFINITY;
-                        sc[mt][sub][n][e] = u;
-                    }
+                for (int nt = 0; nt < NT; nt++) {
+                    sc[nt][sub][2 * n] *= kk;
+                    sc[nt][sub][2 * n + 1] *= kk;
+                }
             }
-        mv = fmaxf(mv, __shfl_xor_sync(0xffffffffu, mv, 1));
-        mv = fmaxf(mv, __shfl_xor_sync(0xffffffffu, mv, 2));
-        // running maxima (log2 units); they move only when some row is kLazy behind
-        float mx[MT][2];
-        bool move = mv > W;
+        if (tail) {
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
+            for (int sub = 0; sub < S::kSub; sub++)
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    const int key = key0 + sub * 16 + n * 8 + r;
+                    if (key >= s.len) vv[sub][n] = 0.0f;
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++)
+                            if (!allowed(p, s, (R0 + nt * 8 + 2 * c + h) / p.group, key)) sc[nt][sub][2 * n + h] = -INFINITY;
+                }
+        }
+        // The running maxima (log2 units) and W move only when some row falls kLazy behind, or a value's scale passes
+        // W: every lane looks at its own scores, one vote a slice; the maxima are exchanged only then.
+        float mx[NT][2], mv = 0.0f;
+#pragma unroll
+        for (int sub = 0; sub < S::kSub; sub++)
+#pragma unroll
+            for (int n = 0; n < 2; n++)  // (an infinite scale makes the rows that see it infinite; it must not set W)
+                if (fabsf(vv[sub][n]) < INFINITY) mv = fmaxf(mv, fabsf(vv[sub][n]));
+        move = mv > W;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                float x = -INFINITY;
+                float x = fmaxf(sc[nt][0][h], sc[nt][0][2 + h]);
 #pragma unroll
-                for (int sub = 0; sub < S::kSub; sub++)
-#pragma unroll
-                    for (int n = 0; n < 2; n++) x = fmaxf(x, fmaxf(sc[mt][sub][n][2 * h], sc[mt][sub][n][2 * h + 1]));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-                mx[mt][h] = fmaxf(m[mt][h], x * rf[mt][h]);
-                move |= mx[mt][h] > m[mt][h] + kLazy || (m[mt][h] == -INFINITY && mx[mt][h] != -INFINITY);
+                for (int sub = 1; sub < S::kSub; sub++) x = fmaxf(x, fmaxf(sc[nt][sub][h], sc[nt][sub][2 + h]));
+                mx[nt][h] = x * rf[nt][h];
+                move |= mx[nt][h] > m[nt][h] + kLazy;  // -inf + kLazy: any finite score moves the first maximum
             }
         if (__any_sync(0xffffffffu, move)) {
             float wf = 1.0f;
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) mv = fmaxf(mv, __shfl_xor_sync(0xffffffffu, mv, o));
             if (mv > W) {
                 const float w2 = pow2(min(exponent_of(mv) - 127 + 1, 127));
                 wf = W / w2;
                 W = w2;
             }
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
+            for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const float a = m[mt][h] == -INFINITY ? 0.0f : exp2_fast(m[mt][h] - mx[mt][h]);
-                    m[mt][h] = mx[mt][h];
-                    l[mt][h] *= a;
+                    float x = mx[nt][h];
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+                    x = fmaxf(m[nt][h], x);
+                    const float a = m[nt][h] == -INFINITY ? 0.0f : exp2_fast(m[nt][h] - x);
+                    m[nt][h] = x;
+                    l[nt][h] *= a;
                     const float f = a * wf;
 #pragma unroll
-                    for (int j = 0; j < NT; j++) {
-                        O[mt][j][2 * h] *= f;
-                        O[mt][j][2 * h + 1] *= f;
+                    for (int j = 0; j < KS; j++) {
+                        O[nt][j][h] *= f;
+                        O[nt][j][2 + h] *= f;
                     }
                 }
         }
         const float vf = kPScale / W;
 #pragma unroll
         for (int sub = 0; sub < S::kSub; sub++) {
-            uint4 P[MT][NP];
+            uint32_t P[PP][NT][2];  // [part][column tile][keys 0 .. 7, 8 .. 15]: the operand of the second product
+            const float w0 = vv[sub][0] * vf, w1 = vv[sub][1] * vf;
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                float pv[2][4];
+            for (int nt = 0; nt < NT; nt++) {
+                float pv[4];
 #pragma unroll
-                for (int n = 0; n < 2; n++)
+                for (int e = 0; e < 4; e++) {
+                    const float base = m[nt][e & 1] == -INFINITY ? 0.0f : m[nt][e & 1];
+                    const float x = exp2_fast(__fmaf_rn(sc[nt][sub][e], rf[nt][e & 1], -base));
+                    l[nt][e & 1] += x;
+                    pv[e] = x * (e < 2 ? w0 : w1);
+                }
+                if (tail) {  // a masked key's value scale may be anything: its weight is zero, not zero times that
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int h = e >> 1;
-                        const float base = m[mt][h] == -INFINITY ? 0.0f : m[mt][h];
-                        const float x = exp2_fast(__fmaf_rn(sc[mt][sub][n][e], rf[mt][h], -base));
-                        l[mt][h] += x;
-                        // a masked key's value scale may be anything: its weight is zero, not zero times that
-                        pv[n][e] = sc[mt][sub][n][e] == -INFINITY ? 0.0f : x * (vv[sub][n][e & 1] * vf);
-                    }
-                P[mt][0] = make_uint4(pack2<__half>(pv[0][0], pv[0][1]), pack2<__half>(pv[0][2], pv[0][3]),
-                                      pack2<__half>(pv[1][0], pv[1][1]), pack2<__half>(pv[1][2], pv[1][3]));
-                if (NP == 2) {
+                    for (int e = 0; e < 4; e++)
+                        if (sc[nt][sub][e] == -INFINITY) pv[e] = 0.0f;
+                }
+                P[0][nt][0] = transposed(pack2<__half>(pv[0], pv[1]));
+                P[0][nt][1] = transposed(pack2<__half>(pv[2], pv[3]));
+                if (PP == 2) {
 #pragma unroll
-                    for (int n = 0; n < 2; n++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) pv[n][e] -= __half2float(__float2half_rn(pv[n][e]));
-                    P[mt][NP - 1] = make_uint4(pack2<__half>(pv[0][0], pv[0][1]), pack2<__half>(pv[0][2], pv[0][3]),
-                                               pack2<__half>(pv[1][0], pv[1][1]), pack2<__half>(pv[1][2], pv[1][3]));
+                    for (int e = 0; e < 4; e++) pv[e] -= __half2float(__float2half_rn(pv[e]));
+                    P[PP - 1][nt][0] = transposed(pack2<__half>(pv[0], pv[1]));
+                    P[PP - 1][nt][1] = transposed(pack2<__half>(pv[2], pv[3]));
                 }
             }
-            // values: lane (r, c) takes elements NT * r .. of keys 2c, 2c + 1, 2c + 8, 2c + 9 of this piece
-            constexpr int WORDS = NT * BITS / 32;  // 32-bit words of a key's elements: 4, 2 (8 bits), 2, 1 (4 bits)
+            // values: lane (r, c) takes elements RUN * r .. of keys 2c, 2c + 1, 2c + 8, 2c + 9 of this piece
             uint32_t w[4][WORDS];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const uint8_t *src = vt + place<S::kRow>(sub * 16 + 2 * c + (k & 1) + 8 * (k >> 1), r * WORDS * 4);
+                const uint8_t *src = kt + (k & 1 ? v_at1 : v_at) + (sub * 16 + 8 * (k >> 1)) * S::kRow;
                 if constexpr (WORDS == 4) {
                     const uint4 u = *reinterpret_cast<const uint4 *>(src);
                     w[k][0] = u.x; w[k][1] = u.y; w[k][2] = u.z; w[k][3] = u.w;
@@ -367,8 +408,6 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 1 ? 2 : 1) tree_attention_k
                 } else {
                     w[k][0] = *reinterpret_cast<const uint32_t *>(src);
                 }
-#pragma unroll
-                for (int i = 0; i < WORDS; i++) w[k][i] ^= BITS == 8 ? 0x80808080u : 0x88888888u;
             }
 #pragma unroll
             for (int i = 0; i < WORDS; i++) {
@@ -376,16 +415,14 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 1 ? 2 : 1) tree_attention_k
                 uint32_t vb[PER][2];
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
+                    const uint32_t lo = __byte_perm(w[2 * h][i], w[2 * h + 1][i], 0x5410);
+                    const uint32_t hi = __byte_perm(w[2 * h][i], w[2 * h + 1][i], 0x7632);
                     if (BITS == 8) {
-                        const uint32_t lo = __byte_perm(w[2 * h][i], w[2 * h + 1][i], 0x5140);
-                        const uint32_t hi = __byte_perm(w[2 * h][i], w[2 * h + 1][i], 0x7362);
-                        vb[0][h] = bytes_to_half2(lo, 0x4140u);
-                        vb[1][h] = bytes_to_half2(lo, 0x4342u);
-                        vb[2][h] = bytes_to_half2(hi, 0x4140u);
-                        vb[3][h] = bytes_to_half2(hi, 0x4342u);
+                        vb[0][h] = bytes_to_half2(lo);
+                        vb[1][h] = bytes_to_half2(lo >> 8);
+                        vb[2][h] = bytes_to_half2(hi);
+                        vb[3][h] = bytes_to_half2(hi >> 8);
                     } else {
-                        const uint32_t lo = __byte_perm(w[2 * h][i], w[2 * h + 1][i], 0x5410);
-                        const uint32_t hi = __byte_perm(w[2 * h][i], w[2 * h + 1][i], 0x7632);
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
                             vb[k][h] = nibbles_to_half2(lo, k);
@@ -394,12 +431,14 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 1 ? 2 : 1) tree_attention_k
                     }
                 }
 #pragma unroll
-                for (int k = 0; k < PER; k++)
+                for (int k = 0; k < PER; k += 2) {  // element tile j: elements RUN * r + 2j (rows r), + 2j + 1 (rows r + 8)
+                    const uint4 a = make_uint4(vb[k][0], vb[k + 1][0], vb[k][1], vb[k + 1][1]);
 #pragma unroll
-                    for (int mt = 0; mt < MT; mt++)
+                    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                        for (int part = 0; part < NP; part++)
-                            mma16816(O[mt][PER * i + k], P[mt][part], vb[k][0], vb[k][1]);
+                        for (int part = 0; part < PP; part++)
+                            mma16816(O[nt][(PER * i + k) / 2], a, P[part][nt][0], P[part][nt][1]);
+                }
             }
         }
         __syncwarp();  // every lane has read the stage before the next turn refills it
@@ -412,25 +451,22 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 1 ? 2 : 1) tree_attention_k
     float *po = reinterpret_cast<float *>(pipe);  // [kWarps][ROWS][HDP]
     const float back = W / kPScale;
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++)
+    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            float sum = l[mt][h];
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            const int row = mt * 16 + r + 8 * h;
-            if (c == 0) {
-                warp_m[warp][row] = m[mt][h];
+            float sum = l[nt][h];
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            const int row = nt * 8 + 2 * c + h;
+            if (r == 0) {
+                warp_m[warp][row] = m[nt][h];
                 warp_l[warp][row] = sum;
             }
-            float *d = po + ((size_t)warp * ROWS + row) * HDP + NT * 2 * c;
+            float *d = po + ((size_t)warp * ROWS + row) * HDP + RUN * r;
 #pragma unroll
-            for (int e = 0; e < 2; e++)
-#pragma unroll
-                for (int j = 0; j < NT; j += 4)
-                    *reinterpret_cast<float4 *>(d + NT * e + j) =
-                        make_float4(O[mt][j][2 * h + e] * back, O[mt][j + 1][2 * h + e] * back,
-                                    O[mt][j + 2][2 * h + e] * back, O[mt][j + 3][2 * h + e] * back);
+            for (int j = 0; j < KS; j += 2)
+                *reinterpret_cast<float4 *>(d + 2 * j) = make_float4(O[nt][j][h] * back, O[nt][j][2 + h] * back,
+                                                                     O[nt][j + 1][h] * back, O[nt][j + 1][2 + h] * back);
         }
     __syncthreads();
     const int rows_here = min(ROWS, nrows - R0);
@@ -477,17 +513,24 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 1 ? 2 : 1) tree_attention_k
     // join the cluster: CTA `split` takes every splits-th piece, reading its sisters' shared memory in rank order
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
+    for (int i = threadIdx.x; i < p.splits * rows_here; i += kWarps * 32) {
+        const int w = i / rows_here, row = i - w * rows_here;
+        all_m[w][row] = *cluster.map_shared_rank(&cta_m[row], w);
+        all_l[w][row] = *cluster.map_shared_rank(&cta_l[row], w);
+    }
+    __syncthreads();
     for (int i = threadIdx.x * p.splits + split; i < rows_here * (HDP / 4); i += kWarps * 32 * p.splits) {
         const int row = i / (HDP / 4), d4 = i % (HDP / 4);
         float mm = -INFINITY;
-        for (int w = 0; w < p.splits; w++) mm = fmaxf(mm, *cluster.map_shared_rank(&cta_m[row], w));
+        for (int w = 0; w < p.splits; w++) mm = fmaxf(mm, all_m[w][row]);
         float sum = 0.0f;
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
         for (int w = 0; w < p.splits; w++) {
-            const float lw = *cluster.map_shared_rank(&cta_l[row], w);
-            if (lw == 0.0f) continue;
-            const float f = exp2_fast(*cluster.map_shared_rank(&cta_m[row], w) - mm);
             const float4 x = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(po + (size_t)row * HDP + 4 * d4, w));
+            const float lw = all_l[w][row];
+            if (lw == 0.0f) continue;
+            const float f = exp2_fast(all_m[w][row] - mm);
             sum += f * lw;
             o.x += f * x.x;
             o.y += f * x.y;
@@ -499,15 +542,15 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 1 ? 2 : 1) tree_attention_k
     cluster.sync();  // no CTA leaves while a sister reads its shared memory
 }
 
-template <typename T, int BITS, int HDP, int MT>
+template <typename T, int BITS, int HDP, int NT>
 static cudaError_t launch(AttnParams p, int max_len, cudaStream_t stream) {
     using S = Slice<HDP, BITS>;
-    constexpr int ROWS = 16 * MT, NP = sizeof(T) == 4 ? 2 : 1;
-    constexpr size_t frag = (size_t)NP * MT * (HDP / 16) * 512;
+    constexpr int ROWS = 8 * NT;
+    constexpr size_t frag = (size_t)Parts<T>::kQ * NT * (HDP / 16) * 256;
     constexpr size_t ring = (size_t)kWarps * S::kWarp + (size_t)ROWS * HDP * 4, join = (size_t)kWarps * ROWS * HDP * 4;
     constexpr size_t smem = frag + (ring > join ? ring : join);
-    static_assert(smem <= 227 * 1024 - 4096, "shared memory of a CTA");
-    auto kernel = tree_attention_kernel<T, BITS, HDP, MT>;
+    static_assert(smem <= 227 * 1024 - 8192, "shared memory of a CTA");
+    auto kernel = tree_attention_kernel<T, BITS, HDP, NT>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
@@ -533,11 +576,18 @@ static cudaError_t launch(AttnParams p, int max_len, cudaStream_t stream) {
     return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
+template <typename T, int BITS, int HDP>
+static cudaError_t launch_rows(const AttnParams &p, int max_len, cudaStream_t stream) {
+    const long long rows = (long long)p.max_new * p.group;
+    if (rows <= 8) return launch<T, BITS, HDP, 1>(p, max_len, stream);
+    if (rows <= 16) return launch<T, BITS, HDP, 2>(p, max_len, stream);
+    if (rows <= 24) return launch<T, BITS, HDP, 3>(p, max_len, stream);
+    return launch<T, BITS, HDP, 4>(p, max_len, stream);
+}
+
 template <typename T, int BITS>
 static cudaError_t launch_size(const AttnParams &p, int max_len, cudaStream_t stream) {
-    const bool wide = (long long)p.max_new * p.group > 16;
-    if (p.head <= 64) return wide ? launch<T, BITS, 64, 2>(p, max_len, stream) : launch<T, BITS, 64, 1>(p, max_len, stream);
-    return wide ? launch<T, BITS, 128, 2>(p, max_len, stream) : launch<T, BITS, 128, 1>(p, max_len, stream);
+    return p.head <= 64 ? launch_rows<T, BITS, 64>(p, max_len, stream) : launch_rows<T, BITS, 128>(p, max_len, stream);
 }
 
 int attn_take_error(cudaStream_t s) {

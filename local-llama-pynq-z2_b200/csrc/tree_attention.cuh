@@ -68,19 +68,18 @@ __device__ __forceinline__ float pow2(int k) { return __int_as_float((k + 127) <
 // Biased exponent of |x| (0 for zero and subnormals, 255 for infinities and NaN).
 __device__ __forceinline__ int exponent_of(float x) { return (__float_as_int(x) >> 23) & 255; }
 
-// Four int8 of a word, with the sign bits flipped by the caller (x ^ 0x80808080), as two exact half2: the byte in the
-// low mantissa of 1024 gives 1024 + (v + 128).
-__device__ __forceinline__ uint32_t bytes_to_half2(uint32_t x, uint32_t selector) {
-    uint32_t h;
-    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(h) : "r"(x), "r"(0x64646464u), "r"(selector));
+// Bytes 0 and 2 of a word (int8) as an exact half2: the byte with its sign bit flipped in the low mantissa of 1024 is
+// 1024 + (v + 128). One logic operation takes the bytes out, flips the signs and puts the exponents in.
+__device__ __forceinline__ uint32_t bytes_to_half2(uint32_t x) {
+    uint32_t h = (x & 0x00FF00FFu) ^ 0x64806480u;
     const uint32_t bias = 0x64806480u;  // 1152
     asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(h) : "r"(bias));
     return h;
 }
 
-// Nibbles k and k + 4 of a word, sign bits flipped (x ^ 0x88888888), as an exact half2: 1024 + (v + 8).
+// Nibbles k and k + 4 of a word (int4) as an exact half2: 1024 + (v + 8).
 __device__ __forceinline__ uint32_t nibbles_to_half2(uint32_t x, int k) {
-    uint32_t h = ((x >> (4 * k)) & 0x000F000Fu) | 0x64006400u;
+    uint32_t h = ((x >> (4 * k)) & 0x000F000Fu) ^ 0x64086408u;
     const uint32_t bias = 0x64086408u;  // 1032
     asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(h) : "r"(bias));
     return h;

@@ -22,20 +22,27 @@ device; they keep no state and use no workspace, so calls on several streams do 
 """
 import ctypes as C
 import math
+import sys
 from collections import namedtuple
 
-_TYPES = {}
+_TYPES = {}     # torch element types -> the library's codes; filled with _T, the torch module, by _torch()
+_T = None
+_raw_stream = None
 
 
 def _torch():
-    import torch
-    if not _TYPES:
+    """torch, imported at the first use (the package itself does not need it)."""
+    global _T, _raw_stream
+    if _T is None:
+        import torch
         _TYPES.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
-    return torch
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda index: torch.cuda.current_stream(index).cuda_stream)
+        _T = torch
+    return _T
 
 
 def _mvb():
-    import sys
     return sys.modules[__package__]
 
 
@@ -45,15 +52,16 @@ def _need(ok, message):
 
 
 def _call(name, device, stream, *args):
-    """One library call on `device` (made current for it) and `stream`."""
-    torch = _torch()
+    """One library call on `device` (made current for it) and `stream`. These calls take a few microseconds on the device
+    for a single token, so the host side is kept short: no formatted text before a check has failed, no stream object."""
     m = _mvb()
     f = getattr(m.lib(), name)
-    handle = (torch.cuda.current_stream(device) if stream is None else stream).cuda_stream
-    if torch.cuda.current_device() == device.index:
+    index = device.index
+    handle = _raw_stream(index) if stream is None else stream.cuda_stream
+    if _T.cuda.current_device() == index:
         rc = f(*args, handle)
     else:
-        with torch.cuda.device(device):
+        with _T.cuda.device(device):
             rc = f(*args, handle)
     if rc != 0:
         m.check(rc, name)
@@ -63,23 +71,26 @@ def _on(device, *tensors):
     for t in tensors:
         if t is not None and t.device != device:
             raise ValueError(f"tensors on {t.device} and {device}: one device is needed")
-    _need(device.type == "cuda", f"CUDA tensors are needed, not {device.type}")
+    if device.type != "cuda":
+        raise ValueError(f"CUDA tensors are needed, not {device.type}")
 
 
 def _rows(name, t, heads, head):
     """Checks a (rows, heads, head) tensor whose heads lie next to one another; its row stride."""
-    _need(t.dim() == 3 and (heads is None or t.shape[1] == heads) and (head is None or t.shape[2] == head),
-          f"{name} is {tuple(t.shape)}: (rows, {heads or 'heads'}, {head or 'head'}) is needed")
-    st = t.stride()
-    _need(st[2] == 1 and (st[1] == t.shape[2] or t.shape[1] == 1), f"{name}: the heads of a row must be contiguous")
-    _need(t.dtype in _TYPES, f"{name} is {t.dtype}: float32, bfloat16 or float16 is needed")
-    return st[0] if t.shape[0] > 1 else t.shape[1] * t.shape[2]  # a single row's stride says nothing
+    shape = t.shape
+    if len(shape) != 3 or (heads is not None and shape[1] != heads) or (head is not None and shape[2] != head):
+        raise ValueError(f"{name} is {tuple(shape)}: (rows, {heads or 'heads'}, {head or 'head'}) is needed")
+    s0, s1, s2 = t.stride()
+    if (s2 != 1 and shape[2] != 1) or (s1 != shape[2] and shape[1] != 1):
+        raise ValueError(f"{name}: the heads of a row must be contiguous")
+    if t.dtype not in _TYPES:
+        raise ValueError(f"{name} is {t.dtype}: float32, bfloat16 or float16 is needed")
+    return s0 if shape[0] > 1 else shape[1] * shape[2]  # a single row's stride says nothing
 
 
-def _int32(name, t, shape):
-    torch = _torch()
-    _need(t.dtype == torch.int32 and tuple(t.shape) == shape and t.is_contiguous(),
-          f"{name} is {t.dtype} {tuple(t.shape)}: contiguous int32 {shape} is needed")
+def _int32(name, t, *shape):
+    if t.dtype is not _T.int32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} is {t.dtype} {tuple(t.shape)}: contiguous int32 {shape} is needed")
 
 
 class KvCache:
@@ -89,22 +100,25 @@ class KvCache:
     __slots__ = ("kq", "ks", "vq", "vs", "pages", "kv_heads", "page", "head", "bits", "device", "args")
 
     def __init__(self, kq, ks, vq, vs):
-        torch = _torch()
-        _need(kq.dim() == 4 and kq.dtype in (torch.int8, torch.uint8),
-              "kq: (pages, kv_heads, page, head) int8, or uint8 with two elements a byte, is needed")
-        self.pages, self.kv_heads, self.page, width = kq.shape
-        self.bits = 8 if kq.dtype == torch.int8 else 4
-        self.head = width * 8 // self.bits
-        _need(vq.shape == kq.shape and vq.dtype == kq.dtype, "vq must be like kq")
-        for name, t in (("ks", ks), ("vs", vs)):
-            _need(t.shape == kq.shape[:3] and t.dtype == torch.float32, f"{name} must be float32 {tuple(kq.shape[:3])}")
-        for t in (kq, ks, vq, vs):
-            _need(t.is_contiguous(), "the cache's tensors must be contiguous")
-        self.device = kq.device
-        _on(self.device, ks, vq, vs)
+        torch = _T or _torch()
+        shape = kq.shape
+        self.bits = bits = {torch.int8: 8, torch.uint8: 4}.get(kq.dtype, 0)
+        if len(shape) != 4 or not bits:
+            raise ValueError("kq: (pages, kv_heads, page, head) int8, or uint8 with two elements a byte, is needed")
+        if vq.shape != shape or vq.dtype is not kq.dtype:
+            raise ValueError("vq must be like kq")
+        for t in (ks, vs):
+            if t.shape != shape[:3] or t.dtype is not torch.float32:
+                raise ValueError(f"ks and vs must be float32 {tuple(shape[:3])}")
+        if not (kq.is_contiguous() and vq.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+            raise ValueError("the cache's tensors must be contiguous")
+        self.device = device = kq.device
+        _on(device, ks, vq, vs)
         self.kq, self.ks, self.vq, self.vs = kq, ks, vq, vs
+        self.pages, self.kv_heads, self.page, width = shape
+        self.head = width if bits == 8 else 2 * width
         self.args = (kq.data_ptr(), ks.data_ptr(), vq.data_ptr(), vs.data_ptr(), self.pages, self.page, self.kv_heads,
-                     self.head, self.bits)
+                     self.head, bits)
 
     @classmethod
     def empty(cls, pages, kv_heads, page, head, bits=8, device="cuda"):
@@ -119,20 +133,22 @@ class KvCache:
 
 
 def _batch(cache, pages, cu, lens):
-    _need(pages.dim() == 2 and cu.dim() == 1 and lens.dim() == 1, "pages (batch, columns), cu and lens (vectors) are needed")
-    b = pages.shape[0]
-    _int32("pages", pages, (b, pages.shape[1]))
-    _int32("cu", cu, (b + 1,))
-    _int32("lens", lens, (b,))
-    _on(cache.device, pages, cu, lens)
-    return (pages.data_ptr(), pages.shape[1], cu.data_ptr(), lens.data_ptr(), b)
+    shape = pages.shape
+    if len(shape) != 2:
+        raise ValueError("pages: (batch, columns) is needed")
+    b, cols = shape
+    _int32("pages", pages, b, cols)
+    _int32("cu", cu, b + 1)
+    _int32("lens", lens, b)
+    return pages.data_ptr(), cols, cu.data_ptr(), lens.data_ptr(), b
 
 
 _LAYOUTS = {"half": 0, "pairs": 1}
 
 
 def _layout(layout):
-    _need(layout in _LAYOUTS, f"layout={layout!r}: 'half' or 'pairs' is needed")
+    if layout not in _LAYOUTS:
+        raise ValueError(f"layout={layout!r}: 'half' or 'pairs' is needed")
     return _LAYOUTS[layout]
 
 
@@ -166,6 +182,9 @@ def rope_table(frequencies, positions, out=None, start=0, factor=1.0, device="cu
     """(positions, rot) float32: row p holds factor * cos of the rot / 2 angles (start + p) * frequencies, then factor *
     sin, angles and functions in 64 bits. frequencies: float64, numpy or a CUDA tensor."""
     torch = _torch()
+    if stream is not None:  # what is made here belongs to the stream that uses it
+        with torch.cuda.stream(stream):
+            return rope_table(frequencies, positions, out, start, factor, device)
     if not torch.is_tensor(frequencies):
         frequencies = torch.as_tensor(frequencies, dtype=torch.float64, device=out.device if out is not None else device)
     _need(frequencies.dtype == torch.float64 and frequencies.dim() == 1 and frequencies.is_contiguous(),
@@ -176,36 +195,34 @@ def rope_table(frequencies, positions, out=None, start=0, factor=1.0, device="cu
     _need(out.dtype == torch.float32 and tuple(out.shape) == (positions, 2 * half) and out.is_contiguous(),
           f"out: contiguous float32 {(positions, 2 * half)} is needed")
     _on(out.device, frequencies)
-    if stream is not None:
-        for t in (out, frequencies):
-            t.record_stream(stream)
-    _call("mvb_rope_table", out.device, stream, frequencies.data_ptr(), out.data_ptr(), half, positions, start,
+    _call("mvb_rope_table", out.device, None, frequencies.data_ptr(), out.data_ptr(), half, positions, start,
           float(factor))
     return out
 
 
 def _table(table):
-    torch = _torch()
-    _need(table.dtype == torch.float32 and table.dim() == 2 and table.is_contiguous(),
-          "rope table: contiguous float32 (positions, rot) is needed")
+    if table.dtype is not _T.float32 or table.dim() != 2 or not table.is_contiguous():
+        raise ValueError("rope table: contiguous float32 (positions, rot) is needed")
+    return table.shape
 
 
 def rope(x, positions, table, out=None, layout="half", stream=None):
     """x (tokens, heads, head) with the first rot elements of each head turned by the table's row of the token's position;
     the other elements as they are. layout "half": pairs (i, i + rot / 2); "pairs": (2i, 2i + 1). out: x's shape and
     type, x itself for in place (the default); it must not overlap x otherwise."""
-    torch = _torch()
+    _T or _torch()
     out = x if out is None else out
     xs = _rows("x", x, None, None)
-    _, heads, head = x.shape
+    n, heads, head = x.shape
     os_ = _rows("out", out, heads, head)
-    _need(out.dtype == x.dtype and out.shape[0] == x.shape[0], "out must be like x")
-    _need(positions.dtype == torch.int32, "positions: int32 is needed")
-    _int32("positions", positions, (x.shape[0],))
-    _table(table)
-    _on(x.device, out, positions, table)
-    _call("mvb_rope", x.device, stream, x.data_ptr(), positions.data_ptr(), table.data_ptr(), out.data_ptr(),
-          _TYPES[x.dtype], x.shape[0], heads, head, table.shape[1], table.shape[0], _layout(layout), xs, os_)
+    if out.dtype is not x.dtype or out.shape[0] != n:
+        raise ValueError("out must be like x")
+    _int32("positions", positions, n)
+    reach, rot = _table(table)
+    device = x.device
+    _on(device, out, positions, table)
+    _call("mvb_rope", device, stream, x.data_ptr(), positions.data_ptr(), table.data_ptr(), out.data_ptr(),
+          _TYPES[x.dtype], n, heads, head, rot, reach, _layout(layout), xs, os_)
     return out
 
 
@@ -215,41 +232,46 @@ def kv_append(cache, k, v, pages, cu, lens, positions=None, rope=None, layout="h
     turned first (and q into q_out, rows of queries, in the same launch; q_out may be q) by the rows' `positions`
     (int32; default the position in the cache; a tree's are those of its depth). A row with an infinity or a NaN is held
     with the scale NaN. Sequences must not share a page that the call writes."""
-    torch = _torch()
-    _TYPES  # filled by _torch()
+    _T or _torch()
     ks, vs = _rows("k", k, cache.kv_heads, cache.head), _rows("v", v, cache.kv_heads, cache.head)
-    n = k.shape[0]
-    _need(v.shape[0] == n and v.dtype == k.dtype, "v must be like k")
+    n, dtype = k.shape[0], k.dtype
+    if v.shape[0] != n or v.dtype is not dtype:
+        raise ValueError("v must be like k")
     b = _batch(cache, pages, cu, lens)
-    _on(cache.device, k, v, positions, rope, q, q_out)
-    if positions is not None:
-        _int32("positions", positions, (n,))
-        _need(rope is not None, "positions without a rope table")
+    _on(cache.device, k, v, pages, cu, lens, positions, rope, q, q_out)
+    pos = table = qp = qop = None
+    reach = rot = qs = qos = heads = 0
     if rope is not None:
-        _table(rope)
-    qs = qos = heads = 0
+        reach, rot = _table(rope)
+        table = rope.data_ptr()
+    if positions is not None:
+        if rope is None:
+            raise ValueError("positions without a rope table")
+        _int32("positions", positions, n)
+        pos = positions.data_ptr()
     if q is not None:
-        _need(rope is not None and q_out is not None, "queries need a rope table and q_out")
-        qs, qos = _rows("q", q, None, cache.head), _rows("q_out", q_out, None, cache.head)
+        if rope is None or q_out is None:
+            raise ValueError("queries need a rope table and q_out")
         heads = q.shape[1]
-        _need(q.shape[0] == n and q_out.shape == q.shape and q.dtype == k.dtype and q_out.dtype == k.dtype,
-              "q and q_out must have k's rows and type")
-    _call("mvb_kv_append", cache.device, stream, *cache.args, *b, n, k.data_ptr(), ks, v.data_ptr(), vs, _TYPES[k.dtype],
-          None if rope is None else rope.data_ptr(), None if positions is None else positions.data_ptr(),
-          0 if rope is None else rope.shape[1], 0 if rope is None else rope.shape[0], _layout(layout),
-          None if q is None else q.data_ptr(), qs, None if q is None else q_out.data_ptr(), qos, heads)
+        qs, qos = _rows("q", q, None, cache.head), _rows("q_out", q_out, heads, cache.head)
+        if q.shape[0] != n or q_out.shape[0] != n or q.dtype is not dtype or q_out.dtype is not dtype:
+            raise ValueError("q and q_out must have k's rows and type")
+        qp, qop = q.data_ptr(), q_out.data_ptr()
+    _call("mvb_kv_append", cache.device, stream, *cache.args, *b, n, k.data_ptr(), ks, v.data_ptr(), vs, _TYPES[dtype],
+          table, pos, rot, reach, _layout(layout), qp, qs, qop, qos, heads)
 
 
 def kv_read(cache, pages, cu, lens, k_out, v_out, stream=None):
     """Cached keys and values back: rows cu[b] .. cu[b + 1] - 1 of k_out and v_out (rows, kv_heads, head; float32,
     bfloat16 or float16) become sequence b's positions lens[b] and on (lens of zeros and cu of running lengths: whole
     contexts). integer * scale, rounded to the output's type."""
-    _torch()
+    _T or _torch()
     ks, vs = _rows("k_out", k_out, cache.kv_heads, cache.head), _rows("v_out", v_out, cache.kv_heads, cache.head)
     n = k_out.shape[0]
-    _need(v_out.shape[0] == n and v_out.dtype == k_out.dtype, "v_out must be like k_out")
+    if v_out.shape[0] != n or v_out.dtype is not k_out.dtype:
+        raise ValueError("v_out must be like k_out")
     b = _batch(cache, pages, cu, lens)
-    _on(cache.device, k_out, v_out)
+    _on(cache.device, k_out, v_out, pages, cu, lens)
     _call("mvb_kv_read", cache.device, stream, *cache.args, *b, n, k_out.data_ptr(), ks, v_out.data_ptr(), vs,
           _TYPES[k_out.dtype])
 
@@ -270,7 +292,7 @@ def tree_mask(parents):
         bits[has, i] = bits[has, flat[has, i]]
         bits[:, i, i] = True
     words = np.packbits(bits, axis=-1, bitorder="little").view("<i8")
-    words = torch.from_numpy(words.reshape(*p.shape, -1).copy())
+    words = torch.from_numpy(words.reshape(*p.shape, bits.shape[-1] // 64).copy())
     return words.to(parents.device) if torch.is_tensor(parents) else words
 
 
@@ -283,25 +305,26 @@ def tree_attention(q, cache, pages, cu, lens, out, tree=None, scale=None, max_ne
     skipped and reported. max_len: about the longest lens[b] + new tokens (default: the page table's reach), which only
     decides how finely the work is split. lse (rows, heads) float32: the log of the sum of exponentials. A row that may
     see nothing gives zeros and lse -inf."""
-    torch = _torch()
+    _T or _torch()
     qs, os_ = _rows("q", q, None, cache.head), _rows("out", out, None, cache.head)
-    n, heads, head = q.shape
-    _need(out.shape == q.shape and out.dtype == q.dtype, "out must be like q")
+    n, heads, head = shape = q.shape
+    dtype = q.dtype
+    if out.shape != shape or out.dtype is not dtype:
+        raise ValueError("out must be like q")
     b = _batch(cache, pages, cu, lens)
-    _on(cache.device, q, out, tree, lse)
-    words = 0
+    _on(cache.device, q, out, pages, cu, lens, tree, lse)
+    words, tp, lp = 0, None, None
     if tree is not None:
-        _need(tree.dtype == torch.int64 and tree.dim() == 2 and tree.shape[0] == n and tree.is_contiguous(),
-              f"tree: contiguous int64 ({n}, words) is needed")
-        words = tree.shape[1]
+        if tree.dtype is not _T.int64 or tree.dim() != 2 or tree.shape[0] != n or not tree.is_contiguous():
+            raise ValueError(f"tree: contiguous int64 ({n}, words) is needed")
+        words, tp = tree.shape[1], tree.data_ptr()
     if lse is not None:
-        _need(lse.dtype == torch.float32 and tuple(lse.shape) == (n, heads) and lse.is_contiguous(),
-              f"lse: contiguous float32 {(n, heads)} is needed")
-    reach = pages.shape[1] * cache.page
-    _call("mvb_tree_attention", cache.device, stream, q.data_ptr(), qs, *cache.args, *b, n, heads, _TYPES[q.dtype],
-          None if tree is None else tree.data_ptr(), words, 1.0 / math.sqrt(head) if scale is None else float(scale),
-          n if max_new is None else max_new, reach if max_len is None else max_len, out.data_ptr(), os_,
-          None if lse is None else lse.data_ptr())
+        if lse.dtype is not _T.float32 or lse.shape != (n, heads) or not lse.is_contiguous():
+            raise ValueError(f"lse: contiguous float32 {(n, heads)} is needed")
+        lp = lse.data_ptr()
+    _call("mvb_tree_attention", cache.device, stream, q.data_ptr(), qs, *cache.args, *b, n, heads, _TYPES[dtype], tp, words,
+          head ** -0.5 if scale is None else float(scale), n if max_new is None else max_new,
+          b[1] * cache.page if max_len is None else max_len, out.data_ptr(), os_, lp)
     return out
 
 
@@ -314,38 +337,41 @@ def logprobs(logits, ids=None, top=0, entropy=True, stream=None):
     logits by the lowest id. Returns LogProbs(logp (rows, n), entropy (rows), top_ids (rows, top) int32, top_logp (rows,
     top)); what was not asked for is None or has no columns. A row that holds a NaN or +inf, or no finite logit, is all
     NaN (its top ids still order the logits, NaN last)."""
-    torch = _torch()
-    _need(logits.dim() == 2 and logits.dtype in _TYPES, "logits: (rows, vocab) float32, bfloat16 or float16 is needed")
+    torch = _T or _torch()
+    if logits.dim() != 2 or logits.dtype not in _TYPES:
+        raise ValueError("logits: (rows, vocab) float32, bfloat16 or float16 is needed")
     n, vocab = logits.shape
-    _need(logits.stride(1) == 1 or vocab == 1, "logits: the elements of a row must be contiguous")
+    stride, one = logits.stride()
+    if one != 1 and vocab != 1:
+        raise ValueError("logits: the elements of a row must be contiguous")
     dev = logits.device
-    nids = 0
-    if ids is not None:
-        _need(ids.dim() == 2 and ids.shape[0] == n, f"ids: ({n}, count) is needed")
-        _int32("ids", ids, tuple(ids.shape))
-        nids = ids.shape[1]
     _on(dev, ids)
-    with torch.cuda.stream(stream) if stream is not None else _NOTHING:
-        logp = torch.empty(n, nids, device=dev) if ids is not None else None
-        ent = torch.empty(n, device=dev) if entropy else None
-        top_ids = torch.empty(n, top, dtype=torch.int32, device=dev)
-        top_logp = torch.empty(n, top, device=dev)
-    _call("mvb_logprobs", dev, stream, logits.data_ptr(), logits.stride(0), _TYPES[logits.dtype], n, vocab,
-          ids.data_ptr() if nids else None, nids, logp.data_ptr() if nids else None,
-          None if ent is None else ent.data_ptr(), top, top_ids.data_ptr() if top else None,
-          top_logp.data_ptr() if top else None)
-    return LogProbs(logp, ent, top_ids, top_logp)
+    nids, ip = 0, None
+    if ids is not None:
+        if ids.dim() != 2:
+            raise ValueError(f"ids: ({n}, count) is needed")
+        nids = ids.shape[1]
+        _int32("ids", ids, n, nids)
+        ip = ids.data_ptr() if nids else None
+    if stream is None:
+        out = _results(torch, dev, n, nids, top, ids is not None, entropy)
+    else:  # memory of the stream that writes it
+        with torch.cuda.stream(stream):
+            out = _results(torch, dev, n, nids, top, ids is not None, entropy)
+    logp, ent, top_ids, top_logp = out
+    _call("mvb_logprobs", dev, stream, logits.data_ptr(), stride, _TYPES[logits.dtype], n, vocab, ip, nids,
+          logp.data_ptr() if nids else None, ent.data_ptr() if entropy else None, top,
+          top_ids.data_ptr() if top else None, top_logp.data_ptr() if top else None)
+    return out
 
 
-class _Nothing:
-    def __enter__(self):
-        return None
+def _results(torch, dev, n, nids, top, has_ids, entropy):
+    f32 = torch.float32
+    return LogProbs(torch.empty((n, nids), dtype=f32, device=dev) if has_ids else None,
+                    torch.empty((n,), dtype=f32, device=dev) if entropy else None,
+                    torch.empty((n, top), dtype=torch.int32, device=dev),
+                    torch.empty((n, top), dtype=f32, device=dev))
 
-    def __exit__(self, *a):
-        return False
-
-
-_NOTHING = _Nothing()
 
 #: what serve_status() returns
 STATUS = {0: "ok", 1: "a page number out of range", 2: "a length or a row range out of range",

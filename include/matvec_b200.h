@@ -246,7 +246,8 @@ int mvb_logprobs(const void *x, long long stride, int dtype, int rows, int vocab
                  float *entropy, int top, int *top_ids, float *top_logp, void *stream);
 
 /* Synchronizes `stream`; 0, or what the serving operators found out of range since the last call, and clears it: 1 a page
- * number, 2 a length or row range, 3 a rotary position, 4 a token id; -1 if the stream failed. */
+ * number, 2 a length or row range, 3 a rotary position, 4 a token id, 5 a wait inside a kernel that gave up;
+ * -1 if the stream failed. */
 int mvb_serve_status(void *stream);
 
 /* ---- Row-sharded matvec with the all-gather fused into the kernel (one process per GPU, NVLink peers) ----

@@ -7,8 +7,10 @@
 // have to be scaled group by group).
 //     scale = fl32(max |x| / Q), Q = 127 or 7;   integer = rint(x / scale), ties to even;   value = integer * scale
 // x is the rotated key in fp64 (the products of an fp32 element with an fp32 cosine are exact there, so each element is
-// rounded once), or the value itself: an integer next to a border comes out the same for every order of evaluation. A row
-// with an infinity or a NaN gets the scale NaN and reads back as NaN. All-zero rows have scale 0.
+// rounded once), or the value itself: an integer next to a border comes out the same for every order of evaluation. The
+// work is done in fp32 all the same: only the elements that may hold the row's maximum, and those within 1e-4 of a border
+// (1 in 5,000), are computed in fp64. A row that has an infinity or a NaN (after the rotation in fp32) gets the scale NaN
+// and reads back as NaN. All-zero rows have scale 0.
 #include <limits.h>
 
 #include "../../include/matvec_b200.h"
@@ -32,64 +34,111 @@ struct KvParams {
     const float *rope;
     long long q_stride, k_stride, v_stride, q_out_stride;
     int heads, rot, table_rows, pairs;
-    int kv_per, kv_chunks, q_per, chunks;
+    int kv_chunks, q_per, chunks;
     // read
     void *k_out, *v_out;
     long long k_out_stride, v_out_stride;
     int tokens_per_block;
 };
 
-// rint(x / scale), |.| <= MOST. y = x * (1 / scale) in fp32 is within 127 * 3 * 2^-24 < 2.3e-5 of the quotient, which
-// decides all but the values within 1e-4 of a border; those (1 in 5,000) take the fp64 quotient, as do scales whose
-// reciprocal leaves fp32's range.
-template <int MOST>
-__device__ __forceinline__ int quantized(double x, float xf, float scale, float inv) {
-    const float y = __fmul_rn(xf, inv);
-    float n = rintf(y);
-    if (scale < 1e-36f || fabsf(fabsf(__fsub_rn(y, n)) - 0.5f) < 1e-4f) {
-        if (!(scale > 0.0f)) return 0;
-        n = (float)rint(__ddiv_rn(x, (double)scale));
+// One element before quantization: x itself, or x c + y s (a turned key), in fp64 (rounded once: both products are exact).
+struct Exact {
+    float x, y, c, s;
+    bool turn;
+    __device__ __forceinline__ double value() const {
+        return turn ? __fma_rn((double)x, (double)c, __dmul_rn((double)y, (double)s)) : (double)x;
     }
-    return max(-MOST, min(MOST, (int)n));
+};
+
+// rint(x / scale) in fp64, at most MOST.
+template <int MOST>
+__device__ __noinline__ float quotient(double x, float scale) {
+    if (!(scale > 0.0f)) return 0.0f;
+    return (float)fmin(fmax(rint(__ddiv_rn(x, (double)scale)), -(double)MOST), (double)MOST);
 }
 
-// Quantizes the rows of a warp (W lanes a row, four elements a lane) and stores integers and scale. x in fp64; every lane
-// of the warp takes part; lanes with on = false hold zeros and store nothing.
-template <int W, int BITS>
-__device__ __forceinline__ void quantize_store(const double (&x)[4], bool on, int l, uint8_t *row, float *scale_at) {
+// Quantizes the rows of a warp (W lanes a row, E elements a lane) and stores integers and scale. f: the elements in fp32
+// (with TURN, turned keys within 1.5 ulp of the larger product, else the elements themselves); exact(k): element k in
+// fp64. Every lane of the warp takes part; lanes with on = false hold zeros and store nothing.
+//
+// scale: of turned keys, |f| finds the candidates for the largest element (within 1e-6 of the largest, which covers f's
+// error; nearly always one lane of the row), their fp64 values decide; rounding to fp32 is monotonic, so the largest of the
+// rounded quotients is the rounded largest quotient. (The fp32 division rounds the quotient of an fp32 element as the
+// fp64 one followed by a rounding does: 53 bits are enough for that.)
+// integers: y = f * (1 / scale) is within 127 * 2^-21 < 6.1e-5 of x / scale, which decides all but the values within 1e-4
+// of a border; those take the fp64 quotient, as do scales whose reciprocal leaves fp32's range. Adding 1.5 * 2^23 rounds y
+// to an integer (ties to even) that stands in the sum's low byte.
+template <int W, int BITS, bool TURN, int E, typename F>
+__device__ __forceinline__ void quantize_store(const Row<E> &f, const F &exact, bool on, int l, uint8_t *row,
+                                               float *scale_at) {
     constexpr int MOST = BITS == 8 ? 127 : 7;
-    double m = fmax(fmax(fabs(x[0]), fabs(x[1])), fmax(fabs(x[2]), fabs(x[3])));
-    // x - x is 0 for finite x, NaN else
-    bool bad = !((x[0] - x[0]) + (x[1] - x[1]) + (x[2] - x[2]) + (x[3] - x[3]) == 0.0);
+    uint32_t mine = 0;  // |f| as bits: infinities and NaN come out largest
 #pragma unroll
-    for (int o = W / 2; o; o >>= 1) {
-        m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
-        bad |= (bool)__shfl_xor_sync(0xffffffffu, (int)bad, o);
+    for (int k = 0; k < E; k++) mine = max(mine, __float_as_uint(f.v[k]) & 0x7FFFFFFFu);
+    uint32_t mb = mine;
+#pragma unroll
+    for (int o = W / 2; o; o >>= 1) mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, o));
+    const bool bad = mb >= 0x7F800000u;
+    const float m = __uint_as_float(mb);
+    float scale;
+    if (TURN) {
+        const float near = m - fmaxf(m * 1e-6f, 1e-44f);
+        scale = 0.0f;
+        if (__uint_as_float(mine) >= near) {
+            double best = 0.0;
+#pragma unroll
+            for (int k = 0; k < E; k++) best = fmax(best, fabs(exact(k)));
+            scale = best > 0.0 ? __double2float_rn(__ddiv_rn(best, (double)MOST)) : 0.0f;
+        }
+#pragma unroll
+        for (int o = W / 2; o; o >>= 1) scale = fmaxf(scale, __shfl_xor_sync(0xffffffffu, scale, o));
+    } else {
+        scale = __fdiv_rn(m, (float)MOST);
     }
-    float scale = __double2float_rn(__ddiv_rn(m, (double)MOST));
     const float inv = __frcp_rn(scale);
-    int n[4];
+    uint32_t n[E];
+    float far = scale >= 1e-36f ? 0.0f : 1.0f;  // the largest distance from an integer
 #pragma unroll
-    for (int k = 0; k < 4; k++) n[k] = bad ? 0 : quantized<MOST>(x[k], __double2float_rn(x[k]), scale, inv);
+    for (int k = 0; k < E; k++) {
+        const float y = __fmul_rn(f.v[k], inv), t = __fadd_rn(y, 12582912.0f);
+        far = fmaxf(far, fabsf(__fsub_rn(y, __fsub_rn(t, 12582912.0f))));
+        n[k] = __float_as_uint(t);
+    }
+    if (far > 0.4999f && !bad) {
+#pragma unroll
+        for (int k = 0; k < E; k++) n[k] = __float_as_uint(__fadd_rn(quotient<MOST>(exact(k), scale), 12582912.0f));
+    }
     if (!on) return;
-    if (BITS == 8)
-        *reinterpret_cast<uint32_t *>(row + 4 * l) =
-            (n[0] & 255) | (n[1] & 255) << 8 | (n[2] & 255) << 16 | (uint32_t)n[3] << 24;
-    else
-        *reinterpret_cast<uint16_t *>(row + 2 * l) =
-            (uint16_t)((n[0] & 15) | (n[1] & 15) << 4 | (n[2] & 15) << 8 | (n[3] & 15) << 12);
+    if (BITS == 8) {
+        uint32_t w[E / 4];
+#pragma unroll
+        for (int k = 0; k < E; k += 4)
+            w[k / 4] = __byte_perm(__byte_perm(n[k], n[k + 1], 0x0040), __byte_perm(n[k + 2], n[k + 3], 0x0040), 0x5410);
+        if (bad) w[0] = w[E / 4 - 1] = 0;
+        if constexpr (E == 8) *reinterpret_cast<uint2 *>(row + 8 * l) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<uint32_t *>(row + 4 * l) = w[0];
+    } else {
+        uint32_t w = 0;
+#pragma unroll
+        for (int k = 0; k < E; k++) w |= (n[k] & 15) << (4 * k);
+        if (bad) w = 0;
+        if constexpr (E == 8) *reinterpret_cast<uint32_t *>(row + 4 * l) = w;
+        else *reinterpret_cast<uint16_t *>(row + 2 * l) = (uint16_t)w;
+    }
     if (l == 0) *scale_at = bad ? __int_as_float(0x7FC00000) : scale;
 }
 
-// One warp: some heads' keys and values of one token into the cache, or some heads of its queries rotated.
-template <typename T, int W, int BITS>
-__global__ void __launch_bounds__(256) kv_append_kernel(const KvParams p) {
+// One warp: 32 / W heads' keys and values of one token into the cache, or some heads of its queries rotated.
+template <typename T, int W, int BITS, int E>
+__global__ void __launch_bounds__(256, 3) kv_append_kernel(const KvParams p) {
     constexpr int R = 32 / W;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane & (W - 1), sub = lane / W;
     const long long item = (long long)blockIdx.x * 8 + warp;
-    const int tok = (int)(item / p.chunks), chunk = (int)(item - (long long)tok * p.chunks);
-    if (tok >= p.rows || tok >= p.bt.cu[p.bt.batch]) return;  // rows behind the last sequence stay as they are
-    const bool on = 4 * l < p.head;
+    // chunk by chunk, so that the warps of a block do alike work (a block of both kinds keeps its queries' warps waiting
+    // idle for those that quantize: 14,000 rows of 32 + 8 heads took 179 us so)
+    const int chunk = (int)(item / p.rows), tok = (int)(item - (long long)chunk * p.rows);
+    if (chunk >= p.chunks || tok >= p.bt.cu[p.bt.batch]) return;  // rows behind the last sequence stay as they are
+    const bool on = E * l < p.head, in_rot = E * l < p.rot;
     const bool is_q = chunk >= p.kv_chunks;
     int b = 0;
     long long at = 0;
@@ -98,87 +147,56 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvParams p) {
         if (b >= p.bt.batch) return;
         at = (long long)p.bt.lens[b] + tok - p.bt.cu[b];
     }
-    Turn t;
-    t.c = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-    t.s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    Turn<E> t;
+#pragma unroll
+    for (int k = 0; k < E; k++) t.c[k] = 1.0f, t.s[k] = 0.0f;
     if (p.rope) {
         const long long pos = p.pos ? p.pos[tok] : at;
         if (pos < 0 || pos >= p.table_rows) {
             if (lane == 0) note(&g_kv_error, kBadPosition);
             return;
         }
-        if (on) t = load_turn(p.rope + pos * p.rot, l, p.rot, p.pairs);
+        t = load_turn<E>(p.rope + pos * p.rot, l, p.rot, p.pairs);
     }
     if (is_q) {
-        const int h0 = (chunk - p.kv_chunks) * p.q_per, h1 = min(h0 + p.q_per, p.heads);
-        const T *x = static_cast<const T *>(p.q) + tok * p.q_stride + 4 * l;
-        T *out = static_cast<T *>(p.q_out) + tok * p.q_out_stride + 4 * l;
-        constexpr int U = 4;
-        for (int h = h0; h < h1; h += U * R) {
-            float4 v[U];
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int hh = h + u * R + sub;
-                v[u] = on && hh < h1 ? load4(x + (size_t)hh * p.head) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            }
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int hh = h + u * R + sub;
-                const float4 y = partners<W>(v[u], l, p.rot, p.pairs);
-                if (on && hh < h1) store4(out + (size_t)hh * p.head, turned(v[u], y, t, l, p.rot, p.pairs));
-            }
-        }
+        const int h0 = (chunk - p.kv_chunks) * p.q_per;
+        turn_heads<W, E>(static_cast<const T *>(p.q) + tok * p.q_stride + E * l,
+                         static_cast<T *>(p.q_out) + tok * p.q_out_stride + E * l, h0, min(h0 + p.q_per, p.heads), p.head,
+                         t, l, sub, p.rot, p.pairs);
         return;
     }
+    const int h = chunk * R + sub;
+    const bool live = on && h < p.kv_heads;
+    const size_t src = (size_t)h * p.head + E * l;
+    const Row<E> k = load_row<E>(static_cast<const T *>(p.k) + tok * p.k_stride + src, live);
+    const Row<E> v = load_row<E>(static_cast<const T *>(p.v) + tok * p.v_stride + src, live);
     const long long slot = at > INT_MAX ? -1 : slot_of(p.bt, b, (int)at, &g_kv_error);
     if (slot < 0) return;
-    const int mask = (1 << p.bt.page_log2) - 1;
     const size_t page = (size_t)(slot >> p.bt.page_log2);
+    const size_t row = ((page * p.kv_heads + min(h, p.kv_heads - 1)) << p.bt.page_log2) +
+                       (size_t)(slot & ((1 << p.bt.page_log2) - 1));
     const int row_bytes = p.head * BITS / 8;
-    const int h0 = chunk * p.kv_per, h1 = min(h0 + p.kv_per, p.kv_heads);
-    for (int h = h0; h < h1; h += R) {
-        const int hh = h + sub;
-        const bool live = on && hh < h1;
-        const float4 z = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const float4 kf =
-            live ? load4(static_cast<const T *>(p.k) + tok * p.k_stride + (size_t)hh * p.head + 4 * l) : z;
-        const float4 vf =
-            live ? load4(static_cast<const T *>(p.v) + tok * p.v_stride + (size_t)hh * p.head + 4 * l) : z;
-        const size_t row = ((page * p.kv_heads + min(hh, p.kv_heads - 1)) << p.bt.page_log2) + (slot & mask);
-        double x[4] = {kf.x, kf.y, kf.z, kf.w};
-        if (p.rope) {
-            const float4 y = partners<W>(kf, l, p.rot, p.pairs);
-            if (4 * l < p.rot) {
-                const float yv[4] = {y.x, y.y, y.z, y.w}, c[4] = {t.c.x, t.c.y, t.c.z, t.c.w},
-                            s[4] = {t.s.x, t.s.y, t.s.z, t.s.w};
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const double bs = __dmul_rn((double)yv[k], (double)s[k]);  // exact: 24 + 24 bits
-                    x[k] = __fma_rn(x[k], (double)c[k], is_first(k, l, p.rot, p.pairs) ? -bs : bs);
-                }
-            }
-        }
-        quantize_store<W, BITS>(x, live, l, p.kq + row * row_bytes, p.ks + row);
-        const double xv[4] = {vf.x, vf.y, vf.z, vf.w};
-        quantize_store<W, BITS>(xv, live, l, p.vq + row * row_bytes, p.vs + row);
-    }
+    quantize_store<W, BITS, false>(v, [&](int i) { return (double)v.v[i]; }, live, l, p.vq + row * row_bytes, p.vs + row);
+    const Row<E> y = p.rope ? partners<W>(k, l, p.rot, p.pairs) : k;
+    const Row<E> f = p.rope ? turned(k, y, t, in_rot) : k;
+    auto exact = [&](int i) { return Exact{k.v[i], y.v[i], t.c[i], t.s[i], p.rope && in_rot}.value(); };
+    if (p.rope) quantize_store<W, BITS, true>(f, exact, live, l, p.kq + row * row_bytes, p.ks + row);
+    else quantize_store<W, BITS, false>(f, exact, live, l, p.kq + row * row_bytes, p.ks + row);
 }
 
 // Eight elements of a cached row (integer * scale, rounded once to fp32, once more to a 16-bit output).
 template <typename T, int BITS>
-__device__ __forceinline__ void read8(const uint8_t *src, float scale, T *dst) {
+__device__ __forceinline__ void write8(uint2 u, float scale, T *dst) {
     int n[8];
     if (BITS == 8) {
-        const uint2 u = *reinterpret_cast<const uint2 *>(src);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             n[k] = (int8_t)(u.x >> (8 * k));
             n[4 + k] = (int8_t)(u.y >> (8 * k));
         }
     } else {
-        const uint32_t u = *reinterpret_cast<const uint32_t *>(src);
 #pragma unroll
-        for (int k = 0; k < 8; k++) n[k] = (int)(u << (28 - 4 * k)) >> 28;
+        for (int k = 0; k < 8; k++) n[k] = (int)(u.x << (28 - 4 * k)) >> 28;
     }
     float f[8];
 #pragma unroll
@@ -193,8 +211,9 @@ __device__ __forceinline__ void read8(const uint8_t *src, float scale, T *dst) {
 }
 
 // One block: the cached rows of some tokens, every head. The tokens' slots are looked up once, a thread each; then W
-// lanes (eight elements a lane) copy a (token, head) row of keys and of values.
+// lanes (eight elements a lane) copy a (token, head) row of keys and of values, kDeep rows in flight.
 constexpr int kReadTokens = 32;  // tokens a block at most
+constexpr int kDeep = 4;
 
 template <typename T, int W, int BITS>
 __global__ void __launch_bounds__(256) kv_read_kernel(const KvParams p) {
@@ -222,25 +241,56 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvParams p) {
     const int l = tid & (W - 1), units = nt * p.kv_heads, mask = (1 << p.bt.page_log2) - 1;
     const int row_bytes = p.head * BITS / 8;
     if (8 * l >= p.head) return;
-#pragma unroll 4
-    for (int u = tid / W; u < units; u += 256 / W) {
-        const int ti = u / p.kv_heads, h = u - ti * p.kv_heads;
-        const long long slot = slots[ti];
-        if (slot < 0) continue;
-        const size_t row =
-            (((size_t)(slot >> p.bt.page_log2) * p.kv_heads + h) << p.bt.page_log2) + (size_t)(slot & mask);
-        const size_t o = (size_t)h * p.head + 8 * l;
-        read8<T, BITS>(p.kq + row * row_bytes + l * BITS, p.ks[row],
-                       static_cast<T *>(p.k_out) + (t0 + ti) * p.k_out_stride + o);
-        read8<T, BITS>(p.vq + row * row_bytes + l * BITS, p.vs[row],
-                       static_cast<T *>(p.v_out) + (t0 + ti) * p.v_out_stride + o);
+    for (int u0 = tid / W; u0 < units; u0 += kDeep * (256 / W)) {
+        uint2 kw[kDeep], vw[kDeep];
+        float ks[kDeep], vs[kDeep];
+        bool live[kDeep];
+        int ti[kDeep], h[kDeep];
+#pragma unroll
+        for (int i = 0; i < kDeep; i++) {
+            const int u = u0 + i * (256 / W);
+            ti[i] = u / p.kv_heads;
+            h[i] = u - ti[i] * p.kv_heads;
+            const long long slot = u < units ? slots[ti[i]] : -1;
+            live[i] = slot >= 0;
+            if (!live[i]) continue;
+            const size_t row =
+                (((size_t)(slot >> p.bt.page_log2) * p.kv_heads + h[i]) << p.bt.page_log2) + (size_t)(slot & mask);
+            const uint8_t *kp = p.kq + row * row_bytes + l * BITS, *vp = p.vq + row * row_bytes + l * BITS;
+            if (BITS == 8) {
+                kw[i] = *reinterpret_cast<const uint2 *>(kp);
+                vw[i] = *reinterpret_cast<const uint2 *>(vp);
+            } else {
+                kw[i].x = *reinterpret_cast<const uint32_t *>(kp);
+                vw[i].x = *reinterpret_cast<const uint32_t *>(vp);
+            }
+            ks[i] = p.ks[row];
+            vs[i] = p.vs[row];
+        }
+#pragma unroll
+        for (int i = 0; i < kDeep; i++) {
+            if (!live[i]) continue;
+            const size_t o = (size_t)h[i] * p.head + 8 * l;
+            write8<T, BITS>(kw[i], ks[i], static_cast<T *>(p.k_out) + (t0 + ti[i]) * p.k_out_stride + o);
+            write8<T, BITS>(vw[i], vs[i], static_cast<T *>(p.v_out) + (t0 + ti[i]) * p.v_out_stride + o);
+        }
     }
 }
 
+template <typename T, int BITS, int E>
+static void launch_lanes(const KvParams &p, unsigned grid, cudaStream_t s) {
+    const int lanes = (p.head + E - 1) / E;  // the fewest lanes that hold a row
+    if (lanes <= 8) kv_append_kernel<T, 8, BITS, E><<<grid, 256, 0, s>>>(p);
+    else if (lanes <= 16) kv_append_kernel<T, 16, BITS, E><<<grid, 256, 0, s>>>(p);
+    else kv_append_kernel<T, 32, BITS, E><<<grid, 256, 0, s>>>(p);
+}
+
 template <typename T, int BITS>
-static void launch_append(const KvParams &p, unsigned grid, cudaStream_t s) {
-    if (p.head <= 64) kv_append_kernel<T, 16, BITS><<<grid, 256, 0, s>>>(p);
-    else kv_append_kernel<T, 32, BITS><<<grid, 256, 0, s>>>(p);
+static void launch_append(const KvParams &p, unsigned grid, bool wide, cudaStream_t s) {
+    if constexpr (sizeof(T) == 2) {
+        if (wide) return launch_lanes<T, BITS, 8>(p, grid, s);
+    }
+    launch_lanes<T, BITS, 4>(p, grid, s);
 }
 
 template <typename T, int BITS>
@@ -347,13 +397,16 @@ extern "C" int mvb_kv_append(void *kq, float *ks, void *vq, float *vs, int pages
     p.table_rows = table_rows;
     p.pairs = layout;
     p.heads = q ? heads : 0;
-    // one pass of a warp a chunk for small calls (latency), more heads a warp where the machine is full anyway (the
-    // sequence, page and table look-ups are then made once for them)
-    const int r = head <= 64 ? 2 : 1;
-    const bool full = (long long)rows * (kv_heads + p.heads) >= 148ll * 64 * 4 * r;
-    p.kv_per = full ? 4 * r : r;
+    // 16 bytes a lane where everything is a multiple of that
+    bool wide = dtype != kF32 && (!rope || rot % 16 == 0) && k_stride % 8 == 0 && v_stride % 8 == 0 &&
+                !(((uintptr_t)k | (uintptr_t)v) & 15);
+    if (q) wide = wide && q_stride % 8 == 0 && q_out_stride % 8 == 0 && !(((uintptr_t)q | (uintptr_t)q_out) & 15);
+    const int lane_elems = wide ? 8 : 4, r = 32 / (head <= 8 * lane_elems ? 8 : head <= 16 * lane_elems ? 16 : 32);
+    // one pass of a warp a chunk; where the machine is full anyway, 8 passes of a token's queries (its position and angles
+    // are then looked up once for them)
+    const bool full = rows >= 148 * 16;
     p.q_per = full ? 8 * r : r;
-    p.kv_chunks = (kv_heads + p.kv_per - 1) / p.kv_per;
+    p.kv_chunks = (kv_heads + r - 1) / r;
     p.chunks = p.kv_chunks + (p.heads + p.q_per - 1) / p.q_per;
     const long long blocks = ((long long)rows * p.chunks + 7) / 8;
     if (blocks > INT_MAX) {
@@ -363,13 +416,13 @@ extern "C" int mvb_kv_append(void *kq, float *ks, void *vq, float *vs, int pages
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const unsigned grid = (unsigned)blocks;
     if (bits == 8) {
-        if (dtype == kF32) launch_append<float, 8>(p, grid, s);
-        else if (dtype == kBF16) launch_append<__nv_bfloat16, 8>(p, grid, s);
-        else launch_append<__half, 8>(p, grid, s);
+        if (dtype == kF32) launch_append<float, 8>(p, grid, wide, s);
+        else if (dtype == kBF16) launch_append<__nv_bfloat16, 8>(p, grid, wide, s);
+        else launch_append<__half, 8>(p, grid, wide, s);
     } else {
-        if (dtype == kF32) launch_append<float, 4>(p, grid, s);
-        else if (dtype == kBF16) launch_append<__nv_bfloat16, 4>(p, grid, s);
-        else launch_append<__half, 4>(p, grid, s);
+        if (dtype == kF32) launch_append<float, 4>(p, grid, wide, s);
+        else if (dtype == kBF16) launch_append<__nv_bfloat16, 4>(p, grid, wide, s);
+        else launch_append<__half, 4>(p, grid, wide, s);
     }
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) {

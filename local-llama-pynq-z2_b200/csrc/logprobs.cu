@@ -29,7 +29,6 @@ namespace cg = cooperative_groups;
 
 static __device__ int g_logp_error;
 
-constexpr int kThreads = 256;
 constexpr int kVecs = 4;      // 16-byte vectors a thread has in flight (a group: one maximum)
 constexpr int kList = 2048;   // candidates
 constexpr int kMostTop = 64;
@@ -94,6 +93,78 @@ __device__ __forceinline__ Sums joined(Sums a, Sums b) {
 
 template <typename T> struct Vec { static constexpr int kN = 16 / sizeof(T); };
 
+// Two fp32 lanes in one register pair: Blackwell's packed adds and multiply-adds, half the instructions.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 halves(uint64_t p) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+    return f;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// Words of a vector (one fp32 or two 16-bit elements): the larger of two without regard to NaN; not below a floor, NaN
+// kept; and the fp32 values. The floor stands for elements whose exponential is zero as long as the maximum is above
+// kSane: it keeps -inf out of (x - m) exp(x - m).
+template <typename T> struct Word;
+template <> struct Word<float> {
+    static constexpr float kSane = -1e29f;
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    }
+    static __device__ __forceinline__ uint32_t floored(uint32_t a) {
+        asm("max.NaN.f32 %0, %0, %1;" : "+r"(a) : "r"(0xF149F2CAu));  // -1e30
+        return a;
+    }
+    static __device__ __forceinline__ float first(uint32_t a) { return __uint_as_float(a); }
+    static __device__ __forceinline__ float second(uint32_t) { return -INFINITY; }
+};
+template <> struct Word<__nv_bfloat16> {
+    static constexpr float kSane = -1e29f;
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ __forceinline__ uint32_t floored(uint32_t a) {
+        asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(a) : "r"(0xF14AF14Au));  // -1.0004e30
+        return a;
+    }
+    static __device__ __forceinline__ float first(uint32_t a) { return __uint_as_float(a << 16); }
+    static __device__ __forceinline__ float second(uint32_t a) { return __uint_as_float(a & 0xFFFF0000u); }
+};
+template <> struct Word<__half> {
+    static constexpr float kSane = -60000.0f;
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ __forceinline__ uint32_t floored(uint32_t a) {
+        asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(a) : "r"(0xFBFFFBFFu));  // -65504
+        return a;
+    }
+    static __device__ __forceinline__ float first(uint32_t a) { return __low2float(*reinterpret_cast<__half2 *>(&a)); }
+    static __device__ __forceinline__ float second(uint32_t a) { return __high2float(*reinterpret_cast<__half2 *>(&a)); }
+};
+
 template <typename T>
 __device__ __forceinline__ void unpack(const uint4 &u, float (&f)[Vec<T>::kN]) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -101,13 +172,9 @@ __device__ __forceinline__ void unpack(const uint4 &u, float (&f)[Vec<T>::kN]) {
     for (int i = 0; i < 4; i++) {
         if constexpr (sizeof(T) == 4) {
             f[i] = __uint_as_float(w[i]);
-        } else if constexpr (Type<T>::kId == kBF16) {
-            f[2 * i] = __uint_as_float(w[i] << 16);
-            f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
         } else {
-            const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-            f[2 * i] = h.x;
-            f[2 * i + 1] = h.y;
+            f[2 * i] = Word<T>::first(w[i]);
+            f[2 * i + 1] = Word<T>::second(w[i]);
         }
     }
 }
@@ -120,8 +187,8 @@ __device__ __forceinline__ uint4 load_stream(const uint4 *p) {
     return v;
 }
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Params p) {
+template <typename T, bool TOP, int kThreads>
+__global__ void __launch_bounds__(kThreads, 768 / kThreads) logprobs_kernel(const Params p) {
     constexpr int N = Vec<T>::kN;
     extern __shared__ __align__(16) float group_max[];  // [iters][kThreads], TOP only
     __shared__ Sums parts[kThreads / 32];
@@ -146,41 +213,92 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Params p) {
     Sums s = {-INFINITY, 0.0f, 0.0f};
     float mine = -INFINITY;  // this thread's largest element of the vectors
     int seen = 0;
-    for (int it = 0, v = v0 + tid; v < v1; it++, v += kVecs * kThreads) {
-        uint4 u[kVecs];
-        const int left = (v1 - v + kThreads - 1) / kThreads;  // vectors of this thread from here on
+    int v = v0 + tid;
+    // whole groups of kVecs vectors
+    uint4 next[kVecs];  // the group after this one, on its way
+    if (v + (kVecs - 1) * kThreads < v1) {
 #pragma unroll
-        for (int k = 0; k < kVecs; k++)
-            if (k < left) u[k] = load_stream(vec + v + k * kThreads);
-        float f[kVecs][N];
-        float g = -INFINITY;
+        for (int k = 0; k < kVecs; k++) next[k] = load_stream(vec + v + k * kThreads);
+    }
+    for (; v + (kVecs - 1) * kThreads < v1; v += kVecs * kThreads, seen++) {
+        uint32_t u[4 * kVecs];
 #pragma unroll
         for (int k = 0; k < kVecs; k++) {
-            if (k < left) {
-                unpack<T>(u[k], f[k]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < N; i++) f[k][i] = -INFINITY;
-            }
-#pragma unroll
-            for (int i = 0; i < N; i++) g = fmaxf(g, f[k][i]);
+            u[4 * k] = next[k].x;
+            u[4 * k + 1] = next[k].y;
+            u[4 * k + 2] = next[k].z;
+            u[4 * k + 3] = next[k].w;
         }
-        if (TOP) group_max[it * kThreads + tid] = g;
-        seen = it + 1;
+        if (v + (2 * kVecs - 1) * kThreads < v1) {
+#pragma unroll
+            for (int k = 0; k < kVecs; k++) next[k] = load_stream(vec + v + (kVecs + k) * kThreads);
+        }
+        uint32_t gm[2] = {u[0], u[1]};
+#pragma unroll
+        for (int k = 2; k < 4 * kVecs; k++) gm[k & 1] = Word<T>::larger(gm[k & 1], u[k]);
+        gm[0] = Word<T>::larger(gm[0], gm[1]);
+        const float g = fmaxf(fmaxf(Word<T>::first(gm[0]), Word<T>::second(gm[0])), -INFINITY);
+        if (TOP) group_max[seen * kThreads + tid] = g;
         mine = fmaxf(mine, g);
         if (g > s.m) move_to(s, g);
-        const float base = s.m == -INFINITY ? 0.0f : s.m;
-        float z = 0.0f, w = 0.0f;
+        if (s.m > Word<T>::kSane) {
+            const uint64_t base = pair(-s.m, -s.m), l2e = pair(kLog2e, kLog2e);
+            uint64_t z[2] = {0, 0}, w[2] = {0, 0};
 #pragma unroll
-        for (int k = 0; k < kVecs; k++)
+            for (int k = 0; k < 4 * kVecs; k += sizeof(T) / 2) {
+                uint64_t x;
+                if constexpr (sizeof(T) == 4) {
+                    x = pair(Word<T>::first(Word<T>::floored(u[k])), Word<T>::first(Word<T>::floored(u[k + 1])));
+                } else {
+                    const uint32_t f = Word<T>::floored(u[k]);
+                    x = pair(Word<T>::first(f), Word<T>::second(f));
+                }
+                const int a = (k / (sizeof(T) / 2)) & 1;
+                const uint64_t d = add2(x, base);
+                const float2 t = halves(mul2(d, l2e));
+                float2 e;
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+                const uint64_t e2 = pair(e.x, e.y);
+                z[a] = add2(z[a], e2);
+                w[a] = fma2(d, e2, w[a]);
+            }
+            const float2 zz = halves(add2(z[0], z[1])), ww = halves(add2(w[0], w[1]));
+            s.z += zz.x + zz.y;
+            s.w += ww.x + ww.y;
+        } else {  // only masks so far: element by element
+            const float base = s.m == -INFINITY ? 0.0f : s.m;
+#pragma unroll
+            for (int k = 0; k < 4 * kVecs; k++) {
+                for (int h = 0; h < 4 / (int)sizeof(T); h++) {
+                    const float d = below(h ? Word<T>::second(u[k]) : Word<T>::first(u[k]), base), e = exp_fast(d);
+                    s.z += e;
+                    s.w = __fmaf_rn(d, e, s.w);
+                }
+            }
+        }
+    }
+    if (v < v1) {  // the last, partial group
+        float g = -INFINITY;
+        for (int k = 0; k < kVecs && v + k * kThreads < v1; k++) {
+            float f[N];
+            unpack<T>(load_stream(vec + v + k * kThreads), f);
+            float gv = f[0];
+#pragma unroll
+            for (int i = 1; i < N; i++) gv = fmaxf(gv, f[i]);
+            g = fmaxf(g, gv);
+            if (gv > s.m) move_to(s, gv);
+            const float base = s.m == -INFINITY ? 0.0f : s.m;
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const float d = below(f[k][i], base), e = exp_fast(d);
-                z += e;
-                w = __fmaf_rn(d, e, w);
+                const float d = below(f[i], base), e = exp_fast(d);
+                s.z += e;
+                s.w = __fmaf_rn(d, e, s.w);
             }
-        s.z += z;
-        s.w += w;
+        }
+        if (TOP) group_max[seen * kThreads + tid] = g;
+        mine = fmaxf(mine, g);
+        seen++;
     }
     if (split == 0 && tid < edge) {
         const float f = to_f32(x[edge_at(tid)]);
@@ -210,14 +328,23 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Params p) {
         cta_sums = t;
     }
     if (TOP) {
-        // the top-th largest of the threads' maxima
-        int rank = 0;
-        for (int i = 0; i < kThreads / 4; i++) {
-            const float4 o = reinterpret_cast<const float4 *>(thread_max)[i];
-            rank += (o.x > mine || (o.x == mine && 4 * i < tid)) + (o.y > mine || (o.y == mine && 4 * i + 1 < tid)) +
-                    (o.z > mine || (o.z == mine && 4 * i + 2 < tid)) + (o.w > mine || (o.w == mine && 4 * i + 3 < tid));
+        // A lower bound of the top-th largest of the threads' maxima, and so of the top-th largest element: the largest
+        // value of 16 leading bits that `top` maxima reach (exact for bf16). One warp, a binary search of 16 votes.
+        if (warp == 0) {
+            uint32_t o[kThreads / 32];
+#pragma unroll
+            for (int i = 0; i < kThreads / 32; i++) o[i] = (uint32_t)(key_of(thread_max[i * 32 + lane], 0) >> 48);
+            uint32_t found = 0;
+#pragma unroll
+            for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
+                int n = 0;
+#pragma unroll
+                for (int i = 0; i < kThreads / 32; i++) n += o[i] >= (found | bit);
+                if (__reduce_add_sync(0xffffffffu, n) >= p.top) found |= bit;
+            }
+            // (-inf and what lies below its 16 bits: everything is a candidate)
+            if (lane == 0) bound = found <= 0x007Fu ? -INFINITY : value_of((unsigned long long)found << 48);
         }
-        if (rank == p.top - 1) bound = mine;
         __syncthreads();
         const float bd = bound;
         // the elements that reach it, into the list while it has room; count counts them all
@@ -388,10 +515,10 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const Params p) {
     }
 }
 
-template <typename T, bool TOP>
-static cudaError_t launch(Params p, cudaStream_t stream) {
+template <typename T, bool TOP, int kThreads>
+static cudaError_t launch_threads(Params p, cudaStream_t stream) {
     constexpr int N = Vec<T>::kN, kChunk = kThreads * kVecs * N;
-    auto kernel = logprobs_kernel<T, TOP>;
+    auto kernel = logprobs_kernel<T, TOP, kThreads>;
     // a row over more CTAs while the grid leaves SMs idle and each CTA still has a chunk, or where its maxima would not
     // fit in shared memory
     int splits = 1;
@@ -420,6 +547,13 @@ static cudaError_t launch(Params p, cudaStream_t stream) {
     return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
+template <typename T, bool TOP>
+static cudaError_t launch(const Params &p, cudaStream_t stream) {
+    // many rows: half the threads a row and twice the rows an SM, so that the ends of rows (joins, candidates) of some
+    // stand beside the streaming of others
+    return p.rows >= 148 * 4 ? launch_threads<T, TOP, 128>(p, stream) : launch_threads<T, TOP, 256>(p, stream);
+}
+
 int logp_take_error(cudaStream_t s) {
     int v = 0;
     if (cudaMemcpyFromSymbolAsync(&v, g_logp_error, sizeof v, 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
@@ -440,6 +574,7 @@ int kv_take_error(cudaStream_t s);
 }  // namespace rows
 namespace attn {
 int attn_take_error(cudaStream_t s);
+int tc_take_error(cudaStream_t s);
 }
 }  // namespace mvb
 
@@ -494,7 +629,8 @@ extern "C" int mvb_logprobs(const void *x, long long stride, int dtype, int rows
 extern "C" int mvb_serve_status(void *stream) {
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     int first = 0;
-    for (auto take : {rows::rope_take_error, rows::kv_take_error, attn::attn_take_error, logp::logp_take_error}) {
+    for (auto take : {rows::rope_take_error, rows::kv_take_error, attn::attn_take_error, attn::tc_take_error,
+                      logp::logp_take_error}) {
         const int v = take(s);
         if (v < 0) {
             set_error("mvb_serve_status: the stream failed: %s", cudaGetErrorString(cudaGetLastError()));

@@ -14,7 +14,7 @@ namespace rows {
 enum : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
 
 // what a kernel found in its index arrays (mvb_serve_status)
-enum : int { kOk = 0, kBadPage = 1, kBadLength = 2, kBadPosition = 3, kBadToken = 4 };
+enum : int { kOk = 0, kBadPage = 1, kBadLength = 2, kBadPosition = 3, kBadToken = 4, kWaitRanOut = 5 };
 
 template <typename T> struct Type;
 template <> struct Type<float> { static constexpr int kId = kF32; };

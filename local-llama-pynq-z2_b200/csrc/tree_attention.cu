@@ -39,8 +39,8 @@ static __device__ int g_attn_error;
 
 constexpr int kWarps = 8;
 constexpr int kStages = 3;
-constexpr float kPScale = 256.0f;   // P' = P * vs * kPScale / W stays below 64 * 256 in fp16
-constexpr float kLazy = 6.0f;       // the running maximum moves only when it is 2^6 behind
+constexpr float kPScale = 4.0f;     // P' = P * vs * kPScale / W stays below 2^14 in fp16
+constexpr float kLazy = 12.0f;      // the running maximum moves only when it is 2^12 behind
 
 template <int HDP, int BITS>
 struct Slice {
@@ -353,7 +353,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 2 ? 2 : 1) tree_attention_k
                     float x = mx[nt][h];
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-                    x = fmaxf(m[nt][h], x);
+                    // only the rows that are behind move, so that a row's result does not depend on its neighbours
+                    if (!(x > m[nt][h] + kLazy)) x = m[nt][h];
                     const float a = m[nt][h] == -INFINITY ? 0.0f : exp2_fast(m[nt][h] - x);
                     m[nt][h] = x;
                     l[nt][h] *= a;
@@ -587,6 +588,7 @@ static cudaError_t launch_rows(const AttnParams &p, int max_len, cudaStream_t st
 
 template <typename T, int BITS>
 static cudaError_t launch_size(const AttnParams &p, int max_len, cudaStream_t stream) {
+    if ((long long)p.max_new * p.group > 32) return launch_tc(p, rows::Type<T>::kId, BITS, max_len, stream);
     return p.head <= 64 ? launch_rows<T, BITS, 64>(p, max_len, stream) : launch_rows<T, BITS, 128>(p, max_len, stream);
 }
 

@@ -1,0 +1,852 @@
+// mvb_tree_attention for many query rows (new tokens x the query heads of one kv head): trees of dozens of tokens, prompt
+// chunks. Same arithmetic as tree_attention.cu (exact integers in fp16, one scale a row, fp32 statistics), on the
+// 5th-generation tensor cores, since each cached byte now meets 33 to 256 rows.
+//
+// One CTA: up to MT = 2 tiles of 128 query rows against 64 keys a step. The cache is converted once for all rows: raw
+// pages -> (bulk copies) -> raw bytes -> (converter warps) -> fp16 tiles in the 128-byte swizzled layout, two of each. Keys
+// are the K-major B operand of S = Q K^T; values, stored by key, are the MN-major B operand of O += P V. P is the A
+// operand in tensor memory, written over the S it came from. Tensor memory: two 64-column slots of S for each row tile
+// (so that the next step's scores stand ready when a softmax ends), then O0 | O1, 128 columns each.
+//
+// Warp roles (512 threads):
+//   warp 0          one thread issues the MMAs: PV0 PV1 QK0'' QK1'' a step. (The oldest warp, which the scheduler prefers:
+//                   as warp 12 it waited for issue slots behind the softmax.)
+//   warp 1          bulk copies of the raw pages, kRaw stages ahead.
+//   warps 4-5, 6-7  converters of K, of V: a thread owns a key. Bytes -> fp16; the keys' or the values' scales.
+//   warps 8-11, 12-15  softmax of row tile 0, 1: a thread owns a row. S from tensor memory, keys' scales, maximum,
+//                   exponentials, values' scales, P in fp16 back to tensor memory. The running maximum and the values' unit
+//                   W move only when a row falls 2^12 behind (then O is scaled in tensor memory, after the product before
+//                   has ended). The unit's factor is folded into the exponent, so it multiplies P and the row's sum alike.
+// What bounds it: for two row tiles of head 128 and 64 keys the exponentials take 1,024 clocks (16 a clock), the MMAs
+// 1,280 (QK at N = 64 waits for shared memory: 48 clocks a product against 32), shared memory 1,150.
+// The keys of a sequence are split over the CTAs of a cluster, joined in distributed shared memory in rank order.
+// Every mbarrier wait is bounded (1 s): a wait that runs out notes the error and the roles stop.
+// Every barrier is waited on before its next phase can end: each role's next arrival needs what the waiter does after.
+#include <cooperative_groups.h>
+#include <math.h>
+
+#include <type_traits>
+
+#include "../../include/matvec_b200.h"
+#include "mvb_runtime.h"
+#include "tree_attention.cuh"
+
+namespace mvb {
+namespace attn {
+
+using namespace rows;
+namespace cg = cooperative_groups;
+
+static __device__ int g_tc_error;
+constexpr int kTcThreads = 512;
+constexpr int kMmaWarp = 0, kLoadWarp = 1;  // first, since the scheduler prefers the oldest warp
+constexpr int kBN = 64;              // keys a step
+constexpr int kRaw = 3;              // raw stages
+constexpr int kScales = 4;           // steps whose scales are kept
+constexpr float kPUnit = 2.0f;       // log2 of P' / (P * vs / W): P' stays below 2^15 in fp16
+constexpr float kBehind = 12.0f;     // (6: some warp of the eight moved nearly every step, 2,000 clocks each time)
+constexpr unsigned long long kWaitNs = 1000000000ull;
+
+__device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint64_t *bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint64_t *bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ unsigned long long clock_ns() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity) {
+    const uint32_t a = smem_addr(bar);
+    unsigned long long t0 = 0;
+    for (uint32_t i = 0;; i++) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(a), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if ((i & 1023) == 1023) {
+            const unsigned long long t = clock_ns();
+            if (!t0) t0 = t;
+            else if (t - t0 > kWaitNs) {
+                note(&g_tc_error, kWaitRanOut);
+                return false;
+            }
+        }
+    }
+}
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     smem_addr(dst)),
+                 "l"(src), "r"(bytes), "r"(smem_addr(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+                 : "memory");
+}
+// One lane of a converged warp. The compiler knows that a branch on elect.sync has one lane, and keeps the products'
+// descriptors in uniform registers across it; from a branch on the lane number, or with the products predicated, each
+// takes ten instructions more to issue (with busy warps beside it 400 clocks against the 64 that it runs).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+
+// Shared-memory matrix descriptor of a 128-byte swizzled tile: rows of 128 bytes, 8-row groups 1024 bytes apart (stride
+// offset); lead: from one block of 64 elements to the next along the major dimension (MN-major tiles only).
+__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t lead) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// Instruction descriptor of kind::f16: D fp32 (bits 4-5 = 1), A and B fp16, B MN-major in bit 16, N >> 3 in bits 17-22,
+// M >> 4 in bits 24-28.
+__host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool b_mn) {
+    return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
+}
+
+// 32 or 16 consecutive columns of this thread's lane, and 16 back.
+__device__ __forceinline__ void tmem_load32(uint32_t addr, float *r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+          "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]),
+          "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
+          "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_load16(uint32_t addr, float *r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+          "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Pairs of fp32 in one instruction.
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void split2(uint64_t p, float &a, float &b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {  // the largest that is a number
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// Sixteen cached integers (16 bytes, or 8 of nibbles) as fp16 in their order: two 16-byte pieces.
+template <int BITS>
+__device__ __forceinline__ uint4 load_sixteen(const uint8_t *src) {
+    if (BITS == 8) return *reinterpret_cast<const uint4 *>(src);
+    const uint2 u = *reinterpret_cast<const uint2 *>(src);
+    return make_uint4(u.x, u.y, 0, 0);
+}
+template <int BITS>
+__device__ __forceinline__ void sixteen(uint4 u, uint4 &a, uint4 &b) {
+    uint32_t h[8];
+    if (BITS == 8) {
+        const uint32_t w[4] = {u.x ^ 0x80808080u, u.y ^ 0x80808080u, u.z ^ 0x80808080u, u.w ^ 0x80808080u};
+        const uint32_t bias = 0x64806480u;  // 1024 + 128
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            h[2 * i] = __byte_perm(w[i], 0x64646464u, 0x4140);
+            h[2 * i + 1] = __byte_perm(w[i], 0x64646464u, 0x4342);
+            asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(h[2 * i]) : "r"(bias));
+            asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(h[2 * i + 1]) : "r"(bias));
+        }
+    } else {
+        const uint32_t w[2] = {u.x, u.y};
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            uint32_t g[4];  // (k, k + 4)
+#pragma unroll
+            for (int k = 0; k < 4; k++) g[k] = nibbles_to_half2(w[i], k);
+            h[4 * i] = __byte_perm(g[0], g[1], 0x5410);
+            h[4 * i + 1] = __byte_perm(g[2], g[3], 0x5410);
+            h[4 * i + 2] = __byte_perm(g[0], g[1], 0x7632);
+            h[4 * i + 3] = __byte_perm(g[2], g[3], 0x7632);
+        }
+    }
+    a = make_uint4(h[0], h[1], h[2], h[3]);
+    b = make_uint4(h[4], h[5], h[6], h[7]);
+}
+
+// 32 mask bits of new tokens j .. j + 31 for new token i (negative j: cached positions, allowed).
+__device__ __forceinline__ uint32_t mask32(const AttnParams &p, const Sequence &s, int i, int j) {
+    if (i >= s.n) return j + 31 < 0 ? 0xFFFFFFFFu : j < 0 ? (1u << -j) - 1 : 0u;
+    auto from = [&](int k) -> uint32_t {  // bits of k .. k + 31, k >= 0
+        uint32_t w;
+        if (!p.tree) {
+            w = i < k ? 0u : i - k >= 31 ? 0xFFFFFFFFu : (2u << (i - k)) - 1;
+        } else {
+            const unsigned long long *t = p.tree + (size_t)(s.row0 + i) * p.words;
+            const int at = k >> 6, sh = k & 63;
+            unsigned long long x = at < p.words ? t[at] >> sh : 0ull;
+            if (sh > 32 && at + 1 < p.words) x |= t[at + 1] << (64 - sh);
+            w = (uint32_t)x;
+        }
+        return s.n - k >= 32 ? w : s.n <= k ? 0u : w & ((1u << (s.n - k)) - 1);
+    };
+    if (j >= 0) return from(j);
+    if (j <= -32) return 0xFFFFFFFFu;
+    return (from(0) << -j) | ((1u << -j) - 1);
+}
+
+template <int QP, int BITS, int HDP, int MT>
+struct TcSmem {
+    static constexpr int kBlocks = HDP / 64;                      // blocks of 64 elements (128 bytes)
+    static constexpr int kQTile = kBlocks * 128 * 128;            // an fp16 tile of 128 rows
+    static constexpr int kTile = kBlocks * kBN * 128;             // of kBN keys
+    static constexpr int kQ = 0;                                  // [MT][QP] tiles
+    static constexpr int kK = kQ + MT * QP * kQTile;              // [2]
+    static constexpr int kV = kK + 2 * kTile;                     // [2]
+    static constexpr int kRawRow = HDP * BITS / 8;
+    static constexpr int kRawTile = kBN * kRawRow;
+    static constexpr int kRawAt = kV + 2 * kTile;                 // [kRaw][K | V | ks | vs]
+    static constexpr int kRawStage = 2 * kRawTile + 2 * kBN * 4;
+    // the partial O of a split, [MT * 128][HDP] fp32, lies over the tiles
+    static constexpr int kJoin = MT * 128 * HDP * 4;
+    static constexpr int kEnd = kRawAt + kRaw * kRawStage;
+    static constexpr int kScale = kEnd > kJoin ? kEnd : kJoin;    // [kScales][kk | vv] fp32
+    static constexpr int kRow = kScale + kScales * 2 * kBN * 4;   // row factors [MT][128]
+    static constexpr int kMl = kRow + MT * 128 * 4;               // this CTA's (max, sum) [2][MT * 128]
+    static constexpr int kAll = kMl + 2 * MT * 128 * 4;           // the cluster's weights [8][MT * 128], sums [MT * 128]
+    static constexpr int kBar = kAll + 9 * MT * 128 * 4;
+    static constexpr size_t kBytes = kBar + 512 + 1024;           // + alignment
+    static_assert(kBytes <= 227 * 1024, "shared memory of a CTA");
+};
+
+template <typename T, int QP, int PP, int BITS, int HDP, int MT>
+__global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const AttnParams p) {
+    using S = TcSmem<QP, BITS, HDP, MT>;
+    constexpr int ROWS = MT * 128;
+    extern __shared__ __align__(1024) uint8_t raw_smem[];
+    uint8_t *smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);
+    uint64_t *bar = reinterpret_cast<uint64_t *>(smem + S::kBar);
+    // (slot = step & 1 where there are two, step % kRaw of raw, step % kScales of scales)
+    uint64_t *raw_full = bar, *raw_empty = raw_full + kRaw, *k_ready = raw_empty + kRaw, *k_free = k_ready + 2,
+             *v_ready = k_free + 2, *v_free = v_ready + 2, *s_full = v_free + 2 /* [m][slot] */,
+             *p_ready = s_full + 4 /* [m][slot] */, *pv_done = p_ready + 4 /* [m] */, *sc_ready = pv_done + 2,
+             *q_ready = sc_ready + kScales, *o_done = q_ready + 1;
+    uint32_t *tmem_at = reinterpret_cast<uint32_t *>(o_done + 1);
+    float *vmax = reinterpret_cast<float *>(bar + 40);  // [kScales][2]
+    float *row_factor = reinterpret_cast<float *>(smem + S::kRow);
+    float *cta_m = reinterpret_cast<float *>(smem + S::kMl), *cta_l = cta_m + ROWS;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int b = blockIdx.z, kvh = blockIdx.y / p.qtiles, qt = blockIdx.y - kvh * p.qtiles, split = blockIdx.x;
+    const Sequence s = sequence_at(p, b, &g_tc_error);
+    const int nrows = s.n * p.group, R0 = qt * ROWS;
+    if (R0 >= nrows) return;  // the whole cluster returns together
+    const int nt = (s.len + kBN - 1) / kBN;
+    const int t0 = (int)((long long)nt * split / p.splits), t1 = (int)((long long)nt * (split + 1) / p.splits);
+    const int mine = t1 - t0;
+
+    if (tid == 0) {
+        for (int i = 0; i < kRaw; i++) {
+            bar_init(&raw_full[i], 1);
+            bar_init(&raw_empty[i], 4);
+        }
+        for (int i = 0; i < 2; i++) {
+            bar_init(&k_ready[i], 2);
+            bar_init(&v_ready[i], 2);
+            bar_init(&k_free[i], 1);
+            bar_init(&v_free[i], 1);
+            bar_init(&pv_done[i], 1);
+        }
+        for (int i = 0; i < 4; i++) {
+            bar_init(&s_full[i], 1);
+            bar_init(&p_ready[i], 4);
+        }
+        for (int i = 0; i < kScales; i++) bar_init(&sc_ready[i], 2);
+        bar_init(q_ready, 8);
+        bar_init(o_done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_at)), "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_at;
+    const int row_bytes = p.head * BITS / 8;
+
+    if (warp < 8) {
+        if (warp >= 4) {
+            // ---------------- converters: one key a thread, warps 4-5 its keys' row, warps 6-7 its values' ----------------
+            const int key = tid & 63, kv = (warp - 4) >> 1, pieces = p.head / 16;
+            uint64_t *ready = kv ? v_ready : k_ready, *free_ = kv ? v_free : k_free;
+            uint8_t *tiles = smem + (kv ? S::kV : S::kK) + key * 128;
+            if (pieces < HDP / 16)  // the columns behind the head are never converted: zeros, so that they add nothing
+                for (int i = 0; i < 2 * S::kBlocks * 8; i++)
+                    *reinterpret_cast<uint4 *>(tiles + (i >> 3) * (kBN * 128) + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+            for (int j = 0; j < mine; j++) {
+                const int slot = j & 1, rs = j % kRaw, ss = j % kScales;
+                const uint8_t *raw = smem + S::kRawAt + rs * S::kRawStage;
+                if (!bar_wait(&raw_full[rs], (j / kRaw) & 1)) break;
+                if (kv) {
+                    // the scales, before the tile is free: the softmax of kScales steps ago, their last reader, is done
+                    // (the step before waited for the product with its P, or a later one)
+                    const bool live = (t0 + j) * kBN + key < s.len;
+                    float *sc = reinterpret_cast<float *>(smem + S::kScale) + ss * 2 * kBN;
+                    const float *rsc = reinterpret_cast<const float *>(raw + 2 * S::kRawTile);
+                    const float x = live ? rsc[kBN + key] : 0.0f;
+                    sc[key] = live ? rsc[key] * p.scale_log2 : 0.0f;
+                    sc[kBN + key] = x;
+                    float mv = fabsf(x) < INFINITY ? fabsf(x) : 0.0f;  // an infinite scale must not set the unit
+#pragma unroll
+                    for (int o = 16; o; o >>= 1) mv = fmaxf(mv, __shfl_xor_sync(0xffffffffu, mv, o));
+                    if (lane == 0) vmax[ss * 2 + (warp & 1)] = mv;
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(&sc_ready[ss]);
+                }
+                // the tile's last product has ended
+                if (j >= 2 && !bar_wait(&free_[slot], ((j >> 1) - 1) & 1)) break;
+                const uint8_t *src = raw + kv * S::kRawTile + key * row_bytes;
+                uint8_t *dst = tiles + slot * S::kTile;
+                // the lanes of a quarter warp start at different pieces: different banks
+                if (pieces == HDP / 16) {
+                    constexpr int PIECES = HDP / 16;
+                    const int first = key & (PIECES - 1);
+                    uint4 raw16[PIECES];  // all loads first (16 integers each: 16 bytes, or 8 in the low half)
+#pragma unroll
+                    for (int i = 0; i < PIECES; i++) raw16[i] = load_sixteen<BITS>(src + (i ^ first) * 2 * BITS);
+#pragma unroll
+                    for (int i = 0; i < PIECES; i++) {
+                        uint4 x, y;
+                        sixteen<BITS>(raw16[i], x, y);
+                        const int c = i ^ first, at = (c >> 2) * (kBN * 128) + ((((2 * c) & 7) ^ (key & 7)) << 4);
+                        *reinterpret_cast<uint4 *>(dst + at) = x;
+                        *reinterpret_cast<uint4 *>(dst + (at ^ 16)) = y;
+                    }
+                } else {
+                    int c = key % pieces;
+                    for (int i = 0; i < pieces; i++) {
+                        uint4 x, y;
+                        sixteen<BITS>(load_sixteen<BITS>(src + c * 2 * BITS), x, y);
+                        const int at = (c >> 2) * (kBN * 128) + ((((2 * c) & 7) ^ (key & 7)) << 4);
+                        *reinterpret_cast<uint4 *>(dst + at) = x;
+                        *reinterpret_cast<uint4 *>(dst + (at ^ 16)) = y;
+                        c = c + 1 == pieces ? 0 : c + 1;
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    bar_arrive(&ready[slot]);
+                    bar_arrive(&raw_empty[rs]);
+                }
+            }
+        } else if (warp == kMmaWarp) {
+            // ---------------- MMA issue ----------------
+            if (mine > 0 && elect_one()) {
+                constexpr uint32_t qk = idesc_f16(128, kBN, false), pv = idesc_f16(128, HDP, true);
+                const uint32_t t = tmem;
+                const uint64_t q0 = tile_desc(smem_addr(smem + S::kQ), 16), k0 = tile_desc(smem_addr(smem + S::kK), 16),
+                               v0 = tile_desc(smem_addr(smem + S::kV), kBN * 128);  // start addresses count 16 bytes
+                auto scores = [&](int slot) {  // S_m[slot] = Q_m K[slot]^T for every row tile, every part of q
+#pragma unroll
+                    for (int m = 0; m < MT; m++) {
+#pragma unroll
+                        for (int part = 0; part < QP; part++)
+#pragma unroll
+                            for (int k = 0; k < HDP / 16; k++)
+                                mma_ss(t + m * 128 + slot * 64,
+                                       q0 + (((m * QP + part) * S::kQTile + (k >> 2) * 16384 + (k & 3) * 32) >> 4),
+                                       k0 + ((slot * S::kTile + (k >> 2) * (kBN * 128) + (k & 3) * 32) >> 4), qk,
+                                       part > 0 || k > 0);
+                        commit(&s_full[2 * m + slot]);
+                    }
+                    commit(&k_free[slot]);
+                };
+                bool ok = bar_wait(q_ready, 0);
+#pragma unroll 1
+                for (int j = 0; j < min(mine, 2) && ok; j++) {
+                    if (!(ok = bar_wait(&k_ready[j], 0))) break;
+                    fence_after();
+                    scores(j);
+                }
+#pragma unroll 1
+                for (int j = 0; j < mine && ok; j++) {
+                    const int slot = j & 1, par = (j >> 1) & 1;
+                    if (!(ok = bar_wait(&v_ready[slot], par))) break;
+#pragma unroll
+                    for (int m = 0; m < MT; m++) {
+                        if (ok) ok = bar_wait(&p_ready[2 * m + slot], par);
+                        if (!ok) break;
+                        fence_after();
+#pragma unroll
+                        for (int part = 0; part < PP; part++)
+#pragma unroll
+                            for (int k = 0; k < kBN / 16; k++)
+                                mma_ts(t + 256 + m * 128, t + m * 128 + slot * 64 + part * 32 + k * 8,
+                                       v0 + ((slot * S::kTile + k * 2048) >> 4), pv, j > 0 || part > 0 || k > 0);
+                        commit(&pv_done[m]);
+                    }
+                    if (!ok) break;
+                    commit(&v_free[slot]);
+                    if (j + 2 < mine) {
+                        if (!(ok = bar_wait(&k_ready[slot], ((j + 2) >> 1) & 1))) break;
+                        fence_after();
+                        scores(slot);
+                    }
+                }
+                commit(o_done);
+            }
+        } else if (warp == kLoadWarp) {
+            // ---------------- raw pages ----------------
+            const int run = min(1 << p.bt.page_log2, kBN), runs = kBN / run;  // keys a copy, copies a step
+            for (int j = 0; j < mine; j++) {
+                const int st = j % kRaw;
+                if (j >= kRaw && !bar_wait(&raw_empty[st], (j / kRaw - 1) & 1)) break;
+                uint8_t *raw = smem + S::kRawAt + st * S::kRawStage;
+                const int key0 = (t0 + j) * kBN, key = key0 + lane * run;
+                const bool on = lane < runs && key < s.len;
+                const uint32_t n = __popc(__ballot_sync(0xffffffffu, on));
+                if (lane == 0) bar_expect(&raw_full[st], n * (uint32_t)run * (2 * row_bytes + 8));
+                __syncwarp();
+                if (on) {
+                    const int pg = page_of(p, b, key, &g_tc_error);
+                    const size_t row = (((size_t)pg * p.kv_heads + kvh) << p.bt.page_log2) +
+                                       (key & ((1 << p.bt.page_log2) - 1));
+                    const uint32_t bytes = run * row_bytes;
+                    bulk_load(raw + lane * bytes, p.kq + row * row_bytes, bytes, &raw_full[st]);
+                    bulk_load(raw + S::kRawTile + lane * bytes, p.vq + row * row_bytes, bytes, &raw_full[st]);
+                    uint8_t *sc = raw + 2 * S::kRawTile + lane * run * 4;
+                    bulk_load(sc, p.ks + row, run * 4, &raw_full[st]);
+                    bulk_load(sc + kBN * 4, p.vs + row, run * 4, &raw_full[st]);
+                }
+            }
+            // copies in flight land before the CTA can end
+            for (int j = mine > kRaw ? mine - kRaw : 0; j < mine; j++) bar_wait(&raw_full[j % kRaw], (j / kRaw) & 1);
+        }
+    } else {
+        // ---------------- softmax: one row a thread ----------------
+        // q: a warp takes a row, scales it by a power of two and stores its fp16 parts, swizzled
+        constexpr int DEEP = 8;  // rows of a warp in flight
+        for (int i0 = warp - 8; i0 < ROWS; i0 += 8 * DEEP) {
+            float4 v[DEEP];
+#pragma unroll
+            for (int u = 0; u < DEEP; u++) {  // (no branch around the loads: all of them are in flight at once)
+                const int R = min(R0 + i0 + 8 * u, nrows - 1), tok = R / p.group;
+                v[u] = load4(static_cast<const T *>(p.q) + (size_t)(s.row0 + tok) * p.q_stride +
+                             (size_t)(kvh * p.group + R - tok * p.group) * p.head + min(4 * lane, p.head - 4));
+            }
+#pragma unroll
+            for (int u = 0; u < DEEP; u++)
+                if (R0 + i0 + 8 * u >= nrows || 4 * lane >= p.head) v[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int u = 0; u < DEEP; u++) {
+                const int i = i0 + 8 * u;
+                int e = max(max(exponent_of(v[u].x), exponent_of(v[u].y)), max(exponent_of(v[u].z), exponent_of(v[u].w)));
+#pragma unroll
+                for (int o = 16; o; o >>= 1) e = max(e, __shfl_xor_sync(0xffffffffu, e, o));
+                const int k = max(-100, min(e - 127 - 8, 119));
+                if (lane == 0) row_factor[i] = pow2(k);
+                const float f = pow2(-k);
+                float x[4] = {v[u].x * f, v[u].y * f, v[u].z * f, v[u].w * f};
+                if (4 * lane < HDP) {
+                    const int r = i & 127;
+                    uint8_t *d = smem + S::kQ + (i >> 7) * QP * S::kQTile + (lane >> 4) * 16384 + r * 128 +
+                                 ((((lane & 15) >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8;
+                    *reinterpret_cast<uint2 *>(d) = make_uint2(pack2<__half>(x[0], x[1]), pack2<__half>(x[2], x[3]));
+                    if (QP == 2) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) x[j] -= __half2float(__float2half_rn(x[j]));
+                        *reinterpret_cast<uint2 *>(d + S::kQTile) =
+                            make_uint2(pack2<__half>(x[0], x[1]), pack2<__half>(x[2], x[3]));
+                    }
+                }
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) bar_arrive(q_ready);
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // the row factors, among the softmax warps
+        const int m = (warp - 8) >> 2, row = tid & 127;
+        const uint32_t lane_at = tmem + ((uint32_t)(row & 96) << 16), o_at = lane_at + 256 + m * 128;
+        const int R = R0 + m * 128 + row, draft = R / p.group;
+        const float rf = MT > m ? row_factor[m * 128 + row] : 0.0f;
+        float mx = -INFINITY, l = 0.0f, lw = -80.0f;  // running maximum and sum (in the unit's factor); lw = log2 of W
+        const bool has = m < MT;
+        // One step; TAIL: some of its keys are new tokens, or none (a variant of its own: the mask's branches cost the
+        // others more than their arithmetic).
+        auto step = [&](int j, auto is_tail) -> bool {
+            constexpr bool TAIL = decltype(is_tail)::value;
+            const int slot = j & 1, par = (j >> 1) & 1, ss = j % kScales, key0 = (t0 + j) * kBN;
+            const uint32_t s_at = lane_at + m * 128 + slot * 64;
+            if (!bar_wait(&s_full[2 * m + slot], par) || !bar_wait(&sc_ready[ss], (j / kScales) & 1)) return false;
+            fence_after();
+            const float *kk = reinterpret_cast<const float *>(smem + S::kScale) + ss * 2 * kBN, *vv = kk + kBN;
+            float u[kBN];
+#pragma unroll
+            for (int c = 0; c < kBN / 32; c++) tmem_load32(s_at + 32 * c, u + 32 * c);
+            const float2 v2 = *reinterpret_cast<const float2 *>(vmax + ss * 2);
+            const float vm = fmaxf(v2.x, v2.y);
+            uint32_t bits[kBN / 32] = {};
+            if (TAIL) {
+#pragma unroll
+                for (int c = 0; c < kBN / 32; c++) bits[c] = mask32(p, s, draft, key0 + 32 * c - s.ctx);
+            }
+            wait_load();
+            float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < kBN; i += 4) {
+                const float4 k4 = *reinterpret_cast<const float4 *>(kk + i);
+                split2(mul2(pair2(u[i], u[i + 1]), pair2(k4.x, k4.y)), u[i], u[i + 1]);
+                split2(mul2(pair2(u[i + 2], u[i + 3]), pair2(k4.z, k4.w)), u[i + 2], u[i + 3]);
+                if (TAIL) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (!((bits[(i + e) >> 5] >> ((i + e) & 31)) & 1)) u[i + e] = -INFINITY;
+                }
+                top[0] = max3(top[0], u[i], u[i + 1]);
+                top[1] = max3(top[1], u[i + 2], u[i + 3]);
+            }
+            const float now = fmaxf(mx, fmaxf(top[0], top[1]) * rf);
+            const float lv = (float)(min(max(exponent_of(vm), 1) - 127 + 1, 127));  // W above this step's scales
+            const bool grow = vm > 0.0f && lv > lw;
+            const bool behind = now > mx + kBehind;
+            if (__any_sync(0xffffffffu, grow || behind)) {
+                const float lw2 = grow ? lv : lw;
+                // O and the sum: exp2(old max - new max), and the old unit in the new one. Only the rows that are behind
+                // move, so that a row's result does not depend on its neighbours.
+                const float mx2 = behind ? now : mx;
+                const float f = mx == -INFINITY ? 0.0f : exp2_fast((mx - mx2) + (lw - lw2));
+                mx = mx2;
+                lw = lw2;
+                l *= f;
+                if (j > 0) {
+                    // (the product of two steps ago has ended: this step's scores were issued after it)
+                    if (!bar_wait(&pv_done[m], (j - 1) & 1)) return false;
+                    fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < HDP / 16; c++) {
+                        float o[16];
+                        tmem_load16(o_at + 16 * c, o);
+                        wait_load();
+#pragma unroll
+                        for (int i = 0; i < 16; i++) o[i] *= f;
+                        tmem_store16(o_at + 16 * c, reinterpret_cast<const uint32_t *>(o));
+                    }
+                }
+            }
+            const float base = (kPUnit - lw) - (mx == -INFINITY ? 0.0f : mx);
+            const uint64_t rf2 = pair2(rf, rf), base2 = pair2(base, base);
+            uint64_t sum[2] = {0, 0};
+            uint32_t low[PP == 2 ? kBN / 2 : 1];
+#pragma unroll
+            for (int c = 0; c < kBN / 32; c++) {
+                uint32_t hi[16];
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                    const float4 w4 = *reinterpret_cast<const float4 *>(vv + 32 * c + i);
+                    const uint64_t w2[2] = {pair2(w4.x, w4.y), pair2(w4.z, w4.w)};
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const int at = 32 * c + i + 2 * h;
+                        float a, d;
+                        split2(fma2(pair2(u[at], u[at + 1]), rf2, base2), a, d);
+                        const uint64_t e2 = pair2(exp2_fast(a), exp2_fast(d));
+                        sum[h] = add2(sum[h], e2);
+                        float x, y;
+                        split2(mul2(e2, w2[h]), x, y);
+                        if (TAIL) {  // a masked key's scale may be anything: its weight is zero, not zero times that
+                            if (u[at] == -INFINITY) x = 0.0f;
+                            if (u[at + 1] == -INFINITY) y = 0.0f;
+                        }
+                        const uint32_t q = pack2<__half>(x, y);
+                        hi[(i + 2 * h) / 2] = q;
+                        if (PP == 2) {
+                            const float2 r = __half22float2(*reinterpret_cast<const __half2 *>(&q));
+                            low[PP == 2 ? at / 2 : 0] = pack2<__half>(x - r.x, y - r.y);
+                        }
+                    }
+                }
+                tmem_store16(s_at + 16 * c, hi);
+            }
+            if (PP == 2) {
+#pragma unroll
+                for (int c = 0; c < kBN / 32; c++) tmem_store16(s_at + 32 + 16 * c, low + (PP == 2 ? 16 * c : 0));
+            }
+            float a, d, a2, d2;
+            split2(sum[0], a, d);
+            split2(sum[1], a2, d2);
+            l += (a + d) + (a2 + d2);
+            wait_store();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&p_ready[2 * m + slot]);
+            return true;
+        };
+        // steps wholly below the context first
+        const int plain = has ? max(0, min(mine, s.ctx / kBN - t0)) : 0;
+        bool ok = has;
+#pragma unroll 1
+        for (int j = 0; j < plain && ok; j++) ok = step(j, std::false_type{});
+#pragma unroll 1
+        for (int j = plain; j < mine && ok; j++) ok = step(j, std::true_type{});
+        if (has && mine > 0) bar_wait(o_done, 0);
+        fence_after();
+        // O in units of W / 2^kPUnit, and the sum in the same: they cancel
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        if (has && p.splits == 1) {
+            if (R < nrows) {
+                const int tok = s.row0 + R / p.group, head = kvh * p.group + R % p.group;
+                if (p.lse)
+                    p.lse[(size_t)tok * p.heads + head] =
+                        l == 0.0f ? -INFINITY : (mx - (kPUnit - lw) + log2f(l)) * 0.693147180559945309f;
+            }
+#pragma unroll
+            for (int c = 0; c < HDP / 32; c++) {
+                float o[32];
+                if (mine > 0) {
+                    tmem_load32(o_at + 32 * c, o);
+                    wait_load();
+                }
+                if (R < nrows) {
+                    T *d = static_cast<T *>(p.out) + (size_t)(s.row0 + R / p.group) * p.out_stride +
+                           (size_t)(kvh * p.group + R % p.group) * p.head;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        if (32 * c + i < p.head)
+                            store4(d + 32 * c + i, l == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                                                             : make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv,
+                                                                           o[i + 3] * inv));
+                }
+            }
+        } else if (has) {
+            // this CTA's part: O divided by its own sum, the row's (max, sum) beside it
+            cta_m[m * 128 + row] = mx;
+            cta_l[m * 128 + row] = l == 0.0f ? 0.0f : l * exp2f(lw - kPUnit);  // the sum in its own units
+            float *po = reinterpret_cast<float *>(smem) + (size_t)(m * 128 + row) * HDP;
+            const float unit = l == 0.0f ? 0.0f : inv;
+#pragma unroll
+            for (int c = 0; c < HDP / 32; c++) {
+                float o[32];
+                if (mine > 0) {
+                    tmem_load32(o_at + 32 * c, o);
+                    wait_load();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; i++) o[i] = 0.0f;
+                }
+                // the 16-byte pieces of a row start at different places: different banks
+#pragma unroll
+                for (int i = 0; i < 32; i += 4)
+                    *reinterpret_cast<float4 *>(po + ((32 * c + i) ^ ((row & 7) << 2))) =
+                        l == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                                  : make_float4(o[i] * unit, o[i + 1] * unit, o[i + 2] * unit, o[i + 3] * unit);
+            }
+        }
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    if (p.splits == 1) return;
+
+    // join the cluster: weights of every CTA's rows first, then each CTA takes its share of the elements
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    float *weight = reinterpret_cast<float *>(smem + S::kAll), *total = weight + 8 * ROWS;
+    const int rows_here = min(ROWS, nrows - R0);
+    for (int i = tid; i < rows_here; i += kTcThreads) {
+        float m = -INFINITY, sum = 0.0f;
+        float ms[8], ls[8];
+#pragma unroll
+        for (int w = 0; w < 8; w++) {
+            ms[w] = w < p.splits ? *cluster.map_shared_rank(&cta_m[i], w) : -INFINITY;
+            ls[w] = w < p.splits ? *cluster.map_shared_rank(&cta_l[i], w) : 0.0f;
+            m = fmaxf(m, ms[w]);
+        }
+#pragma unroll
+        for (int w = 0; w < 8; w++) {
+            const float x = ls[w] == 0.0f ? 0.0f : ls[w] * exp2_fast(ms[w] - m);
+            if (w < p.splits) weight[w * ROWS + i] = x;
+            sum += x;
+        }
+        total[i] = sum;
+        if (split == 0 && p.lse) {
+            const int R = R0 + i;
+            p.lse[(size_t)(s.row0 + R / p.group) * p.heads + kvh * p.group + R % p.group] =
+                sum == 0.0f ? -INFINITY : (m + log2f(sum)) * 0.693147180559945309f;
+        }
+    }
+    __syncthreads();
+    constexpr int kPer = 4;  // elements of a thread in flight
+    const int total4 = rows_here * (HDP / 4);
+    for (int i0 = tid + split * kTcThreads; i0 < total4; i0 += kTcThreads * p.splits * kPer) {
+        float4 o[kPer];
+#pragma unroll
+        for (int u = 0; u < kPer; u++) o[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 2
+        for (int w = 0; w < p.splits; w++) {
+            float4 x[kPer];
+#pragma unroll
+            for (int u = 0; u < kPer; u++) {
+                const int i = min(i0 + u * kTcThreads * p.splits, total4 - 1), row = i / (HDP / 4), d4 = i % (HDP / 4);
+                x[u] = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(
+                    reinterpret_cast<const float *>(smem) + (size_t)row * HDP + ((4 * d4) ^ ((row & 7) << 2)), w));
+            }
+#pragma unroll
+            for (int u = 0; u < kPer; u++) {
+                const float f = weight[w * ROWS + min(i0 + u * kTcThreads * p.splits, total4 - 1) / (HDP / 4)];
+                o[u].x = __fmaf_rn(f, x[u].x, o[u].x);
+                o[u].y = __fmaf_rn(f, x[u].y, o[u].y);
+                o[u].z = __fmaf_rn(f, x[u].z, o[u].z);
+                o[u].w = __fmaf_rn(f, x[u].w, o[u].w);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kPer; u++) {
+            const int i = i0 + u * kTcThreads * p.splits, row = i / (HDP / 4), d4 = i % (HDP / 4);
+            if (i >= total4 || 4 * d4 >= p.head) continue;
+            const float sum = total[row], inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const int R = R0 + row;
+            store4(static_cast<T *>(p.out) + (size_t)(s.row0 + R / p.group) * p.out_stride +
+                       (size_t)(kvh * p.group + R % p.group) * p.head + 4 * d4,
+                   make_float4(o[u].x * inv, o[u].y * inv, o[u].z * inv, o[u].w * inv));
+        }
+    }
+    cluster.sync();  // no CTA leaves while a sister reads its shared memory
+}
+
+template <typename T, int QP, int PP, int BITS, int HDP, int MT>
+static cudaError_t launch(AttnParams p, int max_len, cudaStream_t stream) {
+    using S = TcSmem<QP, BITS, HDP, MT>;
+    // more than half of an SM's shared memory, so that no second CTA waits for tensor memory
+    constexpr size_t smem = S::kBytes > 116 * 1024 ? S::kBytes : 116 * 1024;
+    auto kernel = tree_attention_tc_kernel<T, QP, PP, BITS, HDP, MT>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    p.qtiles = (int)(((long long)p.max_new * p.group + MT * 128 - 1) / (MT * 128));
+    if ((long long)p.qtiles * p.kv_heads > 65535) return cudaErrorInvalidConfiguration;
+    const long long base = (long long)p.qtiles * p.kv_heads * p.bt.batch;
+    // Split a sequence over the CTAs of a cluster so that the estimated time is least: jobs of max_len / splits keys (in
+    // steps) and kFixed steps of starting, filling and joining; three quarters of the longest length on average; the
+    // last jobs end a third of a job apart. (Clusters of 4 and 8 reach 132 and 120 of the 148 SMs. 16 sequences of up to
+    // 16,000 keys, 8 kv heads: 350, 197, 253, 353 us with 1, 2, 4, 8.)
+    constexpr double kFixed = 8;
+    const double steps = (double)max_len / kBN;
+    int splits = 1;
+    double least = 1e30;
+    for (int n = 1; n <= 8; n *= 2) {
+        if (n > 1 && steps < 4 * n) break;
+        const double job = steps / n + kFixed, slots = n <= 2 ? 148 : n == 4 ? 132 : 120, load = 0.75 * base * n / slots;
+        const double t = (load > 1 ? load : 1) * job + job / 3;
+        if (t < least) least = t, splits = n;
+    }
+    p.splits = splits;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(splits, p.kv_heads * p.qtiles, p.bt.batch);
+    cfg.blockDim = dim3(kTcThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = splits;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <typename T, int QP, int PP, int BITS, int HDP>
+static cudaError_t launch_tiles(const AttnParams &p, int max_len, cudaStream_t s) {
+    // two parts of q for two row tiles of 128-element heads do not fit in shared memory
+    if constexpr (QP == 1 || HDP == 64) {
+        if ((long long)p.max_new * p.group > 128) return launch<T, QP, PP, BITS, HDP, 2>(p, max_len, s);
+    }
+    return launch<T, QP, PP, BITS, HDP, 1>(p, max_len, s);
+}
+
+template <int BITS, int HDP>
+static cudaError_t launch_type(const AttnParams &p, int dtype, int max_len, cudaStream_t s) {
+    if (dtype == kF32) return launch_tiles<float, 2, 2, BITS, HDP>(p, max_len, s);
+    if (dtype == kBF16) return launch_tiles<__nv_bfloat16, 1, 1, BITS, HDP>(p, max_len, s);
+    return launch_tiles<__half, 1, 2, BITS, HDP>(p, max_len, s);
+}
+
+cudaError_t launch_tc(const AttnParams &p, int dtype, int bits, int max_len, cudaStream_t s) {
+    if (bits == 8) return p.head <= 64 ? launch_type<8, 64>(p, dtype, max_len, s) : launch_type<8, 128>(p, dtype, max_len, s);
+    return p.head <= 64 ? launch_type<4, 64>(p, dtype, max_len, s) : launch_type<4, 128>(p, dtype, max_len, s);
+}
+
+int tc_take_error(cudaStream_t s) {
+    int v = 0;
+    if (cudaMemcpyFromSymbolAsync(&v, g_tc_error, sizeof v, 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
+        cudaStreamSynchronize(s) != cudaSuccess)
+        return -1;
+    const int z = 0;
+    if (v && (cudaMemcpyToSymbolAsync(g_tc_error, &z, sizeof z, 0, cudaMemcpyHostToDevice, s) != cudaSuccess ||
+              cudaStreamSynchronize(s) != cudaSuccess))
+        return -1;
+    return v;
+}
+
+}  // namespace attn
+}  // namespace mvb

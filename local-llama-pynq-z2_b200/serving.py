@@ -375,7 +375,8 @@ def _results(torch, dev, n, nids, top, has_ids, entropy):
 
 #: what serve_status() returns
 STATUS = {0: "ok", 1: "a page number out of range", 2: "a length or a row range out of range",
-          3: "a rotary position outside its table", 4: "a token id outside the vocabulary"}
+          3: "a rotary position outside its table", 4: "a token id outside the vocabulary",
+          5: "a wait inside a kernel that gave up (a fault of the library or the device)"}
 
 
 def serve_status(stream=None, device=None):

@@ -173,5 +173,5 @@ def test_tree_mask(mvb):
 
 
 def test_status_names_every_code(mvb):
-    assert set(mvb.serving.STATUS) == {0, 1, 2, 3, 4}
+    assert set(mvb.serving.STATUS) == {0, 1, 2, 3, 4, 5}
     assert mvb.lib().mvb_serve_status.restype is C.c_int

@@ -25,6 +25,8 @@
 #include <limits.h>
 #include <math.h>
 
+#include <mutex>
+
 #include "../../include/matvec_b200.h"
 #include "mvb_runtime.h"
 #include "tree_attention.cuh"
@@ -37,7 +39,6 @@ namespace cg = cooperative_groups;
 
 static __device__ int g_attn_error;
 
-constexpr int kWarps = 8;
 constexpr int kStages = 3;
 constexpr float kPScale = 4.0f;     // P' = P * vs * kPScale / W stays below 2^14 in fp16
 constexpr float kLazy = 12.0f;      // the running maximum moves only when it is 2^12 behind
@@ -49,7 +50,7 @@ struct Slice {
     static constexpr int kRow = HDP * BITS / 8;        // bytes of a row in shared memory
     static constexpr int kScales = 2 * kKeys * kRow;   // offset of the scales in a stage
     static constexpr int kStage = 2 * kKeys * kRow + 2 * kKeys * 4;
-    static constexpr int kWarp = kStages * kStage;
+    static constexpr int kWarp = kStages * kStage;  // a warp's ring
     static constexpr int kPieces = BITS == 8 ? kRow / 32 : kRow / 16;  // cp.async a lane and 16-key piece, at most
 };
 
@@ -96,8 +97,8 @@ template <typename T> struct Parts { static constexpr int kQ = 1, kP = 1; };
 template <> struct Parts<__half> { static constexpr int kQ = 1, kP = 2; };
 template <> struct Parts<float> { static constexpr int kQ = 2, kP = 2; };
 
-template <typename T, int BITS, int HDP, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT <= 2 ? 2 : 1) tree_attention_kernel(const AttnParams p) {
+template <typename T, int BITS, int HDP, int NT, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, kWarps == 8 && NT <= 2 ? 2 : 1) tree_attention_kernel(const AttnParams p) {
     using S = Slice<HDP, BITS>;
     constexpr int KS = HDP / 16;                 // k-steps of q.k, and 16-element tiles of O
     constexpr int RUN = HDP / 8;                 // a lane's elements of a value row: RUN * r ..
@@ -543,33 +544,31 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 2 ? 2 : 1) tree_attention_k
     cluster.sync();  // no CTA leaves while a sister reads its shared memory
 }
 
-template <typename T, int BITS, int HDP, int NT>
-static cudaError_t launch(AttnParams p, int max_len, cudaStream_t stream) {
+template <typename T, int BITS, int HDP, int NT, int kWarps>
+static cudaError_t launch_warps(AttnParams p, int max_len, cudaStream_t stream) {
     using S = Slice<HDP, BITS>;
     constexpr int ROWS = 8 * NT;
     constexpr size_t frag = (size_t)Parts<T>::kQ * NT * (HDP / 16) * 256;
     constexpr size_t ring = (size_t)kWarps * S::kWarp + (size_t)ROWS * HDP * 4, join = (size_t)kWarps * ROWS * HDP * 4;
     constexpr size_t smem = frag + (ring > join ? ring : join);
     static_assert(smem <= 227 * 1024 - 8192, "shared memory of a CTA");
-    auto kernel = tree_attention_kernel<T, BITS, HDP, NT>;
+    auto kernel = tree_attention_kernel<T, BITS, HDP, NT, kWarps>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
     p.qtiles = (int)(((long long)p.max_new * p.group + ROWS - 1) / ROWS);
     if ((long long)p.qtiles * p.kv_heads > 65535) return cudaErrorInvalidConfiguration;
-    const long long base = (long long)p.qtiles * p.kv_heads * p.bt.batch;
-    // split a sequence over more CTAs while the grid leaves SMs idle and every warp still has a slice
-    int splits = 1;
-    while (splits < 16 && base * splits * 2 <= 2 * 148 && (long long)splits * 2 * kWarps * S::kKeys <= max_len) splits *= 2;
-    p.splits = splits;
+    // a unit: one slice a warp; starting and joining a CTA cost about eight
+    p.splits = choose_splits((long long)p.qtiles * p.kv_heads * p.bt.batch, p.bt.batch, (double)max_len / (kWarps * S::kKeys), 8.0, 1.0,
+                             [&](int n) { return cluster_slots((const void *)kernel, n, kWarps * 32, smem); });
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(splits, p.kv_heads * p.qtiles, p.bt.batch);
+    cfg.gridDim = dim3(p.splits, p.kv_heads * p.qtiles, p.bt.batch);
     cfg.blockDim = dim3(kWarps * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = splits;
+    attr[0].val.clusterDim.x = p.splits;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
@@ -577,19 +576,67 @@ static cudaError_t launch(AttnParams p, int max_len, cudaStream_t stream) {
     return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
+template <typename T, int BITS, int HDP, int NT>
+static cudaError_t launch(const AttnParams &p, int max_len, cudaStream_t stream) {
+    using S = Slice<HDP, BITS>;
+    // Two CTAs of 8 warps an SM; or, where the jobs are so few that clusters of 16 leave one CTA an SM, and the sequences
+    // long enough for it, one of 16 warps. Three column tiles need more registers: one CTA of 12 warps.
+    const long long base = ((long long)p.max_new * p.group + 8 * NT - 1) / (8 * NT) * p.kv_heads * p.bt.batch;
+    if constexpr (NT <= 2) {
+        if (base <= 18 && max_len >= 2 * 16 * 16 * S::kKeys) return launch_warps<T, BITS, HDP, NT, 16>(p, max_len, stream);
+        return launch_warps<T, BITS, HDP, NT, 8>(p, max_len, stream);
+    } else {
+        return launch_warps<T, BITS, HDP, NT, 12>(p, max_len, stream);
+    }
+}
+
 template <typename T, int BITS, int HDP>
 static cudaError_t launch_rows(const AttnParams &p, int max_len, cudaStream_t stream) {
     const long long rows = (long long)p.max_new * p.group;
     if (rows <= 8) return launch<T, BITS, HDP, 1>(p, max_len, stream);
     if (rows <= 16) return launch<T, BITS, HDP, 2>(p, max_len, stream);
-    if (rows <= 24) return launch<T, BITS, HDP, 3>(p, max_len, stream);
-    return launch<T, BITS, HDP, 4>(p, max_len, stream);
+    return launch<T, BITS, HDP, 3>(p, max_len, stream);
 }
 
 template <typename T, int BITS>
 static cudaError_t launch_size(const AttnParams &p, int max_len, cudaStream_t stream) {
-    if ((long long)p.max_new * p.group > 32) return launch_tc(p, rows::Type<T>::kId, BITS, max_len, stream);
+    // 24 rows: with 8 kv heads of 128 in 8 bits, 24 and 32 rows take 88 and 106 us here against 92 and 92 there for 64
+    // sequences of up to 2,000 keys, 46 and 54 against 50 and 50 for 16 of up to 4,000
+    if ((long long)p.max_new * p.group > 24) return launch_tc(p, rows::Type<T>::kId, BITS, max_len, stream);
     return p.head <= 64 ? launch_rows<T, BITS, 64>(p, max_len, stream) : launch_rows<T, BITS, 128>(p, max_len, stream);
+}
+
+int cluster_slots(const void *kernel, int n, int threads, size_t smem) {
+    struct Entry {
+        const void *kernel;
+        int device, n, slots;
+    };
+    static std::mutex mutex;
+    static Entry known[1024];
+    static int count = 0;
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return n == 1 ? 148 : 0;
+    std::lock_guard<std::mutex> lock(mutex);
+    for (int i = 0; i < count; i++)
+        if (known[i].kernel == kernel && known[i].device == device && known[i].n == n) return known[i].slots;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(n);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = n;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        clusters = 0;
+    }
+    if (count < (int)(sizeof known / sizeof known[0])) known[count++] = Entry{kernel, device, n, clusters * n};
+    return clusters * n;
 }
 
 int attn_take_error(cudaStream_t s) {

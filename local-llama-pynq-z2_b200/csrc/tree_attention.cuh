@@ -85,6 +85,33 @@ __device__ __forceinline__ uint32_t nibbles_to_half2(uint32_t x, int k) {
     return h;
 }
 
+constexpr int kMaxSplits = 16;
+
+// CTAs of `kernel` in clusters of n that the current device holds at once (0 where none fits). Looked up once a kernel,
+// size and device: clusters live inside a GPC, so that sizes which do not divide its SMs leave some idle.
+int cluster_slots(const void *kernel, int n, int threads, size_t smem);
+
+// Over how many CTAs of a cluster a sequence's keys are split, so that the estimated time is least: `base` jobs without a
+// split, `steps` units of work each for the longest sequence, `fixed` units to start, fill and join a CTA, at least `least`
+// units a CTA. One sequence: its jobs are alike and run in whole waves. Several: three quarters of the longest on average,
+// in no order, and the last jobs end a third of a job apart.
+template <typename F>
+inline int choose_splits(long long base, int batch, double steps, double fixed, double least, const F &slots_of) {
+    int best = 1;
+    double best_time = 1e300;
+    for (int n = 1; n <= kMaxSplits; n++) {
+        if (n > 1 && steps < least * n) break;
+        const int slots = slots_of(n);
+        if (slots < n) continue;
+        const double job = steps / n + fixed, fill = (double)base * n / slots;
+        double time = job;
+        if (fill > 1.0) time = batch == 1 ? (double)((base * n + slots - 1) / slots) * job
+                                          : (0.75 * fill > 1.0 ? 0.75 * fill : 1.0) * job + job / 3;
+        if (time < best_time * 0.999) best_time = time, best = n;
+    }
+    return best;
+}
+
 int tc_take_error(cudaStream_t s);
 // The kernel for many query rows; returns the CUDA error of its launch.
 cudaError_t launch_tc(const AttnParams &p, int dtype, int bits, int max_len, cudaStream_t s);

@@ -19,7 +19,9 @@
 //                   has ended). The unit's factor is folded into the exponent, so it multiplies P and the row's sum alike.
 // What bounds it: for two row tiles of head 128 and 64 keys the exponentials take 1,024 clocks (16 a clock), the MMAs
 // 1,280 (QK at N = 64 waits for shared memory: 48 clocks a product against 32), shared memory 1,150.
-// The keys of a sequence are split over the CTAs of a cluster, joined in distributed shared memory in rank order.
+// Up to 128 query rows (MT = 1): both softmax groups take the same rows, for every other step each, with an O and
+// (max, sum) of their own; the two parts are joined like those of the cluster.
+// The keys of a sequence are split over the CTAs of a cluster, joined in distributed shared memory in a fixed order.
 // Every mbarrier wait is bounded (1 s): a wait that runs out notes the error and the roles stop.
 // Every barrier is waited on before its next phase can end: each role's next arrival needs what the waiter does after.
 #include <cooperative_groups.h>
@@ -41,7 +43,6 @@ static __device__ int g_tc_error;
 constexpr int kTcThreads = 512;
 constexpr int kMmaWarp = 0, kLoadWarp = 1;  // first, since the scheduler prefers the oldest warp
 constexpr int kBN = 64;              // keys a step
-constexpr int kRaw = 3;              // raw stages
 constexpr int kScales = 4;           // steps whose scales are kept
 constexpr float kPUnit = 2.0f;       // log2 of P' / (P * vs / W): P' stays below 2^15 in fp16
 constexpr float kBehind = 12.0f;     // (6: some warp of the eight moved nearly every step, 2,000 clocks each time)
@@ -263,14 +264,20 @@ struct TcSmem {
     static constexpr int kRawTile = kBN * kRawRow;
     static constexpr int kRawAt = kV + 2 * kTile;                 // [kRaw][K | V | ks | vs]
     static constexpr int kRawStage = 2 * kRawTile + 2 * kBN * 4;
-    // the partial O of a split, [MT * 128][HDP] fp32, lies over the tiles
-    static constexpr int kJoin = MT * 128 * HDP * 4;
+    // raw stages: as many as fit, up to 6 (keys are converted up to four steps before their values are, and a stage is free
+    // only after its values; with 3 the copies came too late for MT = 1: 2,300 clocks a step)
+    static constexpr int kRest = 32 * 1024;  // what follows the stages, at most
+    static constexpr int kFit = (227 * 1024 - kRest - kRawAt) / kRawStage;
+    static constexpr int kRaw = kFit > 6 ? 6 : kFit;
+    static_assert(kRaw >= 3, "raw stages");
+    // the partial O of both softmax groups, [256][HDP] fp32, lies over the tiles
+    static constexpr int kJoin = 256 * HDP * 4;
     static constexpr int kEnd = kRawAt + kRaw * kRawStage;
     static constexpr int kScale = kEnd > kJoin ? kEnd : kJoin;    // [kScales][kk | vv] fp32
     static constexpr int kRow = kScale + kScales * 2 * kBN * 4;   // row factors [MT][128]
-    static constexpr int kMl = kRow + MT * 128 * 4;               // this CTA's (max, sum) [2][MT * 128]
-    static constexpr int kAll = kMl + 2 * MT * 128 * 4;           // the cluster's weights [8][MT * 128], sums [MT * 128]
-    static constexpr int kBar = kAll + 9 * MT * 128 * 4;
+    static constexpr int kMl = kRow + MT * 128 * 4;               // (max, sum) of both groups' rows [2][256]
+    static constexpr int kAll = kMl + 2 * 256 * 4;                // every part's weights, and their sums [MT * 128]
+    static constexpr int kBar = kAll + (kMaxSplits * (3 - MT) + 1) * MT * 128 * 4;
     static constexpr size_t kBytes = kBar + 512 + 1024;           // + alignment
     static_assert(kBytes <= 227 * 1024, "shared memory of a CTA");
 };
@@ -279,6 +286,9 @@ template <typename T, int QP, int PP, int BITS, int HDP, int MT>
 __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const AttnParams p) {
     using S = TcSmem<QP, BITS, HDP, MT>;
     constexpr int ROWS = MT * 128;
+    constexpr bool ALT = MT == 1;            // the groups alternate over the steps
+    constexpr int PARTS = ALT ? 2 : 1;       // partial results of a row in a CTA
+    constexpr int kRaw = S::kRaw;
     extern __shared__ __align__(1024) uint8_t raw_smem[];
     uint8_t *smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);
     uint64_t *bar = reinterpret_cast<uint64_t *>(smem + S::kBar);
@@ -288,9 +298,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
              *p_ready = s_full + 4 /* [m][slot] */, *pv_done = p_ready + 4 /* [m] */, *sc_ready = pv_done + 2,
              *q_ready = sc_ready + kScales, *o_done = q_ready + 1;
     uint32_t *tmem_at = reinterpret_cast<uint32_t *>(o_done + 1);
-    float *vmax = reinterpret_cast<float *>(bar + 40);  // [kScales][2]
+    float *vmax = reinterpret_cast<float *>(bar + 48);  // [kScales][2]
     float *row_factor = reinterpret_cast<float *>(smem + S::kRow);
-    float *cta_m = reinterpret_cast<float *>(smem + S::kMl), *cta_l = cta_m + ROWS;
+    float *cta_m = reinterpret_cast<float *>(smem + S::kMl), *cta_l = cta_m + 256;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int b = blockIdx.z, kvh = blockIdx.y / p.qtiles, qt = blockIdx.y - kvh * p.qtiles, split = blockIdx.x;
@@ -406,52 +416,48 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
                 const uint32_t t = tmem;
                 const uint64_t q0 = tile_desc(smem_addr(smem + S::kQ), 16), k0 = tile_desc(smem_addr(smem + S::kK), 16),
                                v0 = tile_desc(smem_addr(smem + S::kV), kBN * 128);  // start addresses count 16 bytes
-                auto scores = [&](int slot) {  // S_m[slot] = Q_m K[slot]^T for every row tile, every part of q
-#pragma unroll
-                    for (int m = 0; m < MT; m++) {
-#pragma unroll
-                        for (int part = 0; part < QP; part++)
-#pragma unroll
-                            for (int k = 0; k < HDP / 16; k++)
-                                mma_ss(t + m * 128 + slot * 64,
-                                       q0 + (((m * QP + part) * S::kQTile + (k >> 2) * 16384 + (k & 3) * 32) >> 4),
-                                       k0 + ((slot * S::kTile + (k >> 2) * (kBN * 128) + (k & 3) * 32) >> 4), qk,
-                                       part > 0 || k > 0);
-                        commit(&s_full[2 * m + slot]);
-                    }
-                    commit(&k_free[slot]);
-                };
+                // the group's i-th step is step j of the CTA: the same for both groups, or every other one
+                auto step_of = [&](int m, int i) { return ALT ? 2 * i + m : i; };
                 bool ok = bar_wait(q_ready, 0);
-#pragma unroll 1
-                for (int j = 0; j < min(mine, 2) && ok; j++) {
-                    if (!(ok = bar_wait(&k_ready[j], 0))) break;
+                auto scores = [&](int m, int i) {  // S_m[i & 1] = Q K^T, every part of q; false: gave up
+                    const int j = step_of(m, i), slot = j & 1;
+                    if (j >= mine) return true;
+                    if ((ALT || m == 0) && !bar_wait(&k_ready[slot], (j >> 1) & 1)) return false;
                     fence_after();
-                    scores(j);
-                }
-#pragma unroll 1
-                for (int j = 0; j < mine && ok; j++) {
-                    const int slot = j & 1, par = (j >> 1) & 1;
-                    if (!(ok = bar_wait(&v_ready[slot], par))) break;
 #pragma unroll
-                    for (int m = 0; m < MT; m++) {
-                        if (ok) ok = bar_wait(&p_ready[2 * m + slot], par);
-                        if (!ok) break;
+                    for (int part = 0; part < QP; part++)
+#pragma unroll
+                        for (int k = 0; k < HDP / 16; k++)
+                            mma_ss(t + m * 128 + (i & 1) * 64,
+                                   q0 + ((((ALT ? 0 : m) * QP + part) * S::kQTile + (k >> 2) * 16384 + (k & 3) * 32) >> 4),
+                                   k0 + ((slot * S::kTile + (k >> 2) * (kBN * 128) + (k & 3) * 32) >> 4), qk,
+                                   part > 0 || k > 0);
+                    commit(&s_full[2 * m + (i & 1)]);
+                    if (ALT || m == 1) commit(&k_free[slot]);
+                    return true;
+                };
+#pragma unroll 1
+                for (int i = 0; i < 2 && ok; i++) ok = scores(0, i) && scores(1, i);
+#pragma unroll 1
+                for (int i = 0; step_of(0, i) < mine && ok; i++) {
+#pragma unroll
+                    for (int m = 0; m < 2; m++) {
+                        const int j = step_of(m, i), slot = j & 1;
+                        if (!ok || j >= mine) break;
+                        if ((ALT || m == 0) && !(ok = bar_wait(&v_ready[slot], (j >> 1) & 1))) break;
+                        if (!(ok = bar_wait(&p_ready[2 * m + (i & 1)], (i >> 1) & 1))) break;
                         fence_after();
 #pragma unroll
                         for (int part = 0; part < PP; part++)
 #pragma unroll
                             for (int k = 0; k < kBN / 16; k++)
-                                mma_ts(t + 256 + m * 128, t + m * 128 + slot * 64 + part * 32 + k * 8,
-                                       v0 + ((slot * S::kTile + k * 2048) >> 4), pv, j > 0 || part > 0 || k > 0);
+                                mma_ts(t + 256 + m * 128, t + m * 128 + (i & 1) * 64 + part * 32 + k * 8,
+                                       v0 + ((slot * S::kTile + k * 2048) >> 4), pv, i > 0 || part > 0 || k > 0);
                         commit(&pv_done[m]);
+                        if (ALT || m == 1) commit(&v_free[slot]);
+                        if (ALT) ok = scores(m, i + 2);
                     }
-                    if (!ok) break;
-                    commit(&v_free[slot]);
-                    if (j + 2 < mine) {
-                        if (!(ok = bar_wait(&k_ready[slot], ((j + 2) >> 1) & 1))) break;
-                        fence_after();
-                        scores(slot);
-                    }
+                    if (!ALT && ok) ok = scores(0, i + 2) && scores(1, i + 2);
                 }
                 commit(o_done);
             }
@@ -527,15 +533,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
         asm volatile("bar.sync 1, 256;" ::: "memory");  // the row factors, among the softmax warps
         const int m = (warp - 8) >> 2, row = tid & 127;
         const uint32_t lane_at = tmem + ((uint32_t)(row & 96) << 16), o_at = lane_at + 256 + m * 128;
-        const int R = R0 + m * 128 + row, draft = R / p.group;
-        const float rf = MT > m ? row_factor[m * 128 + row] : 0.0f;
+        const int R = R0 + (ALT ? 0 : m * 128) + row, draft = R / p.group;
+        const float rf = row_factor[ALT ? row : m * 128 + row];
         float mx = -INFINITY, l = 0.0f, lw = -80.0f;  // running maximum and sum (in the unit's factor); lw = log2 of W
-        const bool has = m < MT;
         // One step; TAIL: some of its keys are new tokens, or none (a variant of its own: the mask's branches cost the
         // others more than their arithmetic).
-        auto step = [&](int j, auto is_tail) -> bool {
+        auto step = [&](int i, auto is_tail) -> bool {
             constexpr bool TAIL = decltype(is_tail)::value;
-            const int slot = j & 1, par = (j >> 1) & 1, ss = j % kScales, key0 = (t0 + j) * kBN;
+            const int j = ALT ? 2 * i + m : i, slot = i & 1, par = (i >> 1) & 1, ss = j % kScales, key0 = (t0 + j) * kBN;
             const uint32_t s_at = lane_at + m * 128 + slot * 64;
             if (!bar_wait(&s_full[2 * m + slot], par) || !bar_wait(&sc_ready[ss], (j / kScales) & 1)) return false;
             fence_after();
@@ -578,9 +583,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
                 mx = mx2;
                 lw = lw2;
                 l *= f;
-                if (j > 0) {
+                if (i > 0) {
                     // (the product of two steps ago has ended: this step's scores were issued after it)
-                    if (!bar_wait(&pv_done[m], (j - 1) & 1)) return false;
+                    if (!bar_wait(&pv_done[m], (i - 1) & 1)) return false;
                     fence_after();
 #pragma unroll 1
                     for (int c = 0; c < HDP / 16; c++) {
@@ -641,18 +646,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
             if (lane == 0) bar_arrive(&p_ready[2 * m + slot]);
             return true;
         };
-        // steps wholly below the context first
-        const int plain = has ? max(0, min(mine, s.ctx / kBN - t0)) : 0;
-        bool ok = has;
+        // this group's steps, those wholly below the context first
+        auto share = [&](int n) { return ALT ? max(0, n - m + 1) / 2 : max(0, n); };
+        const int steps = share(mine), plain = share(min(mine, s.ctx / kBN - t0));
+        bool ok = true;
 #pragma unroll 1
-        for (int j = 0; j < plain && ok; j++) ok = step(j, std::false_type{});
+        for (int i = 0; i < plain && ok; i++) ok = step(i, std::false_type{});
 #pragma unroll 1
-        for (int j = plain; j < mine && ok; j++) ok = step(j, std::true_type{});
-        if (has && mine > 0) bar_wait(o_done, 0);
+        for (int i = plain; i < steps && ok; i++) ok = step(i, std::true_type{});
+        if (mine > 0) bar_wait(o_done, 0);
         fence_after();
         // O in units of W / 2^kPUnit, and the sum in the same: they cancel
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        if (has && p.splits == 1) {
+        if (!ALT && p.splits == 1) {
             if (R < nrows) {
                 const int tok = s.row0 + R / p.group, head = kvh * p.group + R % p.group;
                 if (p.lse)
@@ -662,7 +668,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
 #pragma unroll
             for (int c = 0; c < HDP / 32; c++) {
                 float o[32];
-                if (mine > 0) {
+                if (steps > 0) {
                     tmem_load32(o_at + 32 * c, o);
                     wait_load();
                 }
@@ -677,8 +683,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
                                                                            o[i + 3] * inv));
                 }
             }
-        } else if (has) {
-            // this CTA's part: O divided by its own sum, the row's (max, sum) beside it
+        } else {
+            // this group's part: O divided by its own sum, the row's (max, sum) beside it
             cta_m[m * 128 + row] = mx;
             cta_l[m * 128 + row] = l == 0.0f ? 0.0f : l * exp2f(lw - kPUnit);  // the sum in its own units
             float *po = reinterpret_cast<float *>(smem) + (size_t)(m * 128 + row) * HDP;
@@ -686,7 +692,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
 #pragma unroll
             for (int c = 0; c < HDP / 32; c++) {
                 float o[32];
-                if (mine > 0) {
+                if (steps > 0) {
                     tmem_load32(o_at + 32 * c, o);
                     wait_load();
                 } else {
@@ -706,27 +712,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
     __syncthreads();
     fence_after();
     if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
-    if (p.splits == 1) return;
+    if (!ALT && p.splits == 1) return;
 
     // join the cluster: weights of every CTA's rows first, then each CTA takes its share of the elements
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
-    float *weight = reinterpret_cast<float *>(smem + S::kAll), *total = weight + 8 * ROWS;
-    const int rows_here = min(ROWS, nrows - R0);
+    float *weight = reinterpret_cast<float *>(smem + S::kAll), *total = weight + kMaxSplits * PARTS * ROWS;
+    const int rows_here = min(ROWS, nrows - R0), parts = p.splits * PARTS;  // part n: CTA n / PARTS, group n % PARTS
     for (int i = tid; i < rows_here; i += kTcThreads) {
         float m = -INFINITY, sum = 0.0f;
-        float ms[8], ls[8];
-#pragma unroll
-        for (int w = 0; w < 8; w++) {
-            ms[w] = w < p.splits ? *cluster.map_shared_rank(&cta_m[i], w) : -INFINITY;
-            ls[w] = w < p.splits ? *cluster.map_shared_rank(&cta_l[i], w) : 0.0f;
-            m = fmaxf(m, ms[w]);
-        }
-#pragma unroll
-        for (int w = 0; w < 8; w++) {
-            const float x = ls[w] == 0.0f ? 0.0f : ls[w] * exp2_fast(ms[w] - m);
-            if (w < p.splits) weight[w * ROWS + i] = x;
-            sum += x;
+#pragma unroll 8
+        for (int n = 0; n < parts; n++) m = fmaxf(m, *cluster.map_shared_rank(&cta_m[(n % PARTS) * 128 + i], n / PARTS));
+#pragma unroll 8
+        for (int n = 0; n < parts; n++) {
+            const float l = *cluster.map_shared_rank(&cta_l[(n % PARTS) * 128 + i], n / PARTS);
+            const float x = *cluster.map_shared_rank(&cta_m[(n % PARTS) * 128 + i], n / PARTS);
+            const float w = l == 0.0f ? 0.0f : l * exp2_fast(x - m);
+            weight[n * ROWS + i] = w;
+            sum += w;
         }
         total[i] = sum;
         if (split == 0 && p.lse) {
@@ -743,17 +746,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
 #pragma unroll
         for (int u = 0; u < kPer; u++) o[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 2
-        for (int w = 0; w < p.splits; w++) {
+        for (int n = 0; n < parts; n++) {
             float4 x[kPer];
 #pragma unroll
             for (int u = 0; u < kPer; u++) {
                 const int i = min(i0 + u * kTcThreads * p.splits, total4 - 1), row = i / (HDP / 4), d4 = i % (HDP / 4);
                 x[u] = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(
-                    reinterpret_cast<const float *>(smem) + (size_t)row * HDP + ((4 * d4) ^ ((row & 7) << 2)), w));
+                    reinterpret_cast<const float *>(smem) + (size_t)((n % PARTS) * 128 + row) * HDP +
+                        ((4 * d4) ^ ((row & 7) << 2)), n / PARTS));
             }
 #pragma unroll
             for (int u = 0; u < kPer; u++) {
-                const float f = weight[w * ROWS + min(i0 + u * kTcThreads * p.splits, total4 - 1) / (HDP / 4)];
+                const float f = weight[n * ROWS + min(i0 + u * kTcThreads * p.splits, total4 - 1) / (HDP / 4)];
                 o[u].x = __fmaf_rn(f, x[u].x, o[u].x);
                 o[u].y = __fmaf_rn(f, x[u].y, o[u].y);
                 o[u].z = __fmaf_rn(f, x[u].z, o[u].z);
@@ -774,6 +778,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
     cluster.sync();  // no CTA leaves while a sister reads its shared memory
 }
 
+static int slots(const void *kernel, int n, size_t smem) { return cluster_slots(kernel, n, kTcThreads, smem); }
+
 template <typename T, int QP, int PP, int BITS, int HDP, int MT>
 static cudaError_t launch(AttnParams p, int max_len, cudaStream_t stream) {
     using S = TcSmem<QP, BITS, HDP, MT>;
@@ -781,33 +787,20 @@ static cudaError_t launch(AttnParams p, int max_len, cudaStream_t stream) {
     constexpr size_t smem = S::kBytes > 116 * 1024 ? S::kBytes : 116 * 1024;
     auto kernel = tree_attention_tc_kernel<T, QP, PP, BITS, HDP, MT>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
     p.qtiles = (int)(((long long)p.max_new * p.group + MT * 128 - 1) / (MT * 128));
     if ((long long)p.qtiles * p.kv_heads > 65535) return cudaErrorInvalidConfiguration;
     const long long base = (long long)p.qtiles * p.kv_heads * p.bt.batch;
-    // Split a sequence over the CTAs of a cluster so that the estimated time is least: jobs of max_len / splits keys (in
-    // steps) and kFixed steps of starting, filling and joining; three quarters of the longest length on average; the
-    // last jobs end a third of a job apart. (Clusters of 4 and 8 reach 132 and 120 of the 148 SMs. 16 sequences of up to
-    // 16,000 keys, 8 kv heads: 350, 197, 253, 353 us with 1, 2, 4, 8.)
-    constexpr double kFixed = 8;
-    const double steps = (double)max_len / kBN;
-    int splits = 1;
-    double least = 1e30;
-    for (int n = 1; n <= 8; n *= 2) {
-        if (n > 1 && steps < 4 * n) break;
-        const double job = steps / n + kFixed, slots = n <= 2 ? 148 : n == 4 ? 132 : 120, load = 0.75 * base * n / slots;
-        const double t = (load > 1 ? load : 1) * job + job / 3;
-        if (t < least) least = t, splits = n;
-    }
-    p.splits = splits;
+    p.splits = choose_splits(base, p.bt.batch, (double)max_len / kBN, 8.0, 4.0, [&](int n) { return slots((const void *)kernel, n, smem); });
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(splits, p.kv_heads * p.qtiles, p.bt.batch);
+    cfg.gridDim = dim3(p.splits, p.kv_heads * p.qtiles, p.bt.batch);
     cfg.blockDim = dim3(kTcThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = splits;
+    attr[0].val.clusterDim.x = p.splits;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;

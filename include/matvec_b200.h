@@ -186,8 +186,8 @@ int mvb_gemm_status(void *stream);
 
 /* ---- Serving operators: rotary positions, a paged 8- or 4-bit cache, attention over it, log probabilities ----
  * No counterpart in the reference, whose cache is fp32 inside its forward pass. Device pointers, asynchronous on
- * `stream`, on the current device; 0, or -1 with the reason in mvb_last_error(). No call keeps state or needs a workspace, so
- * calls on several streams or in several graphs do not meet. Strides are in elements.
+ * `stream`, on the current device; 0, or -1 with the reason in mvb_last_error(). No call keeps state, so calls on several
+ * streams or in several graphs do not meet. Strides are in elements.
  *
  * dtype of queries, keys, values, outputs and logits: MVB_F32, MVB_BF16 or MVB_F16.
  * Cache: kq, vq hold pages x kv_heads x page rows of head integers (bits 8: int8; bits 4: two's complement nibbles, element
@@ -232,12 +232,15 @@ int mvb_kv_read(const void *kq, const float *ks, const void *vq, const float *vs
  * token (NULL: each sees those before it and itself). heads is a multiple of kv_heads. max_new: at least the most new
  * tokens of a sequence (sequences with more are left out and reported); max_len: about the longest lens[b] + new tokens,
  * which only decides how the work is split. lse (may be NULL): rows x heads, the natural log of the sum of exponentials. A
- * row that sees nothing gives zeros and -inf. fp32 inputs give fp32-accurate results; the same call gives the same bits. */
+ * row that sees nothing gives zeros and -inf. fp32 inputs give fp32-accurate results; the same call gives the same bits.
+ * work (may be NULL; 16-byte aligned): room of work_bytes for this call alone until it has run; with it, few sequences with
+ * long contexts are split over more SMs. mvb_tree_attention_work gives the bytes worth having for such sizes, or 0. */
+size_t mvb_tree_attention_work(int rows, int heads, int kv_heads, int head, int batch, int max_new, int max_len);
 int mvb_tree_attention(const void *q, long long q_stride, const void *kq, const float *ks, const void *vq, const float *vs,
                        int pages, int page, int kv_heads, int head, int bits, const int *table, int table_cols,
                        const int *cu, const int *lens, int batch, int rows, int heads, int dtype, const void *tree,
                        int words, float scale, int max_new, int max_len, void *out, long long out_stride, float *lse,
-                       void *stream);
+                       void *work, size_t work_bytes, void *stream);
 
 /* Rows of logits (vocab <= 2^21, any stride): logp[r * nids + i] = log softmax at ids[r * nids + i] (-1: 0; outside the
  * vocabulary: NaN, reported), entropy[r] (may be NULL) in nats, and the `top` (<= 64) largest logits' ids and log

@@ -136,7 +136,9 @@ def lib():
         L.mvb_kv_read.argtypes = [vp] * 4 + [i] * 5 + [vp, i, vp, vp, i, i, vp, ll, vp, ll, i, vp]
         L.mvb_tree_attention.restype = i
         L.mvb_tree_attention.argtypes = ([vp, ll] + [vp] * 4 + [i] * 5 + [vp, i, vp, vp] + [i] * 4 +
-                                         [vp, i, f, i, i, vp, ll, vp, vp])
+                                         [vp, i, f, i, i, vp, ll, vp, vp, C.c_size_t, vp])
+        L.mvb_tree_attention_work.restype = C.c_size_t
+        L.mvb_tree_attention_work.argtypes = [i] * 7
         L.mvb_logprobs.restype = i
         L.mvb_logprobs.argtypes = [vp, ll, i, i, i, vp, i, vp, vp, i, vp, vp, vp]
         L.mvb_serve_status.restype = i

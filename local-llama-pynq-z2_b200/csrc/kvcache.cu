@@ -41,15 +41,6 @@ struct KvParams {
     int tokens_per_block;
 };
 
-// One element before quantization: x itself, or x c + y s (a turned key), in fp64 (rounded once: both products are exact).
-struct Exact {
-    float x, y, c, s;
-    bool turn;
-    __device__ __forceinline__ double value() const {
-        return turn ? __fma_rn((double)x, (double)c, __dmul_rn((double)y, (double)s)) : (double)x;
-    }
-};
-
 // rint(x / scale) in fp64, at most MOST.
 template <int MOST>
 __device__ __noinline__ float quotient(double x, float scale) {
@@ -59,19 +50,21 @@ __device__ __noinline__ float quotient(double x, float scale) {
 
 // Quantizes the rows of a warp (W lanes a row, E elements a lane) and stores integers and scale. f: the elements in fp32
 // (with TURN, turned keys within 1.5 ulp of the larger product, else the elements themselves); exact(k): element k in
-// fp64. Every lane of the warp takes part; lanes with on = false hold zeros and store nothing.
+// fp64, read again from memory, for the few that need it. Every lane of the warp takes part; lanes with on = false hold
+// zeros and store nothing.
 //
 // scale: of turned keys, |f| finds the candidates for the largest element (within 1e-6 of the largest, which covers f's
-// error; nearly always one lane of the row), their fp64 values decide; rounding to fp32 is monotonic, so the largest of the
-// rounded quotients is the rounded largest quotient. (The fp32 division rounds the quotient of an fp32 element as the
+// error; nearly always one element of the row), their fp64 values decide; rounding to fp32 is monotonic, so the largest of
+// the rounded quotients is the rounded largest quotient. (The fp32 division rounds the quotient of an fp32 element as the
 // fp64 one followed by a rounding does: 53 bits are enough for that.)
-// integers: y = f * (1 / scale) is within 127 * 2^-21 < 6.1e-5 of x / scale, which decides all but the values within 1e-4
-// of a border; those take the fp64 quotient, as do scales whose reciprocal leaves fp32's range. Adding 1.5 * 2^23 rounds y
-// to an integer (ties to even) that stands in the sum's low byte.
+// integers: y = f * (1 / scale) is within MOST * 2^-21 (6.1e-5 for 8 bits) of x / scale, which decides all but the values
+// nearer than kNear to a border (1 in 5,000); those take the fp64 quotient, as do scales whose reciprocal leaves fp32's
+// range. Adding 1.5 * 2^23 rounds y to an integer (ties to even) that stands in the sum's low byte.
 template <int W, int BITS, bool TURN, int E, typename F>
 __device__ __forceinline__ void quantize_store(const Row<E> &f, const F &exact, bool on, int l, uint8_t *row,
                                                float *scale_at) {
     constexpr int MOST = BITS == 8 ? 127 : 7;
+    constexpr float kNear = MOST * 7.9e-7f;
     uint32_t mine = 0;  // |f| as bits: infinities and NaN come out largest
 #pragma unroll
     for (int k = 0; k < E; k++) mine = max(mine, __float_as_uint(f.v[k]) & 0x7FFFFFFFu);
@@ -84,10 +77,15 @@ __device__ __forceinline__ void quantize_store(const Row<E> &f, const F &exact, 
     if (TURN) {
         const float near = m - fmaxf(m * 1e-6f, 1e-44f);
         scale = 0.0f;
-        if (__uint_as_float(mine) >= near) {
-            double best = 0.0;
+        if (__uint_as_float(mine) >= near && on && !bad) {
+            uint32_t candidates = 0;
 #pragma unroll
-            for (int k = 0; k < E; k++) best = fmax(best, fabs(exact(k)));
+            for (int k = 0; k < E; k++) candidates |= (uint32_t)(fabsf(f.v[k]) >= near) << k;
+            double best = 0.0;
+            do {
+                best = fmax(best, fabs(exact(__ffs(candidates) - 1)));
+                candidates &= candidates - 1;
+            } while (candidates);
             scale = best > 0.0 ? __double2float_rn(__ddiv_rn(best, (double)MOST)) : 0.0f;
         }
 #pragma unroll
@@ -95,7 +93,8 @@ __device__ __forceinline__ void quantize_store(const Row<E> &f, const F &exact, 
     } else {
         scale = __fdiv_rn(m, (float)MOST);
     }
-    const float inv = __frcp_rn(scale);
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));  // 1 ulp
     uint32_t n[E];
     float far = scale >= 1e-36f ? 0.0f : 1.0f;  // the largest distance from an integer
 #pragma unroll
@@ -104,9 +103,13 @@ __device__ __forceinline__ void quantize_store(const Row<E> &f, const F &exact, 
         far = fmaxf(far, fabsf(__fsub_rn(y, __fsub_rn(t, 12582912.0f))));
         n[k] = __float_as_uint(t);
     }
-    if (far > 0.4999f && !bad) {
+    if (far > 0.5f - kNear && !bad && on) {
 #pragma unroll
-        for (int k = 0; k < E; k++) n[k] = __float_as_uint(__fadd_rn(quotient<MOST>(exact(k), scale), 12582912.0f));
+        for (int k = 0; k < E; k++) {
+            const float y = __fmul_rn(f.v[k], inv), d = __fsub_rn(y, __fsub_rn(__fadd_rn(y, 12582912.0f), 12582912.0f));
+            if (!(scale >= 1e-36f) || fabsf(d) > 0.5f - kNear)
+                n[k] = __float_as_uint(__fadd_rn(quotient<MOST>(exact(k), scale), 12582912.0f));
+        }
     }
     if (!on) return;
     if (BITS == 8) {
@@ -133,30 +136,32 @@ template <typename T, int W, int BITS, int E>
 __global__ void __launch_bounds__(256, 3) kv_append_kernel(const KvParams p) {
     constexpr int R = 32 / W;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane & (W - 1), sub = lane / W;
-    const long long item = (long long)blockIdx.x * 8 + warp;
-    // chunk by chunk, so that the warps of a block do alike work (a block of both kinds keeps its queries' warps waiting
-    // idle for those that quantize: 14,000 rows of 32 + 8 heads took 179 us so)
-    const int chunk = (int)(item / p.rows), tok = (int)(item - (long long)chunk * p.rows);
-    if (chunk >= p.chunks || tok >= p.bt.cu[p.bt.batch]) return;  // rows behind the last sequence stay as they are
+    // a block's warps do alike work on neighbouring tokens (a block of both kinds keeps its queries' warps waiting idle for
+    // those that quantize: 14,000 rows of 32 + 8 heads took 179 us so)
+    const int chunk = blockIdx.y;
+    const long long tok = (long long)blockIdx.x * 8 + warp;
+    if (tok >= p.rows || tok >= p.bt.cu[p.bt.batch]) return;  // rows behind the last sequence stay as they are
     const bool on = E * l < p.head, in_rot = E * l < p.rot;
     const bool is_q = chunk >= p.kv_chunks;
     int b = 0;
     long long at = 0;
     if (!is_q || !p.pos) {
-        b = sequence_of(p.bt.cu, p.bt.batch, tok);
+        b = sequence_of(p.bt.cu, p.bt.batch, (int)tok);
         if (b >= p.bt.batch) return;
         at = (long long)p.bt.lens[b] + tok - p.bt.cu[b];
     }
     Turn<E> t;
 #pragma unroll
     for (int k = 0; k < E; k++) t.c[k] = 1.0f, t.s[k] = 0.0f;
+    const float *trow = nullptr;
     if (p.rope) {
         const long long pos = p.pos ? p.pos[tok] : at;
         if (pos < 0 || pos >= p.table_rows) {
             if (lane == 0) note(&g_kv_error, kBadPosition);
             return;
         }
-        t = load_turn<E>(p.rope + pos * p.rot, l, p.rot, p.pairs);
+        trow = p.rope + pos * p.rot;
+        t = load_turn<E>(trow, l, p.rot, p.pairs);
     }
     if (is_q) {
         const int h0 = (chunk - p.kv_chunks) * p.q_per;
@@ -167,21 +172,35 @@ __global__ void __launch_bounds__(256, 3) kv_append_kernel(const KvParams p) {
     }
     const int h = chunk * R + sub;
     const bool live = on && h < p.kv_heads;
-    const size_t src = (size_t)h * p.head + E * l;
-    const Row<E> k = load_row<E>(static_cast<const T *>(p.k) + tok * p.k_stride + src, live);
-    const Row<E> v = load_row<E>(static_cast<const T *>(p.v) + tok * p.v_stride + src, live);
+    const size_t src = (size_t)min(h, p.kv_heads - 1) * p.head;
+    const T *kr = static_cast<const T *>(p.k) + tok * p.k_stride + src, *vr = static_cast<const T *>(p.v) + tok * p.v_stride + src;
+    const Row<E> k = load_row<E>(kr + E * l, live), v = load_row<E>(vr + E * l, live);
     const long long slot = at > INT_MAX ? -1 : slot_of(p.bt, b, (int)at, &g_kv_error);
     if (slot < 0) return;
     const size_t page = (size_t)(slot >> p.bt.page_log2);
     const size_t row = ((page * p.kv_heads + min(h, p.kv_heads - 1)) << p.bt.page_log2) +
                        (size_t)(slot & ((1 << p.bt.page_log2) - 1));
     const int row_bytes = p.head * BITS / 8;
-    quantize_store<W, BITS, false>(v, [&](int i) { return (double)v.v[i]; }, live, l, p.vq + row * row_bytes, p.vs + row);
-    const Row<E> y = p.rope ? partners<W>(k, l, p.rot, p.pairs) : k;
-    const Row<E> f = p.rope ? turned(k, y, t, in_rot) : k;
-    auto exact = [&](int i) { return Exact{k.v[i], y.v[i], t.c[i], t.s[i], p.rope && in_rot}.value(); };
-    if (p.rope) quantize_store<W, BITS, true>(f, exact, live, l, p.kq + row * row_bytes, p.ks + row);
-    else quantize_store<W, BITS, false>(f, exact, live, l, p.kq + row * row_bytes, p.ks + row);
+    quantize_store<W, BITS, false>(v, [&](int i) { return (double)to_f32(vr[E * l + i]); }, live, l, p.vq + row * row_bytes,
+                                   p.vs + row);
+    if (p.rope) {
+        const Row<E> y = partners<W>(k, l, p.rot, p.pairs);
+        // both products of an fp32 element and an fp32 cosine are exact in fp64: one rounding
+        auto exact = [&](int i) {
+            const int e = E * l + i;
+            const double x = to_f32(kr[e]);
+            if (e >= p.rot) return x;
+            const bool first = p.pairs ? !(e & 1) : 2 * e < p.rot;
+            const int angle = p.pairs ? e / 2 : first ? e : e - p.rot / 2;
+            const double other = to_f32(kr[p.pairs ? e ^ 1 : first ? e + p.rot / 2 : e - p.rot / 2]);
+            const double s = trow[p.rot / 2 + angle];
+            return __fma_rn(x, (double)trow[angle], __dmul_rn(other, first ? -s : s));
+        };
+        quantize_store<W, BITS, true>(turned(k, y, t, in_rot), exact, live, l, p.kq + row * row_bytes, p.ks + row);
+    } else {
+        quantize_store<W, BITS, false>(k, [&](int i) { return (double)to_f32(kr[E * l + i]); }, live, l,
+                                       p.kq + row * row_bytes, p.ks + row);
+    }
 }
 
 // Eight elements of a cached row (integer * scale, rounded once to fp32, once more to a 16-bit output).
@@ -278,7 +297,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvParams p) {
 }
 
 template <typename T, int BITS, int E>
-static void launch_lanes(const KvParams &p, unsigned grid, cudaStream_t s) {
+static void launch_lanes(const KvParams &p, dim3 grid, cudaStream_t s) {
     const int lanes = (p.head + E - 1) / E;  // the fewest lanes that hold a row
     if (lanes <= 8) kv_append_kernel<T, 8, BITS, E><<<grid, 256, 0, s>>>(p);
     else if (lanes <= 16) kv_append_kernel<T, 16, BITS, E><<<grid, 256, 0, s>>>(p);
@@ -286,7 +305,7 @@ static void launch_lanes(const KvParams &p, unsigned grid, cudaStream_t s) {
 }
 
 template <typename T, int BITS>
-static void launch_append(const KvParams &p, unsigned grid, bool wide, cudaStream_t s) {
+static void launch_append(const KvParams &p, dim3 grid, bool wide, cudaStream_t s) {
     if constexpr (sizeof(T) == 2) {
         if (wide) return launch_lanes<T, BITS, 8>(p, grid, s);
     }
@@ -408,13 +427,12 @@ extern "C" int mvb_kv_append(void *kq, float *ks, void *vq, float *vs, int pages
     p.q_per = full ? 8 * r : r;
     p.kv_chunks = (kv_heads + r - 1) / r;
     p.chunks = p.kv_chunks + (p.heads + p.q_per - 1) / p.q_per;
-    const long long blocks = ((long long)rows * p.chunks + 7) / 8;
-    if (blocks > INT_MAX) {
-        set_error("%s: rows=%d are too many for one call", who, rows);
+    if (p.chunks > 65535) {
+        set_error("%s: kv_heads=%d heads=%d are too many for one call", who, kv_heads, p.heads);
         return -1;
     }
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const unsigned grid = (unsigned)blocks;
+    const dim3 grid((unsigned)(((long long)rows + 7) / 8), p.chunks);
     if (bits == 8) {
         if (dtype == kF32) launch_append<float, 8>(p, grid, wide, s);
         else if (dtype == kBF16) launch_append<__nv_bfloat16, 8>(p, grid, wide, s);

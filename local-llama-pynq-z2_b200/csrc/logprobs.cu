@@ -4,11 +4,12 @@
 //     entropy = -sum p ln p = ln z - (sum (x - m) exp(x - m)) / z
 //     top: the `top` largest logits by (value, lowest index first), with their log probabilities
 //
-// One pass over the logits: each thread keeps (m, z, w = sum (x - m) exp(x - m)) of its elements, moved to a new maximum
-// once per 4 vectors, and for the top tokens only the maximum of those 4 vectors (one shared-memory word per 16 or 32
-// elements), so that the streaming loop has no candidate lists and no barriers. Afterwards the top-th largest of the
-// threads' own maxima is a lower bound of the top-th largest element; the few vectors whose maximum reaches it are read
-// again (from L2) and their elements that reach it ranked. Rows with more such elements than the list holds (a
+// One pass over the logits: each thread keeps (m, z, w = sum (x - m) exp(x - m)) of its elements (m starts as its warp's
+// first maximum and moves only when it is 4 behind), and for the top tokens only the maximum of each 4 vectors (one
+// shared-memory word per 16 or 32 elements), so that the streaming loop has no candidate lists and no barriers. Afterwards
+// the top-th largest of the threads' own maxima (its 16 leading bits) is a lower bound of the top-th largest element; the
+// few groups whose maximum reaches it are listed, their vectors read again (from L2), a thread each, and their elements
+// that reach it ranked. Rows with more such elements than the list holds (a
 // vocabulary masked to a few tokens: the rest all equal) take the elements above the bound, then those equal to it in
 // the order of their index; where even the former overflow, `top` rounds of an arg max.
 // A few rows: a row is split over a cluster of up to 16 CTAs, joined through distributed shared memory in rank order.
@@ -32,6 +33,8 @@ static __device__ int g_logp_error;
 constexpr int kVecs = 4;      // 16-byte vectors a thread has in flight (a group: one maximum)
 constexpr int kList = 2048;   // candidates
 constexpr int kMostTop = 64;
+constexpr int kGroups = 512;    // groups that are read again, listed; more are scanned by their own threads
+constexpr float kBehind = 4.0f;
 constexpr float kLog2e = 1.44269504088896341f;
 
 struct Params {
@@ -190,6 +193,9 @@ __device__ __forceinline__ uint4 load_stream(const uint4 *p) {
 template <typename T, bool TOP, int kThreads>
 __global__ void __launch_bounds__(kThreads, 768 / kThreads) logprobs_kernel(const Params p) {
     constexpr int N = Vec<T>::kN;
+    // turns of the streaming loop that share a maximum: 32 elements of a thread (with 16 for fp32 the maxima of a 151,936
+    // word vocabulary take 38 KB and two thirds of the threads fit)
+    constexpr int kTurns = sizeof(T) / 2, kGroupVecs = kVecs * kTurns;
     extern __shared__ __align__(16) float group_max[];  // [iters][kThreads], TOP only
     __shared__ Sums parts[kThreads / 32];
     __shared__ Sums cta_sums;
@@ -197,7 +203,8 @@ __global__ void __launch_bounds__(kThreads, 768 / kThreads) logprobs_kernel(cons
     __shared__ unsigned long long list[TOP ? kList : 1], best[TOP ? kMostTop : 1];
     __shared__ unsigned long long round_best[kThreads / 32];
     __shared__ float bound;
-    __shared__ int count, above, taken, warp_count[kThreads / 32];
+    __shared__ int count, above, taken, listed, warp_count[kThreads / 32];
+    __shared__ uint16_t groups[TOP ? kGroups : 1];
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int row = blockIdx.x / p.splits, split = blockIdx.x - row * p.splits;
@@ -214,13 +221,14 @@ __global__ void __launch_bounds__(kThreads, 768 / kThreads) logprobs_kernel(cons
     float mine = -INFINITY;  // this thread's largest element of the vectors
     int seen = 0;
     int v = v0 + tid;
-    // whole groups of kVecs vectors
+    // whole groups of kVecs vectors, the same number for every thread
+    const int whole = (v1 - v0) / (kVecs * kThreads);
     uint4 next[kVecs];  // the group after this one, on its way
-    if (v + (kVecs - 1) * kThreads < v1) {
+    if (whole > 0) {
 #pragma unroll
         for (int k = 0; k < kVecs; k++) next[k] = load_stream(vec + v + k * kThreads);
     }
-    for (; v + (kVecs - 1) * kThreads < v1; v += kVecs * kThreads, seen++) {
+    for (; seen < whole; v += kVecs * kThreads, seen++) {
         uint32_t u[4 * kVecs];
 #pragma unroll
         for (int k = 0; k < kVecs; k++) {
@@ -229,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, 768 / kThreads) logprobs_kernel(cons
             u[4 * k + 2] = next[k].z;
             u[4 * k + 3] = next[k].w;
         }
-        if (v + (2 * kVecs - 1) * kThreads < v1) {
+        if (seen + 1 < whole) {
 #pragma unroll
             for (int k = 0; k < kVecs; k++) next[k] = load_stream(vec + v + (kVecs + k) * kThreads);
         }
@@ -238,9 +246,18 @@ __global__ void __launch_bounds__(kThreads, 768 / kThreads) logprobs_kernel(cons
         for (int k = 2; k < 4 * kVecs; k++) gm[k & 1] = Word<T>::larger(gm[k & 1], u[k]);
         gm[0] = Word<T>::larger(gm[0], gm[1]);
         const float g = fmaxf(fmaxf(Word<T>::first(gm[0]), Word<T>::second(gm[0])), -INFINITY);
-        if (TOP) group_max[seen * kThreads + tid] = g;
+        if (TOP) {
+            float &gm_at = group_max[seen / kTurns * kThreads + tid];
+            gm_at = seen % kTurns ? fmaxf(gm_at, g) : g;
+        }
         mine = fmaxf(mine, g);
-        if (g > s.m) move_to(s, g);
+        if (seen == 0) {
+            float first = g;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) first = fmaxf(first, __shfl_xor_sync(0xffffffffu, first, o));
+            s.m = first;
+        }
+        if (g > s.m + kBehind) move_to(s, g);
         if (s.m > Word<T>::kSane) {
             const uint64_t base = pair(-s.m, -s.m), l2e = pair(kLog2e, kLog2e);
             uint64_t z[2] = {0, 0}, w[2] = {0, 0};
@@ -287,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 768 / kThreads) logprobs_kernel(cons
 #pragma unroll
             for (int i = 1; i < N; i++) gv = fmaxf(gv, f[i]);
             g = fmaxf(g, gv);
-            if (gv > s.m) move_to(s, gv);
+            if (gv > s.m + kBehind) move_to(s, gv);
             const float base = s.m == -INFINITY ? 0.0f : s.m;
 #pragma unroll
             for (int i = 0; i < N; i++) {
@@ -296,32 +313,47 @@ __global__ void __launch_bounds__(kThreads, 768 / kThreads) logprobs_kernel(cons
                 s.w = __fmaf_rn(d, e, s.w);
             }
         }
-        if (TOP) group_max[seen * kThreads + tid] = g;
+        if (TOP) {
+            float &gm_at = group_max[seen / kTurns * kThreads + tid];
+            gm_at = seen % kTurns ? fmaxf(gm_at, g) : g;
+        }
         mine = fmaxf(mine, g);
         seen++;
     }
     if (split == 0 && tid < edge) {
         const float f = to_f32(x[edge_at(tid)]);
-        if (f > s.m) move_to(s, f);
+        if (f > s.m + kBehind) move_to(s, f);
         const float d = below(f, s.m == -INFINITY ? 0.0f : s.m), e = exp_fast(d);
         s.z += e;
         s.w = __fmaf_rn(d, e, s.w);
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const Sums t = {__shfl_xor_sync(0xffffffffu, s.m, o), __shfl_xor_sync(0xffffffffu, s.z, o),
-                        __shfl_xor_sync(0xffffffffu, s.w, o)};
-        s = joined(s, t);
+    // the given tokens' logits, on their way while the rest is joined
+    float given = 0.0f;
+    int id = -1;
+    if (split == 0 && tid < p.nids) {
+        id = p.ids[(size_t)row * p.nids + tid];
+        if ((unsigned)id < (unsigned)p.vocab) given = to_f32(x[id]);
     }
-    if (lane == 0) parts[warp] = s;
+    {  // the warp's sums: one move to its maximum, then plain sums
+        float m = s.m;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        move_to(s, m);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            s.z += __shfl_xor_sync(0xffffffffu, s.z, o);
+            s.w += __shfl_xor_sync(0xffffffffu, s.w, o);
+        }
+        if (lane == 0) parts[warp] = s;
+    }
     if (TOP) thread_max[tid] = mine;
     if (tid == 0) {
         bound = -INFINITY;
-        count = above = taken = 0;
+        count = above = taken = listed = 0;
     }
     if (TOP && tid < kMostTop) best[tid] = 0;
     __syncthreads();
-    if (tid == 0) {
+    if (warp == 1 && lane == 0) {
         Sums t = parts[0];
 #pragma unroll
         for (int w = 1; w < kThreads / 32; w++) t = joined(t, parts[w]);
@@ -357,13 +389,35 @@ __global__ void __launch_bounds__(kThreads, 768 / kThreads) logprobs_kernel(cons
             const float v = to_f32(x[edge_at(tid)]);
             if (v >= bd) offer(v, edge_at(tid));
         }
-        for (int it = 0; it < seen; it++) {
+        const int entries = (seen + kTurns - 1) / kTurns;
+        if (mine >= bd) {
+#pragma unroll 8
+            for (int it = 0; it < entries; it++)
+                if (group_max[it * kThreads + tid] >= bd) {
+                    const int at = atomicAdd(&listed, 1);
+                    if (at < kGroups) groups[at] = (uint16_t)(it * kThreads + tid);
+                }
+        }
+        __syncthreads();
+        const int ng = listed;
+        if (ng <= kGroups) {  // the groups' vectors, a thread each
+            for (int i = tid; i < ng * kGroupVecs; i += kThreads) {
+                const int g = groups[i / kGroupVecs];
+                const int v = v0 + g % kThreads + ((g / kThreads) * kGroupVecs + i % kGroupVecs) * kThreads;
+                if (v >= v1) continue;
+                float f[N];
+                unpack<T>(vec[v], f);
+#pragma unroll
+                for (int e = 0; e < N; e++)
+                    if (f[e] >= bd) offer(f[e], head + v * N + e);
+            }
+        } else for (int it = 0; it < entries; it++) {
             if (!(group_max[it * kThreads + tid] >= bd)) continue;
             if (*(volatile int *)&count > kList) {  // only the number above the bound matters now
                 if (!(group_max[it * kThreads + tid] > bd)) continue;
             }
-            const int v = v0 + tid + it * kVecs * kThreads;
-            for (int k = 0; k < kVecs && v + k * kThreads < v1; k++) {
+            const int v = v0 + tid + it * kGroupVecs * kThreads;
+            for (int k = 0; k < kGroupVecs && v + k * kThreads < v1; k++) {
                 float f[N];
                 unpack<T>(vec[v + k * kThreads], f);
 #pragma unroll
@@ -384,10 +438,10 @@ __global__ void __launch_bounds__(kThreads, 768 / kThreads) logprobs_kernel(cons
                 if (v > bd) list[atomicAdd(&count, 1)] = key_of(v, i);
             };
             if (split == 0 && tid < edge) above_only(to_f32(x[edge_at(tid)]), edge_at(tid));
-            for (int it = 0; it < seen; it++) {
+            for (int it = 0; it < entries; it++) {
                 if (!(group_max[it * kThreads + tid] > bd)) continue;
-                const int v = v0 + tid + it * kVecs * kThreads;
-                for (int k = 0; k < kVecs && v + k * kThreads < v1; k++) {
+                const int v = v0 + tid + it * kGroupVecs * kThreads;
+                for (int k = 0; k < kGroupVecs && v + k * kThreads < v1; k++) {
                     float f[N];
                     unpack<T>(vec[v + k * kThreads], f);
 #pragma unroll
@@ -496,12 +550,14 @@ __global__ void __launch_bounds__(kThreads, 768 / kThreads) logprobs_kernel(cons
     const float logz = all.z > 0.0f ? logf(all.z) : __int_as_float(0x7FC00000);
     if (tid == 0 && p.entropy) p.entropy[row] = logz - all.w / all.z;
     for (int i = tid; i < p.nids; i += kThreads) {
-        const int id = p.ids[(size_t)row * p.nids + i];
+        if (i != tid) {  // more tokens than threads
+            id = p.ids[(size_t)row * p.nids + i];
+            if ((unsigned)id < (unsigned)p.vocab) given = to_f32(x[id]);
+        }
         float r = 0.0f;  // -1: no token
         if (id != -1) {
-            if ((unsigned)id < (unsigned)p.vocab) {
-                r = (to_f32(x[id]) - all.m) - logz;
-            } else {
+            r = (given - all.m) - logz;
+            if ((unsigned)id >= (unsigned)p.vocab) {
                 r = __int_as_float(0x7FC00000);
                 note(&g_logp_error, kBadToken);
             }
@@ -517,7 +573,7 @@ __global__ void __launch_bounds__(kThreads, 768 / kThreads) logprobs_kernel(cons
 
 template <typename T, bool TOP, int kThreads>
 static cudaError_t launch_threads(Params p, cudaStream_t stream) {
-    constexpr int N = Vec<T>::kN, kChunk = kThreads * kVecs * N;
+    constexpr int kChunk = kThreads * 32;  // elements of a row of maxima: 32 a thread
     auto kernel = logprobs_kernel<T, TOP, kThreads>;
     // a row over more CTAs while the grid leaves SMs idle and each CTA still has a chunk, or where its maxima would not
     // fit in shared memory

@@ -41,10 +41,9 @@ struct RopeParams {
 template <typename T, int W, int E>
 __global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane & (W - 1), sub = lane / W;
-    const long long item = (long long)blockIdx.x * (blockDim.x / 32) + warp;
-    const long long tok = item / p.chunks;
+    const long long tok = (long long)blockIdx.x * 8 + warp;
     if (tok >= p.tokens) return;
-    const int h0 = (int)(item - tok * p.chunks) * p.heads_per_warp, h1 = min(h0 + p.heads_per_warp, p.heads);
+    const int h0 = blockIdx.y * p.heads_per_warp, h1 = min(h0 + p.heads_per_warp, p.heads);
     const int pos = p.pos[tok];
     if ((unsigned)pos >= (unsigned)p.table_rows) {
         if (lane == 0) note(&g_rope_error, kBadPosition);
@@ -56,7 +55,7 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
 }
 
 template <typename T, int E>
-static void launch_lanes(const RopeParams &p, unsigned grid, cudaStream_t s) {
+static void launch_lanes(const RopeParams &p, dim3 grid, cudaStream_t s) {
     // the fewest lanes that hold a row
     const int lanes = (p.head + E - 1) / E;
     if (lanes <= 8) rope_kernel<T, 8, E><<<grid, 256, 0, s>>>(p);
@@ -65,7 +64,7 @@ static void launch_lanes(const RopeParams &p, unsigned grid, cudaStream_t s) {
 }
 
 template <typename T>
-static void launch_rope(const RopeParams &p, unsigned grid, bool wide, cudaStream_t s) {
+static void launch_rope(const RopeParams &p, dim3 grid, bool wide, cudaStream_t s) {
     if constexpr (sizeof(T) == 2) {
         if (wide) return launch_lanes<T, 8>(p, grid, s);
     }
@@ -153,15 +152,15 @@ extern "C" int mvb_rope(const void *x, const int *pos, const float *table, void 
     // a whole token a warp when there are tokens enough to fill the machine, else fewer heads a warp (latency)
     p.heads_per_warp = tokens >= 148 * 24 ? heads : (long long)tokens * heads >= 148ll * 64 * 4 * r ? 4 * r : r;
     p.chunks = (heads + p.heads_per_warp - 1) / p.heads_per_warp;
-    const long long blocks = ((long long)tokens * p.chunks + 7) / 8;
-    if (blocks > INT_MAX) {
-        set_error("mvb_rope: tokens=%d heads=%d are too many for one call", tokens, heads);
+    if (p.chunks > 65535) {
+        set_error("mvb_rope: heads=%d are too many for one call", heads);
         return -1;
     }
+    const dim3 grid((unsigned)(((long long)tokens + 7) / 8), p.chunks);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (dtype == kF32) launch_rope<float>(p, (unsigned)blocks, wide, s);
-    else if (dtype == kBF16) launch_rope<__nv_bfloat16>(p, (unsigned)blocks, wide, s);
-    else launch_rope<__half>(p, (unsigned)blocks, wide, s);
+    if (dtype == kF32) launch_rope<float>(p, grid, wide, s);
+    else if (dtype == kBF16) launch_rope<__nv_bfloat16>(p, grid, wide, s);
+    else launch_rope<__half>(p, grid, wide, s);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) {
         set_error("mvb_rope: launch failed: %s", cudaGetErrorString(e));

@@ -112,14 +112,15 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 && NT <= 2 ? 2 : 1) t
     uint8_t *pipe = smem + QP * NT * KS * 256;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-    const int b = blockIdx.z, kvh = blockIdx.y / p.qtiles, qt = blockIdx.y - kvh * p.qtiles, split = blockIdx.x;
+    const int b = blockIdx.z, kvh = blockIdx.y / p.qtiles, qt = blockIdx.y - kvh * p.qtiles;
+    const int split = blockIdx.x % p.splits, super = blockIdx.x / p.splits;
     const Sequence s = sequence_at(p, b, &g_attn_error);
     const int nrows = s.n * p.group, R0 = qt * ROWS;
     if (R0 >= nrows) return;  // the whole cluster returns together
 
     // this warp's slices
     const int ns = (s.len + S::kKeys - 1) / S::kKeys;
-    const int s0 = (int)((long long)ns * split / p.splits), s1 = (int)((long long)ns * (split + 1) / p.splits);
+    const int s0 = (int)((long long)ns * blockIdx.x / gridDim.x), s1 = (int)((long long)ns * (blockIdx.x + 1) / gridDim.x);
     const int row_bytes = p.head * BITS / 8, piece = row_bytes % 16 ? 8 : 16;
     uint8_t *mine = pipe + warp * S::kWarp;
     const uint32_t mine_u = (uint32_t)__cvta_generic_to_shared(mine);
@@ -475,6 +476,14 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 && NT <= 2 ? 2 : 1) t
     auto finish = [&](int row, int d4, float4 o, float sum, float mm) {
         const int R = R0 + row, tok = s.row0 + R / p.group, head = kvh * p.group + R % p.group;
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key: o is zero too
+        if (p.supers > 1) {
+            const size_t at = ((size_t)super * p.rows + tok) * p.heads + head;
+            if (4 * d4 < p.head)
+                *reinterpret_cast<float4 *>(p.work + at * p.head + 4 * d4) =
+                    make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+            if (d4 == 0) work_ml(p)[at] = make_float2(mm, sum);
+            return;
+        }
         if (4 * d4 < p.head)
             store4(static_cast<T *>(p.out) + (size_t)tok * p.out_stride + (size_t)head * p.head + 4 * d4,
                    make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
@@ -544,6 +553,13 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 && NT <= 2 ? 2 : 1) t
     cluster.sync();  // no CTA leaves while a sister reads its shared memory
 }
 
+// How many clusters a sequence may be split over: as many as the caller's workspace holds parts of.
+int most_supers(const AttnParams &p) {
+    const size_t one = work_need(p, 1);
+    const size_t n = p.work && one ? p.work_bytes / one : 1;
+    return n < 2 ? 1 : n > kMaxSupers ? kMaxSupers : (int)n;
+}
+
 template <typename T, int BITS, int HDP, int NT, int kWarps>
 static cudaError_t launch_warps(AttnParams p, int max_len, cudaStream_t stream) {
     using S = Slice<HDP, BITS>;
@@ -558,11 +574,14 @@ static cudaError_t launch_warps(AttnParams p, int max_len, cudaStream_t stream) 
     if (e != cudaSuccess) return e;
     p.qtiles = (int)(((long long)p.max_new * p.group + ROWS - 1) / ROWS);
     if ((long long)p.qtiles * p.kv_heads > 65535) return cudaErrorInvalidConfiguration;
-    // a unit: one slice a warp; starting and joining a CTA cost about eight
-    p.splits = choose_splits((long long)p.qtiles * p.kv_heads * p.bt.batch, p.bt.batch, (double)max_len / (kWarps * S::kKeys), 8.0, 1.0,
-                             [&](int n) { return cluster_slots((const void *)kernel, n, kWarps * 32, smem); });
+    // a unit: one slice a warp, about 2 us of streaming; a CTA starts and joins in about 6 us, a second kernel in 4
+    const Split cut = choose_splits((long long)p.qtiles * p.kv_heads * p.bt.batch, p.bt.batch,
+                                    (double)max_len / (kWarps * S::kKeys), 3.0, 8.0, 2.0, 1.0, most_supers(p),
+                                    [&](int n) { return cluster_slots((const void *)kernel, n, kWarps * 32, smem); });
+    p.splits = cut.splits;
+    p.supers = cut.supers;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.splits, p.kv_heads * p.qtiles, p.bt.batch);
+    cfg.gridDim = dim3(p.splits * p.supers, p.kv_heads * p.qtiles, p.bt.batch);
     cfg.blockDim = dim3(kWarps * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
@@ -573,7 +592,8 @@ static cudaError_t launch_warps(AttnParams p, int max_len, cudaStream_t stream) 
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, p);
+    e = cudaLaunchKernelEx(&cfg, kernel, p);
+    return e == cudaSuccess && p.supers > 1 ? launch_join(p, rows::Type<T>::kId, stream) : e;
 }
 
 template <typename T, int BITS, int HDP, int NT>
@@ -604,6 +624,47 @@ static cudaError_t launch_size(const AttnParams &p, int max_len, cudaStream_t st
     // sequences of up to 2,000 keys, 46 and 54 against 50 and 50 for 16 of up to 4,000
     if ((long long)p.max_new * p.group > 24) return launch_tc(p, rows::Type<T>::kId, BITS, max_len, stream);
     return p.head <= 64 ? launch_rows<T, BITS, 64>(p, max_len, stream) : launch_rows<T, BITS, 128>(p, max_len, stream);
+}
+
+// One block a (new token, sequence): every head's parts, weighted by sum * 2^(max - largest).
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(const AttnParams p) {
+    const Sequence s = sequence_at(p, blockIdx.y, &g_attn_error);
+    if ((int)blockIdx.x >= s.n) return;
+    const int tok = s.row0 + blockIdx.x, quads = p.head / 4;
+    const float2 *ml = work_ml(p) + (size_t)tok * p.heads;
+    const size_t next = (size_t)p.rows * p.heads;  // rows of one part
+    for (int i = threadIdx.x; i < p.heads * quads; i += 256) {
+        const int head = i / quads, d4 = i - head * quads;
+        float m = -INFINITY, sum = 0.0f;
+        for (int w = 0; w < p.supers; w++) m = fmaxf(m, ml[w * next + head].x);
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+        for (int w = 0; w < p.supers; w++) {
+            const float2 x = ml[w * next + head];
+            const float4 v = *reinterpret_cast<const float4 *>(p.work + (w * next + (size_t)tok * p.heads + head) * p.head + 4 * d4);
+            if (x.y == 0.0f) continue;
+            const float f = x.y * exp2_fast(x.x - m);
+            sum += f;
+            o.x = __fmaf_rn(f, v.x, o.x);
+            o.y = __fmaf_rn(f, v.y, o.y);
+            o.z = __fmaf_rn(f, v.z, o.z);
+            o.w = __fmaf_rn(f, v.w, o.w);
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        store4(static_cast<T *>(p.out) + (size_t)tok * p.out_stride + (size_t)head * p.head + 4 * d4,
+               make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+        if (d4 == 0 && p.lse)
+            p.lse[(size_t)tok * p.heads + head] = sum == 0.0f ? -INFINITY : (m + log2f(sum)) * 0.693147180559945309f;
+    }
+}
+
+cudaError_t launch_join(const AttnParams &p, int dtype, cudaStream_t s) {
+    const dim3 grid(p.max_new, p.bt.batch);
+    if (dtype == kF32) join_kernel<float><<<grid, 256, 0, s>>>(p);
+    else if (dtype == kBF16) join_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(p);
+    else join_kernel<__half><<<grid, 256, 0, s>>>(p);
+    return cudaGetLastError();
 }
 
 int cluster_slots(const void *kernel, int n, int threads, size_t smem) {
@@ -657,11 +718,25 @@ int attn_take_error(cudaStream_t s) {
 using namespace mvb;
 using namespace mvb::attn;
 
+// Bytes of workspace that let a call of these sizes split its sequences over more SMs than clusters reach: for few jobs
+// (sequences x kv heads x tiles of query rows) with long contexts; 0 where a workspace would not be used.
+extern "C" size_t mvb_tree_attention_work(int rows, int heads, int kv_heads, int head, int batch, int max_new, int max_len) {
+    if (rows <= 0 || heads <= 0 || kv_heads <= 0 || head <= 0 || batch <= 0 || max_new <= 0) return 0;
+    const long long jobs = (long long)batch * kv_heads * (((long long)max_new * (heads / kv_heads) + 255) / 256);
+    if (jobs > 18 || max_len < 16384) return 0;
+    AttnParams p = {};
+    p.rows = rows;
+    p.heads = heads;
+    p.head = head;
+    return work_need(p, kMaxSupers);
+}
+
 extern "C" int mvb_tree_attention(const void *q, long long q_stride, const void *kq, const float *ks, const void *vq,
                                   const float *vs, int pages, int page, int kv_heads, int head, int bits,
                                   const int *table, int table_cols, const int *cu, const int *lens, int batch, int rows,
                                   int heads, int dtype, const void *tree, int words, float scale, int max_new,
-                                  int max_len, void *out, long long out_stride, float *lse, void *stream) {
+                                  int max_len, void *out, long long out_stride, float *lse, void *work,
+                                  size_t work_bytes, void *stream) {
     const char *who = "mvb_tree_attention";
     if (bits != 4 && bits != 8) {
         set_error("%s: unsupported bits=%d (need 4 or 8)", who, bits);
@@ -687,7 +762,7 @@ extern "C" int mvb_tree_attention(const void *q, long long q_stride, const void 
     if (!q || !out || !kq || !ks || !vq || !vs || !table || !cu || !lens || ((uintptr_t)q & need) ||
         ((uintptr_t)out & need) || ((uintptr_t)kq & 15) || ((uintptr_t)vq & 15) || ((uintptr_t)ks & 15) ||
         ((uintptr_t)vs & 15) || ((uintptr_t)table & 3) || ((uintptr_t)cu & 3) || ((uintptr_t)lens & 3) ||
-        ((uintptr_t)tree & 7) || ((uintptr_t)lse & 3) || q_stride % 4 || out_stride % 4) {
+        ((uintptr_t)tree & 7) || ((uintptr_t)lse & 3) || ((uintptr_t)work & 15) || q_stride % 4 || out_stride % 4) {
         set_error("%s: null or misaligned pointer or stride (cache 16 bytes, q and out four elements, tree 8)", who);
         return -1;
     }
@@ -721,6 +796,8 @@ extern "C" int mvb_tree_attention(const void *q, long long q_stride, const void 
     p.group = heads / kv_heads;
     p.head = head;
     p.max_new = max_new;
+    p.work = static_cast<float *>(work);
+    p.work_bytes = work ? work_bytes : 0;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t e;
     if (bits == 8)

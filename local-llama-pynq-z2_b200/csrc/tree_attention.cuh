@@ -15,8 +15,23 @@ struct AttnParams {
     const unsigned long long *tree;  // or null: each new token sees those before it and itself
     long long q_stride, out_stride;
     float scale_log2;  // the softmax scale times log2(e)
-    int words, rows, heads, kv_heads, group, head, max_new, qtiles, splits;
+    int words, rows, heads, kv_heads, group, head, max_new, qtiles;
+    // A sequence's keys lie over `splits` CTAs of a cluster (blockIdx.x % splits), joined there, and, where few sequences leave
+    // SMs idle that clusters do not reach, over `supers` such clusters (blockIdx.x / splits), whose results go to `work`
+    // and are joined by a second kernel: [supers][rows][heads] x head fp32, then [supers][rows][heads] x (max, sum).
+    int splits, supers;
+    float *work;
+    size_t work_bytes;
 };
+
+__device__ __forceinline__ float2 *work_ml(const AttnParams &p) {
+    return reinterpret_cast<float2 *>(p.work + (size_t)p.supers * p.rows * p.heads * p.head);
+}
+inline size_t work_need(const AttnParams &p, int supers) {
+    return (size_t)supers * p.rows * p.heads * (p.head + 2) * 4;
+}
+// The second kernel: p.supers parts of every row joined into p.out and p.lse.
+cudaError_t launch_join(const AttnParams &p, int dtype, cudaStream_t s);
 
 // One sequence of the batch, its index arrays checked (a value out of range is noted and clamped: no access leaves
 // the arrays, and mvb_serve_status tells).
@@ -85,29 +100,42 @@ __device__ __forceinline__ uint32_t nibbles_to_half2(uint32_t x, int k) {
     return h;
 }
 
-constexpr int kMaxSplits = 16;
+constexpr int kMaxSplits = 16, kMaxSupers = 8;
+int most_supers(const AttnParams &p);
 
 // CTAs of `kernel` in clusters of n that the current device holds at once (0 where none fits). Looked up once a kernel,
 // size and device: clusters live inside a GPC, so that sizes which do not divide its SMs leave some idle.
 int cluster_slots(const void *kernel, int n, int threads, size_t smem);
 
-// Over how many CTAs of a cluster a sequence's keys are split, so that the estimated time is least: `base` jobs without a
-// split, `steps` units of work each for the longest sequence, `fixed` units to start, fill and join a CTA, at least `least`
-// units a CTA. One sequence: its jobs are alike and run in whole waves. Several: three quarters of the longest on average,
-// in no order, and the last jobs end a third of a job apart.
+// Over how many CTAs of a cluster (splits) and how many clusters (supers, at most most_supers) a sequence's keys are split,
+// so that the estimated time is least: `base` jobs without a split, `steps` units of work each for the longest sequence,
+// `fixed` units to start, fill and join a CTA (`more` where the CTAs exceed one wave) and `join` for a second kernel, at
+// least `least` units a CTA. One
+// sequence: its jobs are alike and run in whole waves. Several: three quarters of the longest on average, in no order, and
+// the last jobs end a third of a job apart.
+struct Split {
+    int splits, supers;
+};
 template <typename F>
-inline int choose_splits(long long base, int batch, double steps, double fixed, double least, const F &slots_of) {
-    int best = 1;
+inline Split choose_splits(long long base, int batch, double steps, double fixed, double more, double join, double least,
+                           int most_supers,
+                           const F &slots_of) {
+    Split best = {1, 1};
     double best_time = 1e300;
     for (int n = 1; n <= kMaxSplits; n++) {
         if (n > 1 && steps < least * n) break;
         const int slots = slots_of(n);
         if (slots < n) continue;
-        const double job = steps / n + fixed, fill = (double)base * n / slots;
-        double time = job;
-        if (fill > 1.0) time = batch == 1 ? (double)((base * n + slots - 1) / slots) * job
-                                          : (0.75 * fill > 1.0 ? 0.75 * fill : 1.0) * job + job / 3;
-        if (time < best_time * 0.999) best_time = time, best = n;
+        for (int m = 1; m <= most_supers; m++) {
+            if (m > 1 && steps < least * n * m) break;
+            const double fill = (double)base * n * m / slots, job = steps / (n * m) + (fill > 1.0 ? more : fixed);
+            double time = job;
+            if (fill > 1.0) time = batch == 1 ? (double)((base * n * m + slots - 1) / slots) * job
+                                              : (0.75 * fill > 1.0 ? 0.75 * fill : 1.0) * job + job / 3;
+            if (m > 1) time += join;
+            if (time < best_time * 0.999) best_time = time, best = Split{n, m};
+            if (fill > 2.0) break;
+        }
     }
     return best;
 }

@@ -30,6 +30,7 @@
 #include <type_traits>
 
 #include "../../include/matvec_b200.h"
+#include "barriers.cuh"
 #include "mvb_runtime.h"
 #include "tree_attention.cuh"
 
@@ -40,58 +41,14 @@ using namespace rows;
 namespace cg = cooperative_groups;
 
 static __device__ int g_tc_error;
+__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity) { return rows::bar_wait(bar, parity, &g_tc_error); }
 constexpr int kTcThreads = 512;
 constexpr int kMmaWarp = 0, kLoadWarp = 1;  // first, since the scheduler prefers the oldest warp
 constexpr int kBN = 64;              // keys a step
 constexpr int kScales = 4;           // steps whose scales are kept
 constexpr float kPUnit = 2.0f;       // log2 of P' / (P * vs / W): P' stays below 2^15 in fp16
 constexpr float kBehind = 12.0f;     // (6: some warp of the eight moved nearly every step, 2,000 clocks each time)
-constexpr unsigned long long kWaitNs = 1000000000ull;
 
-__device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void bar_init(uint64_t *bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void bar_arrive(uint64_t *bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
-}
-__device__ __forceinline__ void bar_expect(uint64_t *bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ unsigned long long clock_ns() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity) {
-    const uint32_t a = smem_addr(bar);
-    unsigned long long t0 = 0;
-    for (uint32_t i = 0;; i++) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done)
-            : "r"(a), "r"(parity)
-            : "memory");
-        if (done) return true;
-        if ((i & 1023) == 1023) {
-            const unsigned long long t = clock_ns();
-            if (!t0) t0 = t;
-            else if (t - t0 > kWaitNs) {
-                note(&g_tc_error, kWaitRanOut);
-                return false;
-            }
-        }
-    }
-}
-__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                     smem_addr(dst)),
-                 "l"(src), "r"(bytes), "r"(smem_addr(bar))
-                 : "memory");
-}
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void commit(uint64_t *bar) {
@@ -277,7 +234,11 @@ struct TcSmem {
     static constexpr int kRow = kScale + kScales * 2 * kBN * 4;   // row factors [MT][128]
     static constexpr int kMl = kRow + MT * 128 * 4;               // (max, sum) of both groups' rows [2][256]
     static constexpr int kAll = kMl + 2 * 256 * 4;                // every part's weights, and their sums [MT * 128]
-    static constexpr int kBar = kAll + (kMaxSplits * (3 - MT) + 1) * MT * 128 * 4;
+    static constexpr int kAllEnd = kAll + (kMaxSplits * (3 - MT) + 1) * MT * 128 * 4;
+    static constexpr int kPmBytes = kMaxSplits * (3 - MT) * MT * 128 * 4;  // every part's maxima, behind the partial O
+    static constexpr bool kPmInside = kEnd - kJoin >= kPmBytes;
+    static constexpr int kPm = kPmInside ? kJoin : kAllEnd;
+    static constexpr int kBar = kAllEnd + (kPmInside ? 0 : kPmBytes);
     static constexpr size_t kBytes = kBar + 512 + 1024;           // + alignment
     static_assert(kBytes <= 227 * 1024, "shared memory of a CTA");
 };
@@ -303,12 +264,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
     float *cta_m = reinterpret_cast<float *>(smem + S::kMl), *cta_l = cta_m + 256;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int b = blockIdx.z, kvh = blockIdx.y / p.qtiles, qt = blockIdx.y - kvh * p.qtiles, split = blockIdx.x;
+    const int b = blockIdx.z, kvh = blockIdx.y / p.qtiles, qt = blockIdx.y - kvh * p.qtiles;
+    const int split = blockIdx.x % p.splits, super = blockIdx.x / p.splits;
     const Sequence s = sequence_at(p, b, &g_tc_error);
     const int nrows = s.n * p.group, R0 = qt * ROWS;
     if (R0 >= nrows) return;  // the whole cluster returns together
     const int nt = (s.len + kBN - 1) / kBN;
-    const int t0 = (int)((long long)nt * split / p.splits), t1 = (int)((long long)nt * (split + 1) / p.splits);
+    const int t0 = (int)((long long)nt * blockIdx.x / gridDim.x), t1 = (int)((long long)nt * (blockIdx.x + 1) / gridDim.x);
     const int mine = t1 - t0;
 
     if (tid == 0) {
@@ -658,7 +620,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
         fence_after();
         // O in units of W / 2^kPUnit, and the sum in the same: they cancel
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        if (!ALT && p.splits == 1) {
+        if (!ALT && p.splits * p.supers == 1) {
             if (R < nrows) {
                 const int tok = s.row0 + R / p.group, head = kvh * p.group + R % p.group;
                 if (p.lse)
@@ -712,68 +674,61 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
     __syncthreads();
     fence_after();
     if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
-    if (!ALT && p.splits == 1) return;
+    if (!ALT && p.splits * p.supers == 1) return;
 
     // join the cluster: weights of every CTA's rows first, then each CTA takes its share of the elements
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
     float *weight = reinterpret_cast<float *>(smem + S::kAll), *total = weight + kMaxSplits * PARTS * ROWS;
+    float *part_m = reinterpret_cast<float *>(smem + S::kPm);
     const int rows_here = min(ROWS, nrows - R0), parts = p.splits * PARTS;  // part n: CTA n / PARTS, group n % PARTS
+#pragma unroll 4
+    for (int i = tid; i < parts * ROWS; i += kTcThreads) {
+        const int n = i / ROWS, at = (n % PARTS) * 128 + i % ROWS;
+        part_m[i] = *cluster.map_shared_rank(&cta_m[at], n / PARTS);
+        weight[i] = *cluster.map_shared_rank(&cta_l[at], n / PARTS);
+    }
+    __syncthreads();
     for (int i = tid; i < rows_here; i += kTcThreads) {
         float m = -INFINITY, sum = 0.0f;
-#pragma unroll 8
-        for (int n = 0; n < parts; n++) m = fmaxf(m, *cluster.map_shared_rank(&cta_m[(n % PARTS) * 128 + i], n / PARTS));
-#pragma unroll 8
+        for (int n = 0; n < parts; n++) m = fmaxf(m, part_m[n * ROWS + i]);
         for (int n = 0; n < parts; n++) {
-            const float l = *cluster.map_shared_rank(&cta_l[(n % PARTS) * 128 + i], n / PARTS);
-            const float x = *cluster.map_shared_rank(&cta_m[(n % PARTS) * 128 + i], n / PARTS);
-            const float w = l == 0.0f ? 0.0f : l * exp2_fast(x - m);
+            const float l = weight[n * ROWS + i], w = l == 0.0f ? 0.0f : l * exp2_fast(part_m[n * ROWS + i] - m);
             weight[n * ROWS + i] = w;
             sum += w;
         }
         total[i] = sum;
-        if (split == 0 && p.lse) {
+        if (split == 0) {
             const int R = R0 + i;
-            p.lse[(size_t)(s.row0 + R / p.group) * p.heads + kvh * p.group + R % p.group] =
-                sum == 0.0f ? -INFINITY : (m + log2f(sum)) * 0.693147180559945309f;
+            const size_t at = (size_t)(s.row0 + R / p.group) * p.heads + kvh * p.group + R % p.group;
+            if (p.supers > 1) work_ml(p)[(size_t)super * p.rows * p.heads + at] = make_float2(m, sum);
+            else if (p.lse) p.lse[at] = sum == 0.0f ? -INFINITY : (m + log2f(sum)) * 0.693147180559945309f;
         }
     }
     __syncthreads();
-    constexpr int kPer = 4;  // elements of a thread in flight
     const int total4 = rows_here * (HDP / 4);
-    for (int i0 = tid + split * kTcThreads; i0 < total4; i0 += kTcThreads * p.splits * kPer) {
-        float4 o[kPer];
-#pragma unroll
-        for (int u = 0; u < kPer; u++) o[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 2
+    for (int i = tid + split * kTcThreads; i < total4; i += kTcThreads * p.splits) {
+        const int row = i / (HDP / 4), d4 = i % (HDP / 4);
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
         for (int n = 0; n < parts; n++) {
-            float4 x[kPer];
-#pragma unroll
-            for (int u = 0; u < kPer; u++) {
-                const int i = min(i0 + u * kTcThreads * p.splits, total4 - 1), row = i / (HDP / 4), d4 = i % (HDP / 4);
-                x[u] = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(
-                    reinterpret_cast<const float *>(smem) + (size_t)((n % PARTS) * 128 + row) * HDP +
-                        ((4 * d4) ^ ((row & 7) << 2)), n / PARTS));
-            }
-#pragma unroll
-            for (int u = 0; u < kPer; u++) {
-                const float f = weight[n * ROWS + min(i0 + u * kTcThreads * p.splits, total4 - 1) / (HDP / 4)];
-                o[u].x = __fmaf_rn(f, x[u].x, o[u].x);
-                o[u].y = __fmaf_rn(f, x[u].y, o[u].y);
-                o[u].z = __fmaf_rn(f, x[u].z, o[u].z);
-                o[u].w = __fmaf_rn(f, x[u].w, o[u].w);
-            }
+            const float4 x = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(
+                reinterpret_cast<const float *>(smem) + (size_t)((n % PARTS) * 128 + row) * HDP + ((4 * d4) ^ ((row & 7) << 2)),
+                n / PARTS));
+            const float f = weight[n * ROWS + row];
+            o.x = __fmaf_rn(f, x.x, o.x);
+            o.y = __fmaf_rn(f, x.y, o.y);
+            o.z = __fmaf_rn(f, x.z, o.z);
+            o.w = __fmaf_rn(f, x.w, o.w);
         }
-#pragma unroll
-        for (int u = 0; u < kPer; u++) {
-            const int i = i0 + u * kTcThreads * p.splits, row = i / (HDP / 4), d4 = i % (HDP / 4);
-            if (i >= total4 || 4 * d4 >= p.head) continue;
-            const float sum = total[row], inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            const int R = R0 + row;
-            store4(static_cast<T *>(p.out) + (size_t)(s.row0 + R / p.group) * p.out_stride +
-                       (size_t)(kvh * p.group + R % p.group) * p.head + 4 * d4,
-                   make_float4(o[u].x * inv, o[u].y * inv, o[u].z * inv, o[u].w * inv));
-        }
+        if (4 * d4 >= p.head) continue;
+        const float sum = total[row], inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int R = R0 + row, tok = s.row0 + R / p.group, head = kvh * p.group + R % p.group;
+        o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        if (p.supers > 1)
+            *reinterpret_cast<float4 *>(p.work + (((size_t)super * p.rows + tok) * p.heads + head) * p.head + 4 * d4) = o;
+        else
+            store4(static_cast<T *>(p.out) + (size_t)tok * p.out_stride + (size_t)head * p.head + 4 * d4, o);
     }
     cluster.sync();  // no CTA leaves while a sister reads its shared memory
 }
@@ -792,9 +747,13 @@ static cudaError_t launch(AttnParams p, int max_len, cudaStream_t stream) {
     p.qtiles = (int)(((long long)p.max_new * p.group + MT * 128 - 1) / (MT * 128));
     if ((long long)p.qtiles * p.kv_heads > 65535) return cudaErrorInvalidConfiguration;
     const long long base = (long long)p.qtiles * p.kv_heads * p.bt.batch;
-    p.splits = choose_splits(base, p.bt.batch, (double)max_len / kBN, 8.0, 4.0, [&](int n) { return slots((const void *)kernel, n, smem); });
+    // a unit: a step, 1.2 us with two row tiles; a CTA starts, fills and joins in about 8 us, a second kernel takes 4
+    const Split cut = choose_splits(base, p.bt.batch, (double)max_len / kBN, 6.0, 8.0, 3.0, 4.0, most_supers(p),
+                                    [&](int n) { return slots((const void *)kernel, n, smem); });
+    p.splits = cut.splits;
+    p.supers = cut.supers;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.splits, p.kv_heads * p.qtiles, p.bt.batch);
+    cfg.gridDim = dim3(p.splits * p.supers, p.kv_heads * p.qtiles, p.bt.batch);
     cfg.blockDim = dim3(kTcThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
@@ -805,7 +764,8 @@ static cudaError_t launch(AttnParams p, int max_len, cudaStream_t stream) {
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, p);
+    e = cudaLaunchKernelEx(&cfg, kernel, p);
+    return e == cudaSuccess && p.supers > 1 ? launch_join(p, rows::Type<T>::kId, stream) : e;
 }
 
 template <typename T, int QP, int PP, int BITS, int HDP>

@@ -18,7 +18,7 @@ are. All of it is read on the device: a call may be captured in a CUDA graph and
 Checks: types, shapes, strides and devices are checked here (ValueError) and in the library (MatvecError). What only the
 device can see (a page number, position or length out of range) is skipped there, never followed, and reported by
 serve_status(). Calls are asynchronous on `stream` (default: the current stream of the tensors' device) and may run on any
-device; they keep no state and use no workspace, so calls on several streams do not meet.
+device; they keep no state, and memory that a call needs is its own, so calls on several streams do not meet.
 """
 import ctypes as C
 import math
@@ -322,9 +322,20 @@ def tree_attention(q, cache, pages, cu, lens, out, tree=None, scale=None, max_ne
         if lse.dtype is not _T.float32 or lse.shape != (n, heads) or not lse.is_contiguous():
             raise ValueError(f"lse: contiguous float32 {(n, heads)} is needed")
         lp = lse.data_ptr()
+    max_new = n if max_new is None else max_new
+    max_len = b[1] * cache.page if max_len is None else max_len
+    work, wp, wn = None, None, 0
+    if b[4] * cache.kv_heads <= 18 and max_len >= 16384:  # few jobs, long contexts: a workspace may help
+        wn = _mvb().lib().mvb_tree_attention_work(n, heads, cache.kv_heads, head, b[4], max_new, max_len)
+        if wn:
+            if stream is None:
+                work = _T.empty(wn, dtype=_T.uint8, device=cache.device)
+            else:  # memory of the stream that uses it
+                with _T.cuda.stream(stream):
+                    work = _T.empty(wn, dtype=_T.uint8, device=cache.device)
+            wp = work.data_ptr()
     _call("mvb_tree_attention", cache.device, stream, q.data_ptr(), qs, *cache.args, *b, n, heads, _TYPES[dtype], tp, words,
-          head ** -0.5 if scale is None else float(scale), n if max_new is None else max_new,
-          b[1] * cache.page if max_len is None else max_len, out.data_ptr(), os_, lp)
+          head ** -0.5 if scale is None else float(scale), max_new, max_len, out.data_ptr(), os_, lp, wp, wn)
     return out
 
 

@@ -33,7 +33,8 @@ def read(L, **kw):
 
 
 def attention(L, **kw):
-    tail = dict(heads=4, dtype=0, tree=P, words=1, scale=0.125, max_new=2, max_len=50, out=P, out_stride=256, lse=P)
+    tail = dict(heads=4, dtype=0, tree=P, words=1, scale=0.125, max_new=2, max_len=50, out=P, out_stride=256, lse=P, work=None,
+                work_bytes=0)
     q = dict(q=P, q_stride=256)
     a = kv_args(**{k: v for k, v in kw.items() if k not in tail and k not in q})
     tail.update({k: v for k, v in kw.items() if k in tail})
@@ -63,7 +64,7 @@ def test_read_refuses(mvb, bad):
 @pytest.mark.parametrize("bad", CACHE_BAD + [dict(heads=3), dict(heads=0), dict(dtype=5), dict(batch=70000), dict(words=0),
                                              dict(max_new=-1), dict(max_len=-1), dict(scale=math.inf),
                                              dict(scale=math.nan), dict(q=P + 4), dict(out=None), dict(lse=P + 2),
-                                             dict(tree=P + 4), dict(q_stride=258), dict(max_new=1 << 30, rows=1 << 30)])
+                                             dict(tree=P + 4), dict(work=P + 8), dict(q_stride=258), dict(max_new=1 << 30, rows=1 << 30)])
 def test_attention_refuses(mvb, bad):
     assert attention(mvb.lib(), **bad) == -1
     assert "mvb_tree_attention" in mvb.last_error()

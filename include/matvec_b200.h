@@ -89,6 +89,13 @@ void *mvb_qwen_stream(void *model);
  * the head_k head logits. Returns the greedy head row (argmax, first of ties), or -1. */
 int mvb_qwen_forward(void *model, int token, int pos, float *logits);
 
+/* Log probabilities over the head's logits of the last step (mvb_qwen_forward, mvb_qwen_decode), computed where they lie
+ * (mvb_logprobs) instead of downloading them: of the n <= 1024 given head rows, the entropy (nats), and the `top` <= 64 most
+ * probable head rows, equal logits by the lowest row. Host arrays; any may be NULL whose count is 0 (entropy always). Head
+ * rows are token ids with a full head or a runq handle. 0, or -1. */
+int mvb_qwen_logprobs(void *model, const int *rows, int n, float *logp, float *entropy, int top, int *top_rows,
+                      float *top_logp);
+
 /* Feeds prompt[0 .. n-2] at positions 0 .. n-2 and leaves prompt[n-1] as the input of position n-1, like
  * qwen.c generate() before its first sampled token. The fed tokens run through the layers in batches of up to 256
  * with the tensor-core matmul (mvb_gemm4) and a batched causal attention, writing the KV-cache rows one decode
@@ -229,7 +236,7 @@ int mvb_kv_read(const void *kq, const float *ks, const void *vq, const float *vs
 
 /* Attention of the batch's new tokens, whose keys and values are in the cache: out = softmax(scale * q k) v over positions
  * below lens[b] and, of the new ones, those that `tree` allows: rows x words 64-bit words, bit j for the sequence's j-th new
- * token (NULL: each sees those before it and itself). heads is a multiple of kv_heads. max_new: at least the most new
+ * token (NULL: each sees those before it and itself). heads is a multiple of kv_heads; out may be q. max_new: at least the most new
  * tokens of a sequence (sequences with more are left out and reported); max_len: about the longest lens[b] + new tokens,
  * which only decides how the work is split. lse (may be NULL): rows x heads, the natural log of the sum of exponentials. A
  * row that sees nothing gives zeros and -inf. fp32 inputs give fp32-accurate results; the same call gives the same bits.

@@ -72,6 +72,8 @@ def lib():
         L.mvb_qwen_stream.argtypes = [vp]
         L.mvb_qwen_forward.restype = i
         L.mvb_qwen_forward.argtypes = [vp, i, i, vp]
+        L.mvb_qwen_logprobs.restype = i
+        L.mvb_qwen_logprobs.argtypes = [vp, ip, i, C.POINTER(C.c_float), C.POINTER(C.c_float), i, ip, C.POINTER(C.c_float)]
         L.mvb_qwen_prefill.restype = i
         L.mvb_qwen_prefill.argtypes = [vp, ip, i]
         L.mvb_qwen_prefill_tokenwise.restype = i
@@ -404,6 +406,18 @@ class QwenDecoder:
         if row < 0:
             raise MatvecError("mvb_qwen_forward failed: " + last_error())
         return row, lg
+
+    def logprobs(self, rows=(), top=0):
+        """(log probabilities of the head rows `rows`, entropy in nats, the `top` most probable head rows, their log
+        probabilities) of the last forward() or decode() step, computed on the device from its logits."""
+        import numpy as np
+        r = self._ids(rows).reshape(-1)
+        logp, ent = np.empty(r.size, np.float32), C.c_float()
+        top_rows, top_logp = np.empty(top, np.int32), np.empty(top, np.float32)
+        ip, fp = C.POINTER(C.c_int), C.POINTER(C.c_float)
+        check(lib().mvb_qwen_logprobs(self.h, r.ctypes.data_as(ip), r.size, logp.ctypes.data_as(fp), C.byref(ent), top,
+                                      top_rows.ctypes.data_as(ip), top_logp.ctypes.data_as(fp)), "mvb_qwen_logprobs")
+        return logp, ent.value, top_rows, top_logp
 
     def prefill(self, prompt):
         p = self._ids(prompt)

@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(256, 3) kv_append_kernel(const KvParams p) {
     // those that quantize: 14,000 rows of 32 + 8 heads took 179 us so)
     const int chunk = blockIdx.y;
     const long long tok = (long long)blockIdx.x * 8 + warp;
-    if (tok >= p.rows || tok >= p.bt.cu[p.bt.batch]) return;  // rows behind the last sequence stay as they are
+    if (tok >= p.rows || tok >= p.bt.cu[p.bt.batch] || tok < p.bt.cu[0]) return;  // rows of no sequence stay as they are
     const bool on = E * l < p.head, in_rot = E * l < p.rot;
     const bool is_q = chunk >= p.kv_chunks;
     int b = 0;
@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvParams p) {
     if (tid < nt) {
         const int tok = t0 + tid;
         long long slot = -1;
-        if (tok < p.bt.cu[p.bt.batch]) {
+        if (tok < p.bt.cu[p.bt.batch] && tok >= p.bt.cu[0]) {
             int lo = 0, hi = p.bt.batch;  // the first sequence that ends behind the row
             while (lo < hi) {
                 const int mid = (lo + hi) >> 1;

@@ -155,6 +155,8 @@ struct Model {
     cudaGraphExec_t stamp_graph = nullptr;
     unsigned long long *stamps = nullptr;
     bool stamping = false;  // set while the stamped copy is captured
+    // mvb_qwen_logprobs' ids and results (allocated on first use)
+    int *lp = nullptr;
     struct Info { const char *kind; int layer; };
     std::vector<Info> info;  // one per kernel of the step, in launch order
     // batched prefill buffers (allocated on first use): up to `cap` tokens per batch
@@ -398,7 +400,7 @@ static void destroy(Model *m) {
     if (m->ring) cudaFreeHost(m->ring);
     void *bufs[] = {m->image, m->x, m->xb, m->qkv, m->hb, m->logits, m->kcache, m->vcache, m->rope, m->xq_n,
                     m->xs_n, m->counters, m->prompt, m->ids, m->st, m->stamps, m->pf.x, m->pf.qkv, m->pf.qb, m->pf.att,
-                    m->pf.out, m->pf.h1, m->pf.h3, m->pf.xs, m->pf.xq};
+                    m->pf.out, m->pf.h1, m->pf.h3, m->pf.xs, m->pf.xq, m->lp};
     for (void *b : bufs)
         if (b) cudaFree(b);
     for (int i = 0; i < 2; i++) {
@@ -1001,6 +1003,44 @@ extern "C" int mvb_qwen_forward(void *model, int token, int pos, float *logits) 
         wait_stream(*m, "mvb_qwen_forward", timeout_s()))
         return -1;
     return s.last_row;
+}
+
+extern "C" int mvb_qwen_logprobs(void *model, const int *rows, int n, float *logp, float *entropy, int top, int *top_rows,
+                                 float *top_logp) {
+    constexpr int kIds = 1024, kTop = 64;
+    Model *m = static_cast<Model *>(model);
+    if (!m) return -1;
+    if (n < 0 || n > kIds || top < 0 || top > kTop || top > m->head_rows || (n && (!rows || !logp)) ||
+        (top && (!top_rows || !top_logp))) {
+        set_error("mvb_qwen_logprobs: need 0 <= n <= %d, 0 <= top <= min(%d, head rows), and arrays for both", kIds, kTop);
+        return -1;
+    }
+    for (int i = 0; i < n; i++)
+        if (rows[i] < 0 || rows[i] >= m->head_rows) {
+            set_error("mvb_qwen_logprobs: head row %d out of range", rows[i]);
+            return -1;
+        }
+    if (!m->lp && cudaMalloc(&m->lp, (2 * kIds + 2 * kTop + 1) * 4) != cudaSuccess) {
+        set_error("mvb_qwen_logprobs: no device memory");
+        return -1;
+    }
+    int *ids = m->lp, *tops = ids + 2 * kIds;
+    float *lps = reinterpret_cast<float *>(ids + kIds), *tlp = reinterpret_cast<float *>(tops + kTop), *ent = tlp + kTop;
+    cudaError_t e = n ? cudaMemcpyAsync(ids, rows, (size_t)n * 4, cudaMemcpyHostToDevice, m->stream) : cudaSuccess;
+    if (e == cudaSuccess && mvb_logprobs(m->logits, m->head_rows, MVB_F32, 1, m->head_rows, ids, n, lps, ent, top, tops, tlp,
+                                         m->stream))
+        return -1;
+    if (e == cudaSuccess && n) e = cudaMemcpyAsync(logp, lps, (size_t)n * 4, cudaMemcpyDeviceToHost, m->stream);
+    if (e == cudaSuccess && entropy) e = cudaMemcpyAsync(entropy, ent, 4, cudaMemcpyDeviceToHost, m->stream);
+    if (e == cudaSuccess && top) {
+        e = cudaMemcpyAsync(top_rows, tops, (size_t)top * 4, cudaMemcpyDeviceToHost, m->stream);
+        if (e == cudaSuccess) e = cudaMemcpyAsync(top_logp, tlp, (size_t)top * 4, cudaMemcpyDeviceToHost, m->stream);
+    }
+    if (e != cudaSuccess) {
+        set_error("mvb_qwen_logprobs: copy failed: %s", cudaGetErrorString(e));
+        return -1;
+    }
+    return wait_stream(*m, "mvb_qwen_logprobs", timeout_s());
 }
 
 static int check_prompt(Model *m, const int *prompt, int n, const char *who) {

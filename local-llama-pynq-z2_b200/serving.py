@@ -298,8 +298,8 @@ def tree_mask(parents):
 
 def tree_attention(q, cache, pages, cu, lens, out, tree=None, scale=None, max_new=None, max_len=None, lse=None, stream=None):
     """Attention of the batch's new tokens over their sequences' cached positions and, of the new ones (appended already,
-    token i at position lens[b] + i), over those their mask allows. q, out (rows, heads, head), heads a multiple of the
-    cache's kv_heads. tree (rows, words) int64: bit j of a row allows its sequence's j-th new token; None: each sees those
+    token i at position lens[b] + i), over those their mask allows. q, out (rows, heads, head; out may be q), heads a multiple
+    of the cache's kv_heads. tree (rows, words) int64: bit j of a row allows its sequence's j-th new token; None: each sees those
     before it and itself, so that one new token a sequence is a decode step and many are a prompt. scale: default
     1 / sqrt(head). max_new: at least the most new tokens of a sequence (default: all rows); sequences with more are
     skipped and reported. max_len: about the longest lens[b] + new tokens (default: the page table's reach), which only

@@ -8,22 +8,26 @@
 // operand in tensor memory, written over the S it came from. Tensor memory: two 64-column slots of S for each row tile
 // (so that the next step's scores stand ready when a softmax ends), then O0 | O1, 128 columns each.
 //
-// Warp roles (512 threads):
+// Warp roles (768 threads):
 //   warp 0          one thread issues the MMAs: PV0 PV1 QK0'' QK1'' a step. (The oldest warp, which the scheduler prefers:
 //                   as warp 12 it waited for issue slots behind the softmax.)
 //   warp 1          bulk copies of the raw pages, kRaw stages ahead.
-//   warps 4-5, 6-7  converters of K, of V: a thread owns a key. Bytes -> fp16; the keys' or the values' scales.
-//   warps 8-11, 12-15  softmax of row tile 0, 1: a thread owns a row. S from tensor memory, keys' scales, maximum,
-//                   exponentials, values' scales, P in fp16 back to tensor memory. The running maximum and the values' unit
-//                   W move only when a row falls 2^12 behind (then O is scaled in tensor memory, after the product before
-//                   has ended). The unit's factor is folded into the exponent, so it multiplies P and the row's sum alike.
+//   warps 2, 4, 6 and 3, 5, 7  converters of K, of V, a step's tile a warp: bytes -> fp16; the scales.
+//   warps 8-15, 16-23  softmax of row tile 0, 1: two threads a row, 32 of the step's keys each, so that every scheduler has
+//                   four such warps to hide one another's latencies (with one thread a row, 64 keys each, a step took 2,350
+//                   clocks). S from tensor memory, keys' scales, maximum, exponentials, values' scales, P in fp16 back to
+//                   tensor memory. The running maximum and the values' unit W move only when a row falls 2^12 behind (then O
+//                   is scaled in tensor memory, after the product before has ended): a row's two threads vote on that with
+//                   the barrier that also keeps either's P off the other's unread S, and exchange their maxima only then.
+//                   The unit's factor is folded into the exponent, so it multiplies P and the row's sum alike.
 // What bounds it: for two row tiles of head 128 and 64 keys the exponentials take 1,024 clocks (16 a clock), the MMAs
 // 1,280 (QK at N = 64 waits for shared memory: 48 clocks a product against 32), shared memory 1,150.
 // Up to 128 query rows (MT = 1): both softmax groups take the same rows, for every other step each, with an O and
 // (max, sum) of their own; the two parts are joined like those of the cluster.
 // The keys of a sequence are split over the CTAs of a cluster, joined in distributed shared memory in a fixed order.
 // Every mbarrier wait is bounded (1 s): a wait that runs out notes the error and the roles stop.
-// Every barrier is waited on before its next phase can end: each role's next arrival needs what the waiter does after.
+// Every barrier is waited on before its next phase can end (each role's next arrival needs what the waiter does after),
+// and by a warp that has seen the phase before.
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -42,10 +46,13 @@ namespace cg = cooperative_groups;
 
 static __device__ int g_tc_error;
 __device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity) { return rows::bar_wait(bar, parity, &g_tc_error); }
-constexpr int kTcThreads = 512;
+constexpr int kTcThreads = 768;
 constexpr int kMmaWarp = 0, kLoadWarp = 1;  // first, since the scheduler prefers the oldest warp
 constexpr int kBN = 64;              // keys a step
-constexpr int kScales = 4;           // steps whose scales are kept
+// A parity says which of two phases a barrier is in, so a waiter must have seen the phase before: the barriers that several
+// warps of a kind wait on in turn are as many as make the same warp wait on each (multiples of 3).
+constexpr int kFree = 6;             // barriers of tiles set free
+constexpr int kScales = 8;           // steps whose scales are kept
 constexpr float kPUnit = 2.0f;       // log2 of P' / (P * vs / W): P' stays below 2^15 in fp16
 constexpr float kBehind = 12.0f;     // (6: some warp of the eight moved nearly every step, 2,000 clocks each time)
 
@@ -225,14 +232,15 @@ struct TcSmem {
     // only after its values; with 3 the copies came too late for MT = 1: 2,300 clocks a step)
     static constexpr int kRest = 32 * 1024;  // what follows the stages, at most
     static constexpr int kFit = (227 * 1024 - kRest - kRawAt) / kRawStage;
-    static constexpr int kRaw = kFit > 6 ? 6 : kFit;
-    static_assert(kRaw >= 3, "raw stages");
+    static constexpr int kRaw = kFit >= 6 ? 6 : 3;  // a multiple of the three converters of a kind, see kFree
+    static_assert(kFit >= 3, "raw stages");
     // the partial O of both softmax groups, [256][HDP] fp32, lies over the tiles
     static constexpr int kJoin = 256 * HDP * 4;
     static constexpr int kEnd = kRawAt + kRaw * kRawStage;
     static constexpr int kScale = kEnd > kJoin ? kEnd : kJoin;    // [kScales][kk | vv] fp32
     static constexpr int kRow = kScale + kScales * 2 * kBN * 4;   // row factors [MT][128]
-    static constexpr int kMl = kRow + MT * 128 * 4;               // (max, sum) of both groups' rows [2][256]
+    static constexpr int kXm = kRow + MT * 128 * 4;               // what a row's two threads exchange [2][2][128]
+    static constexpr int kMl = kXm + 4 * 128 * 4;               // (max, sum) of both groups' rows [2][256]
     static constexpr int kAll = kMl + 2 * 256 * 4;                // every part's weights, and their sums [MT * 128]
     static constexpr int kAllEnd = kAll + (kMaxSplits * (3 - MT) + 1) * MT * 128 * 4;
     static constexpr int kPmBytes = kMaxSplits * (3 - MT) * MT * 128 * 4;  // every part's maxima, behind the partial O
@@ -253,13 +261,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
     extern __shared__ __align__(1024) uint8_t raw_smem[];
     uint8_t *smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);
     uint64_t *bar = reinterpret_cast<uint64_t *>(smem + S::kBar);
-    // (slot = step & 1 where there are two, step % kRaw of raw, step % kScales of scales)
+    // (slot = step & 1 where there are two, step % kRaw of raw, % kScales of scales, % kFree of tiles set free)
     uint64_t *raw_full = bar, *raw_empty = raw_full + kRaw, *k_ready = raw_empty + kRaw, *k_free = k_ready + 2,
-             *v_ready = k_free + 2, *v_free = v_ready + 2, *s_full = v_free + 2 /* [m][slot] */,
+             *v_ready = k_free + kFree, *v_free = v_ready + 2, *s_full = v_free + kFree /* [m][slot] */,
              *p_ready = s_full + 4 /* [m][slot] */, *pv_done = p_ready + 4 /* [m] */, *sc_ready = pv_done + 2,
              *q_ready = sc_ready + kScales, *o_done = q_ready + 1;
     uint32_t *tmem_at = reinterpret_cast<uint32_t *>(o_done + 1);
-    float *vmax = reinterpret_cast<float *>(bar + 48);  // [kScales][2]
+    float *vmax = reinterpret_cast<float *>(bar + 50);  // [kScales]
     float *row_factor = reinterpret_cast<float *>(smem + S::kRow);
     float *cta_m = reinterpret_cast<float *>(smem + S::kMl), *cta_l = cta_m + 256;
 
@@ -276,21 +284,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
     if (tid == 0) {
         for (int i = 0; i < kRaw; i++) {
             bar_init(&raw_full[i], 1);
-            bar_init(&raw_empty[i], 4);
+            bar_init(&raw_empty[i], 2);
         }
         for (int i = 0; i < 2; i++) {
-            bar_init(&k_ready[i], 2);
-            bar_init(&v_ready[i], 2);
-            bar_init(&k_free[i], 1);
-            bar_init(&v_free[i], 1);
+            bar_init(&k_ready[i], 1);
+            bar_init(&v_ready[i], 1);
             bar_init(&pv_done[i], 1);
         }
         for (int i = 0; i < 4; i++) {
             bar_init(&s_full[i], 1);
-            bar_init(&p_ready[i], 4);
+            bar_init(&p_ready[i], 8);
         }
-        for (int i = 0; i < kScales; i++) bar_init(&sc_ready[i], 2);
-        bar_init(q_ready, 8);
+        for (int i = 0; i < kScales; i++) bar_init(&sc_ready[i], 1);
+        for (int i = 0; i < kFree; i++) {
+            bar_init(&k_free[i], 1);
+            bar_init(&v_free[i], 1);
+        }
+        bar_init(q_ready, 16);
         bar_init(o_done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -306,62 +316,72 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
     const int row_bytes = p.head * BITS / 8;
 
     if (warp < 8) {
-        if (warp >= 4) {
-            // ---------------- converters: one key a thread, warps 4-5 its keys' row, warps 6-7 its values' ----------------
-            const int key = tid & 63, kv = (warp - 4) >> 1, pieces = p.head / 16;
+        if (warp >= 2) {
+            // ---------------- converters: a tile a warp, two keys a lane ----------------
+            // warps 2, 4, 6 take the keys of every third step, 3, 5, 7 the values (two warps a tile, every tile: waits and
+            // fences of each step took as long as its conversion, 2,300 clocks together)
+            const int kv = warp & 1, pieces = p.head / 16;
             uint64_t *ready = kv ? v_ready : k_ready, *free_ = kv ? v_free : k_free;
-            uint8_t *tiles = smem + (kv ? S::kV : S::kK) + key * 128;
-            if (pieces < HDP / 16)  // the columns behind the head are never converted: zeros, so that they add nothing
-                for (int i = 0; i < 2 * S::kBlocks * 8; i++)
-                    *reinterpret_cast<uint4 *>(tiles + (i >> 3) * (kBN * 128) + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
-            for (int j = 0; j < mine; j++) {
+            uint8_t *tiles = smem + (kv ? S::kV : S::kK);
+            if (pieces < HDP / 16 && warp < 6)  // the columns behind the head are never converted: zeros add nothing
+                for (int i = lane; i < S::kTile / 16; i += 32)
+                    reinterpret_cast<uint4 *>(tiles + ((warp - 2) >> 1) * S::kTile)[i] = make_uint4(0, 0, 0, 0);
+            asm volatile("bar.sync 1, 192;" ::: "memory");
+            for (int j = (warp - 2) >> 1; j < mine; j += 3) {
                 const int slot = j & 1, rs = j % kRaw, ss = j % kScales;
                 const uint8_t *raw = smem + S::kRawAt + rs * S::kRawStage;
                 if (!bar_wait(&raw_full[rs], (j / kRaw) & 1)) break;
                 if (kv) {
-                    // the scales, before the tile is free: the softmax of kScales steps ago, their last reader, is done
-                    // (the step before waited for the product with its P, or a later one)
-                    const bool live = (t0 + j) * kBN + key < s.len;
+                    // the scales, before the tile is free: the softmax of kScales steps ago, their last reader, is done (this
+                    // warp's step before last waited for the product of five steps ago)
                     float *sc = reinterpret_cast<float *>(smem + S::kScale) + ss * 2 * kBN;
                     const float *rsc = reinterpret_cast<const float *>(raw + 2 * S::kRawTile);
-                    const float x = live ? rsc[kBN + key] : 0.0f;
-                    sc[key] = live ? rsc[key] * p.scale_log2 : 0.0f;
-                    sc[kBN + key] = x;
-                    float mv = fabsf(x) < INFINITY ? fabsf(x) : 0.0f;  // an infinite scale must not set the unit
+                    float mv = 0.0f;
+#pragma unroll
+                    for (int key = lane; key < kBN; key += 32) {
+                        const bool live = (t0 + j) * kBN + key < s.len;
+                        const float x = live ? rsc[kBN + key] : 0.0f;
+                        sc[key] = live ? rsc[key] * p.scale_log2 : 0.0f;
+                        sc[kBN + key] = x;
+                        if (fabsf(x) < INFINITY) mv = fmaxf(mv, fabsf(x));  // an infinite scale must not set the unit
+                    }
 #pragma unroll
                     for (int o = 16; o; o >>= 1) mv = fmaxf(mv, __shfl_xor_sync(0xffffffffu, mv, o));
-                    if (lane == 0) vmax[ss * 2 + (warp & 1)] = mv;
+                    if (lane == 0) vmax[ss] = mv;
                     __syncwarp();
                     if (lane == 0) bar_arrive(&sc_ready[ss]);
                 }
                 // the tile's last product has ended
-                if (j >= 2 && !bar_wait(&free_[slot], ((j >> 1) - 1) & 1)) break;
-                const uint8_t *src = raw + kv * S::kRawTile + key * row_bytes;
-                uint8_t *dst = tiles + slot * S::kTile;
-                // the lanes of a quarter warp start at different pieces: different banks
-                if (pieces == HDP / 16) {
-                    constexpr int PIECES = HDP / 16;
-                    const int first = key & (PIECES - 1);
-                    uint4 raw16[PIECES];  // all loads first (16 integers each: 16 bytes, or 8 in the low half)
+                if (j >= 2 && !bar_wait(&free_[(j - 2) % kFree], ((j - 2) / kFree) & 1)) break;
+#pragma unroll 1
+                for (int key = lane; key < kBN; key += 32) {
+                    const uint8_t *src = raw + kv * S::kRawTile + key * row_bytes;
+                    uint8_t *dst = tiles + slot * S::kTile + key * 128;
+                    // the lanes of a quarter warp start at different pieces: different banks
+                    if (pieces == HDP / 16) {
+                        constexpr int PIECES = HDP / 16;
+                        const int first = key & (PIECES - 1);
+                        uint4 raw16[PIECES];  // all loads first (16 integers each: 16 bytes, or 8 in the low half)
 #pragma unroll
-                    for (int i = 0; i < PIECES; i++) raw16[i] = load_sixteen<BITS>(src + (i ^ first) * 2 * BITS);
+                        for (int i = 0; i < PIECES; i++) raw16[i] = load_sixteen<BITS>(src + (i ^ first) * 2 * BITS);
 #pragma unroll
-                    for (int i = 0; i < PIECES; i++) {
-                        uint4 x, y;
-                        sixteen<BITS>(raw16[i], x, y);
-                        const int c = i ^ first, at = (c >> 2) * (kBN * 128) + ((((2 * c) & 7) ^ (key & 7)) << 4);
-                        *reinterpret_cast<uint4 *>(dst + at) = x;
-                        *reinterpret_cast<uint4 *>(dst + (at ^ 16)) = y;
-                    }
-                } else {
-                    int c = key % pieces;
-                    for (int i = 0; i < pieces; i++) {
-                        uint4 x, y;
-                        sixteen<BITS>(load_sixteen<BITS>(src + c * 2 * BITS), x, y);
-                        const int at = (c >> 2) * (kBN * 128) + ((((2 * c) & 7) ^ (key & 7)) << 4);
-                        *reinterpret_cast<uint4 *>(dst + at) = x;
-                        *reinterpret_cast<uint4 *>(dst + (at ^ 16)) = y;
-                        c = c + 1 == pieces ? 0 : c + 1;
+                        for (int i = 0; i < PIECES; i++) {
+                            uint4 x, y;
+                            sixteen<BITS>(raw16[i], x, y);
+                            const int c = i ^ first, at = (c >> 2) * (kBN * 128) + ((((2 * c) & 7) ^ (key & 7)) << 4);
+                            *reinterpret_cast<uint4 *>(dst + at) = x;
+                            *reinterpret_cast<uint4 *>(dst + (at ^ 16)) = y;
+                        }
+                    } else {
+                        int c = key % pieces;
+                        for (int i = 0; i < pieces; i++) {
+                            uint4 x, y;
+                            sixteen<BITS>(load_sixteen<BITS>(src + c * 2 * BITS), x, y);
+                            const int at = (c >> 2) * (kBN * 128) + ((((2 * c) & 7) ^ (key & 7)) << 4);
+                            *reinterpret_cast<uint4 *>(dst + at) = x;
+                            *reinterpret_cast<uint4 *>(dst + (at ^ 16)) = y;
+                            c = c + 1 == pieces ? 0 : c + 1;
+                        }
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -395,7 +415,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
                                    k0 + ((slot * S::kTile + (k >> 2) * (kBN * 128) + (k & 3) * 32) >> 4), qk,
                                    part > 0 || k > 0);
                     commit(&s_full[2 * m + (i & 1)]);
-                    if (ALT || m == 1) commit(&k_free[slot]);
+                    if (ALT || m == 1) commit(&k_free[j % kFree]);
                     return true;
                 };
 #pragma unroll 1
@@ -416,10 +436,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
                                 mma_ts(t + 256 + m * 128, t + m * 128 + (i & 1) * 64 + part * 32 + k * 8,
                                        v0 + ((slot * S::kTile + k * 2048) >> 4), pv, i > 0 || part > 0 || k > 0);
                         commit(&pv_done[m]);
-                        if (ALT || m == 1) commit(&v_free[slot]);
-                        if (ALT) ok = scores(m, i + 2);
+                        if (ALT || m == 1) commit(&v_free[j % kFree]);
+                        ok = scores(m, i + 2);
                     }
-                    if (!ALT && ok) ok = scores(0, i + 2) && scores(1, i + 2);
                 }
                 commit(o_done);
             }
@@ -451,23 +470,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
             for (int j = mine > kRaw ? mine - kRaw : 0; j < mine; j++) bar_wait(&raw_full[j % kRaw], (j / kRaw) & 1);
         }
     } else {
-        // ---------------- softmax: one row a thread ----------------
+        // ---------------- softmax: two threads a row ----------------
         // q: a warp takes a row, scales it by a power of two and stores its fp16 parts, swizzled
-        constexpr int DEEP = 8;  // rows of a warp in flight
-        for (int i0 = warp - 8; i0 < ROWS; i0 += 8 * DEEP) {
+        constexpr int DEEP = 4;  // rows of a warp in flight
+        for (int i0 = warp - 8; i0 < ROWS; i0 += 16 * DEEP) {
             float4 v[DEEP];
 #pragma unroll
             for (int u = 0; u < DEEP; u++) {  // (no branch around the loads: all of them are in flight at once)
-                const int R = min(R0 + i0 + 8 * u, nrows - 1), tok = R / p.group;
+                const int R = min(R0 + i0 + 16 * u, nrows - 1), tok = R / p.group;
                 v[u] = load4(static_cast<const T *>(p.q) + (size_t)(s.row0 + tok) * p.q_stride +
                              (size_t)(kvh * p.group + R - tok * p.group) * p.head + min(4 * lane, p.head - 4));
             }
 #pragma unroll
             for (int u = 0; u < DEEP; u++)
-                if (R0 + i0 + 8 * u >= nrows || 4 * lane >= p.head) v[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (R0 + i0 + 16 * u >= nrows || 4 * lane >= p.head) v[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int u = 0; u < DEEP; u++) {
-                const int i = i0 + 8 * u;
+                const int i = i0 + 16 * u;
                 int e = max(max(exponent_of(v[u].x), exponent_of(v[u].y)), max(exponent_of(v[u].z), exponent_of(v[u].w)));
 #pragma unroll
                 for (int o = 16; o; o >>= 1) e = max(e, __shfl_xor_sync(0xffffffffu, e, o));
@@ -492,8 +511,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) bar_arrive(q_ready);
-        asm volatile("bar.sync 1, 256;" ::: "memory");  // the row factors, among the softmax warps
-        const int m = (warp - 8) >> 2, row = tid & 127;
+        asm volatile("bar.sync 10, 512;" ::: "memory");  // the row factors, among the softmax warps
+        const int m = (warp - 8) >> 3, half = ((warp - 8) >> 2) & 1, row = tid & 127;
+        const int pair = 2 + m * 4 + (warp & 3);  // the named barrier of a row's two warps
+        float *mine_x = reinterpret_cast<float *>(smem + S::kXm) + (m * 2 + half) * 128 + row;
+        const float *other_x = reinterpret_cast<const float *>(smem + S::kXm) + (m * 2 + 1 - half) * 128 + row;
         const uint32_t lane_at = tmem + ((uint32_t)(row & 96) << 16), o_at = lane_at + 256 + m * 128;
         const int R = R0 + (ALT ? 0 : m * 128) + row, draft = R / p.group;
         const float rf = row_factor[ALT ? row : m * 128 + row];
@@ -504,39 +526,47 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
             constexpr bool TAIL = decltype(is_tail)::value;
             const int j = ALT ? 2 * i + m : i, slot = i & 1, par = (i >> 1) & 1, ss = j % kScales, key0 = (t0 + j) * kBN;
             const uint32_t s_at = lane_at + m * 128 + slot * 64;
-            if (!bar_wait(&s_full[2 * m + slot], par) || !bar_wait(&sc_ready[ss], (j / kScales) & 1)) return false;
+            const bool fine = bar_wait(&s_full[2 * m + slot], par) && bar_wait(&sc_ready[ss], (j / kScales) & 1);
             fence_after();
-            const float *kk = reinterpret_cast<const float *>(smem + S::kScale) + ss * 2 * kBN, *vv = kk + kBN;
-            float u[kBN];
-#pragma unroll
-            for (int c = 0; c < kBN / 32; c++) tmem_load32(s_at + 32 * c, u + 32 * c);
-            const float2 v2 = *reinterpret_cast<const float2 *>(vmax + ss * 2);
-            const float vm = fmaxf(v2.x, v2.y);
-            uint32_t bits[kBN / 32] = {};
-            if (TAIL) {
-#pragma unroll
-                for (int c = 0; c < kBN / 32; c++) bits[c] = mask32(p, s, draft, key0 + 32 * c - s.ctx);
-            }
+            const float *kk = reinterpret_cast<const float *>(smem + S::kScale) + ss * 2 * kBN + 32 * half, *vv = kk + kBN;
+            float u[32];
+            tmem_load32(s_at + 32 * half, u);
+            const float vm = vmax[ss];
+            const uint32_t bits = TAIL ? mask32(p, s, draft, key0 + 32 * half - s.ctx) : ~0u;
             wait_load();
             float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int i = 0; i < kBN; i += 4) {
+            for (int i = 0; i < 32; i += 4) {
                 const float4 k4 = *reinterpret_cast<const float4 *>(kk + i);
                 split2(mul2(pair2(u[i], u[i + 1]), pair2(k4.x, k4.y)), u[i], u[i + 1]);
                 split2(mul2(pair2(u[i + 2], u[i + 3]), pair2(k4.z, k4.w)), u[i + 2], u[i + 3]);
                 if (TAIL) {
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        if (!((bits[(i + e) >> 5] >> ((i + e) & 31)) & 1)) u[i + e] = -INFINITY;
+                        if (!((bits >> (i + e)) & 1)) u[i + e] = -INFINITY;
                 }
                 top[0] = max3(top[0], u[i], u[i + 1]);
                 top[1] = max3(top[1], u[i + 2], u[i + 3]);
             }
-            const float now = fmaxf(mx, fmaxf(top[0], top[1]) * rf);
+            float now = fmaxf(mx, fmaxf(top[0], top[1]) * rf);
             const float lv = (float)(min(max(exponent_of(vm), 1) - 127 + 1, 127));  // W above this step's scales
             const bool grow = vm > 0.0f && lv > lw;
-            const bool behind = now > mx + kBehind;
-            if (__any_sync(0xffffffffu, grow || behind)) {
+            uint32_t vote;  // of both warps; after it both have read their S
+            asm volatile(
+                "{\n\t.reg .pred a, b;\n\tsetp.ne.u32 a, %1, 0;\n\t"
+                "barrier.cta.red.or.pred b, %2, 64, a;\n\tselp.u32 %0, 1, 0, b;\n\t}"
+                : "=r"(vote)
+                : "r"((uint32_t)(grow || now > mx + kBehind || !fine)), "r"(pair)
+                : "memory");
+            if (vote) {
+                // a wait that ran out on either side ends both (NaN stands for it)
+                *mine_x = fine ? now : __int_as_float(0x7FC00000);
+                asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
+                const float theirs = *other_x;
+                asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
+                if (__any_sync(0xffffffffu, !fine || theirs != theirs)) return false;
+                now = fmaxf(now, theirs);
+                const bool behind = now > mx + kBehind;
                 const float lw2 = grow ? lv : lw;
                 // O and the sum: exp2(old max - new max), and the old unit in the new one. Only the rows that are behind
                 // move, so that a row's result does not depend on its neighbours.
@@ -546,16 +576,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
                 lw = lw2;
                 l *= f;
                 if (i > 0) {
-                    // (the product of two steps ago has ended: this step's scores were issued after it)
-                    if (!bar_wait(&pv_done[m], (i - 1) & 1)) return false;
+                    // (the product of two steps ago has ended: this step's scores were issued after it; where this wait
+                    // runs out, the results are void and the error is noted)
+                    bar_wait(&pv_done[m], (i - 1) & 1);
                     fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < HDP / 16; c++) {
+                    for (int c = half * (HDP / 32); c < (half + 1) * (HDP / 32); c++) {
                         float o[16];
                         tmem_load16(o_at + 16 * c, o);
                         wait_load();
 #pragma unroll
-                        for (int i = 0; i < 16; i++) o[i] *= f;
+                        for (int e = 0; e < 16; e++) o[e] *= f;
                         tmem_store16(o_at + 16 * c, reinterpret_cast<const uint32_t *>(o));
                     }
                 }
@@ -563,41 +594,34 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
             const float base = (kPUnit - lw) - (mx == -INFINITY ? 0.0f : mx);
             const uint64_t rf2 = pair2(rf, rf), base2 = pair2(base, base);
             uint64_t sum[2] = {0, 0};
-            uint32_t low[PP == 2 ? kBN / 2 : 1];
+            uint32_t hi[16], low[PP == 2 ? 16 : 1];
 #pragma unroll
-            for (int c = 0; c < kBN / 32; c++) {
-                uint32_t hi[16];
+            for (int i = 0; i < 32; i += 4) {
+                const float4 w4 = *reinterpret_cast<const float4 *>(vv + i);
+                const uint64_t w2[2] = {pair2(w4.x, w4.y), pair2(w4.z, w4.w)};
 #pragma unroll
-                for (int i = 0; i < 32; i += 4) {
-                    const float4 w4 = *reinterpret_cast<const float4 *>(vv + 32 * c + i);
-                    const uint64_t w2[2] = {pair2(w4.x, w4.y), pair2(w4.z, w4.w)};
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const int at = 32 * c + i + 2 * h;
-                        float a, d;
-                        split2(fma2(pair2(u[at], u[at + 1]), rf2, base2), a, d);
-                        const uint64_t e2 = pair2(exp2_fast(a), exp2_fast(d));
-                        sum[h] = add2(sum[h], e2);
-                        float x, y;
-                        split2(mul2(e2, w2[h]), x, y);
-                        if (TAIL) {  // a masked key's scale may be anything: its weight is zero, not zero times that
-                            if (u[at] == -INFINITY) x = 0.0f;
-                            if (u[at + 1] == -INFINITY) y = 0.0f;
-                        }
-                        const uint32_t q = pack2<__half>(x, y);
-                        hi[(i + 2 * h) / 2] = q;
-                        if (PP == 2) {
-                            const float2 r = __half22float2(*reinterpret_cast<const __half2 *>(&q));
-                            low[PP == 2 ? at / 2 : 0] = pack2<__half>(x - r.x, y - r.y);
-                        }
+                for (int h = 0; h < 2; h++) {
+                    const int at = i + 2 * h;
+                    float a, d;
+                    split2(fma2(pair2(u[at], u[at + 1]), rf2, base2), a, d);
+                    const uint64_t e2 = pair2(exp2_fast(a), exp2_fast(d));
+                    sum[h] = add2(sum[h], e2);
+                    float x, y;
+                    split2(mul2(e2, w2[h]), x, y);
+                    if (TAIL) {  // a masked key's scale may be anything: its weight is zero, not zero times that
+                        if (u[at] == -INFINITY) x = 0.0f;
+                        if (u[at + 1] == -INFINITY) y = 0.0f;
+                    }
+                    const uint32_t q = pack2<__half>(x, y);
+                    hi[at / 2] = q;
+                    if (PP == 2) {
+                        const float2 r = __half22float2(*reinterpret_cast<const __half2 *>(&q));
+                        low[PP == 2 ? at / 2 : 0] = pack2<__half>(x - r.x, y - r.y);
                     }
                 }
-                tmem_store16(s_at + 16 * c, hi);
             }
-            if (PP == 2) {
-#pragma unroll
-                for (int c = 0; c < kBN / 32; c++) tmem_store16(s_at + 32 + 16 * c, low + (PP == 2 ? 16 * c : 0));
-            }
+            tmem_store16(s_at + 16 * half, hi);
+            if (PP == 2) tmem_store16(s_at + 32 + 16 * half, low);
             float a, d, a2, d2;
             split2(sum[0], a, d);
             split2(sum[1], a2, d2);
@@ -618,55 +642,53 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
         for (int i = plain; i < steps && ok; i++) ok = step(i, std::true_type{});
         if (mine > 0) bar_wait(o_done, 0);
         fence_after();
+        // the row's sum of both threads
+        *mine_x = l;
+        asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
+        l = half ? *other_x + l : l + *other_x;
         // O in units of W / 2^kPUnit, and the sum in the same: they cancel
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const int c0 = half * (HDP / 32);  // this thread's half of O, 16 columns at a time
         if (!ALT && p.splits * p.supers == 1) {
-            if (R < nrows) {
-                const int tok = s.row0 + R / p.group, head = kvh * p.group + R % p.group;
-                if (p.lse)
-                    p.lse[(size_t)tok * p.heads + head] =
-                        l == 0.0f ? -INFINITY : (mx - (kPUnit - lw) + log2f(l)) * 0.693147180559945309f;
-            }
-#pragma unroll
-            for (int c = 0; c < HDP / 32; c++) {
-                float o[32];
-                if (steps > 0) {
-                    tmem_load32(o_at + 32 * c, o);
+            const int tok = s.row0 + R / p.group, head = kvh * p.group + R % p.group;
+            if (R < nrows && p.lse && half == 0)
+                p.lse[(size_t)tok * p.heads + head] =
+                    l == 0.0f ? -INFINITY : (mx - (kPUnit - lw) + log2f(l)) * 0.693147180559945309f;
+#pragma unroll 1
+            for (int c = c0; c < c0 + HDP / 32; c++) {
+                float o[16];
+                if (mine > 0) {
+                    tmem_load16(o_at + 16 * c, o);
                     wait_load();
                 }
-                if (R < nrows) {
-                    T *d = static_cast<T *>(p.out) + (size_t)(s.row0 + R / p.group) * p.out_stride +
-                           (size_t)(kvh * p.group + R % p.group) * p.head;
+                if (R >= nrows) continue;
+                T *d = static_cast<T *>(p.out) + (size_t)tok * p.out_stride + (size_t)head * p.head + 16 * c;
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4)
-                        if (32 * c + i < p.head)
-                            store4(d + 32 * c + i, l == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
-                                                             : make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv,
-                                                                           o[i + 3] * inv));
-                }
+                for (int i = 0; i < 16; i += 4)
+                    if (16 * c + i < p.head)
+                        store4(d + i, l == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                                                : make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv));
             }
         } else {
             // this group's part: O divided by its own sum, the row's (max, sum) beside it
-            cta_m[m * 128 + row] = mx;
-            cta_l[m * 128 + row] = l == 0.0f ? 0.0f : l * exp2f(lw - kPUnit);  // the sum in its own units
+            if (half == 0) {
+                cta_m[m * 128 + row] = mx;
+                cta_l[m * 128 + row] = l == 0.0f ? 0.0f : l * exp2f(lw - kPUnit);  // the sum in its own units
+            }
             float *po = reinterpret_cast<float *>(smem) + (size_t)(m * 128 + row) * HDP;
-            const float unit = l == 0.0f ? 0.0f : inv;
-#pragma unroll
-            for (int c = 0; c < HDP / 32; c++) {
-                float o[32];
+#pragma unroll 1
+            for (int c = c0; c < c0 + HDP / 32; c++) {
+                float o[16];
                 if (steps > 0) {
-                    tmem_load32(o_at + 32 * c, o);
+                    tmem_load16(o_at + 16 * c, o);
                     wait_load();
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; i++) o[i] = 0.0f;
                 }
                 // the 16-byte pieces of a row start at different places: different banks
 #pragma unroll
-                for (int i = 0; i < 32; i += 4)
-                    *reinterpret_cast<float4 *>(po + ((32 * c + i) ^ ((row & 7) << 2))) =
-                        l == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
-                                  : make_float4(o[i] * unit, o[i + 1] * unit, o[i + 2] * unit, o[i + 3] * unit);
+                for (int i = 0; i < 16; i += 4)
+                    *reinterpret_cast<float4 *>(po + ((16 * c + i) ^ ((row & 7) << 2))) =
+                        steps <= 0 || l == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                                                : make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
             }
         }
     }

@@ -152,8 +152,8 @@ def test_out_over_q(torch, mvb, new, ctx):
     """out may be q: every row is read before one is written, however the work is split."""
     c = Case(torch, mvb, [ctx, 7], [new, 2], 2, 64, 8, 32)
     q = torch.randn(c.rows, 6, 64, device="cuda")
-    want = mvb.tree_attention(q, c.cache, *c.batch(), torch.empty_like(q), max_new=new)
-    mvb.tree_attention(q, c.cache, *c.batch(), q, max_new=new)
+    want = mvb.tree_attention(q, c.cache, *c.batch(), torch.empty_like(q), max_new=max(new, 2))
+    mvb.tree_attention(q, c.cache, *c.batch(), q, max_new=max(new, 2))
     assert torch.equal(q, want)
 
 

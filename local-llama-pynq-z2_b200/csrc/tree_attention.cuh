@@ -110,7 +110,7 @@ int cluster_slots(const void *kernel, int n, int threads, size_t smem);
 // Over how many CTAs of a cluster (splits) and how many clusters (supers, at most most_supers) a sequence's keys are split,
 // so that the estimated time is least: `base` jobs without a split, `steps` units of work each for the longest sequence,
 // `fixed` units to start, fill and join a CTA (`more` where the CTAs exceed one wave) and `join` for a second kernel, at
-// least `least` units a CTA. One
+// least `least` units a CTA and, where slots allow, `fewest` CTAs. One
 // sequence: its jobs are alike and run in whole waves. Several: three quarters of the longest on average, in no order, and
 // the last jobs end a third of a job apart.
 struct Split {
@@ -118,23 +118,23 @@ struct Split {
 };
 template <typename F>
 inline Split choose_splits(long long base, int batch, double steps, double fixed, double more, double join, double least,
-                           int most_supers,
-                           const F &slots_of) {
+                           int fewest, int most_supers, const F &slots_of) {
     Split best = {1, 1};
     double best_time = 1e300;
     for (int n = 1; n <= kMaxSplits; n++) {
-        if (n > 1 && steps < least * n) break;
+        if (n > fewest && steps < least * n) break;
         const int slots = slots_of(n);
         if (slots < n) continue;
         for (int m = 1; m <= most_supers; m++) {
-            if (m > 1 && steps < least * n * m) break;
+            if (n * m > fewest && m > 1 && steps < least * n * m) break;
             const double fill = (double)base * n * m / slots, job = steps / (n * m) + (fill > 1.0 ? more : fixed);
             double time = job;
             if (fill > 1.0) time = batch == 1 ? (double)((base * n * m + slots - 1) / slots) * job
                                               : (0.75 * fill > 1.0 ? 0.75 * fill : 1.0) * job + job / 3;
             if (m > 1) time += join;
+            if (n * m < fewest) time += 1e6 * (fewest - n * m);
             if (time < best_time * 0.999) best_time = time, best = Split{n, m};
-            if (fill > 2.0) break;
+            if (fill > 2.0 && n * m >= fewest) break;
         }
     }
     return best;

@@ -51,7 +51,7 @@ constexpr int kMmaWarp = 0, kLoadWarp = 1;  // first, since the scheduler prefer
 constexpr int kBN = 64;              // keys a step
 // A parity says which of two phases a barrier is in, so a waiter must have seen the phase before: the barriers that several
 // warps of a kind wait on in turn are as many as make the same warp wait on each (multiples of 3).
-constexpr int kFree = 6;             // barriers of tiles set free
+constexpr int kTurns = 6;            // barriers of raw stages filled and read, and of tiles set free
 constexpr int kScales = 8;           // steps whose scales are kept
 constexpr float kPUnit = 2.0f;       // log2 of P' / (P * vs / W): P' stays below 2^15 in fp16
 constexpr float kBehind = 12.0f;     // (6: some warp of the eight moved nearly every step, 2,000 clocks each time)
@@ -232,8 +232,8 @@ struct TcSmem {
     // only after its values; with 3 the copies came too late for MT = 1: 2,300 clocks a step)
     static constexpr int kRest = 32 * 1024;  // what follows the stages, at most
     static constexpr int kFit = (227 * 1024 - kRest - kRawAt) / kRawStage;
-    static constexpr int kRaw = kFit >= 6 ? 6 : 3;  // a multiple of the three converters of a kind, see kFree
-    static_assert(kFit >= 3, "raw stages");
+    static constexpr int kRaw = kFit > 6 ? 6 : kFit;
+    static_assert(kRaw >= 3 && kRaw <= kTurns, "raw stages");
     // the partial O of both softmax groups, [256][HDP] fp32, lies over the tiles
     static constexpr int kJoin = 256 * HDP * 4;
     static constexpr int kEnd = kRawAt + kRaw * kRawStage;
@@ -261,9 +261,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
     extern __shared__ __align__(1024) uint8_t raw_smem[];
     uint8_t *smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);
     uint64_t *bar = reinterpret_cast<uint64_t *>(smem + S::kBar);
-    // (slot = step & 1 where there are two, step % kRaw of raw, % kScales of scales, % kFree of tiles set free)
-    uint64_t *raw_full = bar, *raw_empty = raw_full + kRaw, *k_ready = raw_empty + kRaw, *k_free = k_ready + 2,
-             *v_ready = k_free + kFree, *v_free = v_ready + 2, *s_full = v_free + kFree /* [m][slot] */,
+    // (slot = step & 1 where there are two, step % kScales of scales, % kTurns of raw stages and of tiles set free)
+    uint64_t *raw_full = bar, *raw_empty = raw_full + kTurns, *k_ready = raw_empty + kTurns, *k_free = k_ready + 2,
+             *v_ready = k_free + kTurns, *v_free = v_ready + 2, *s_full = v_free + kTurns /* [m][slot] */,
              *p_ready = s_full + 4 /* [m][slot] */, *pv_done = p_ready + 4 /* [m] */, *sc_ready = pv_done + 2,
              *q_ready = sc_ready + kScales, *o_done = q_ready + 1;
     uint32_t *tmem_at = reinterpret_cast<uint32_t *>(o_done + 1);
@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
     const int mine = t1 - t0;
 
     if (tid == 0) {
-        for (int i = 0; i < kRaw; i++) {
+        for (int i = 0; i < kTurns; i++) {
             bar_init(&raw_full[i], 1);
             bar_init(&raw_empty[i], 2);
         }
@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
             bar_init(&p_ready[i], 8);
         }
         for (int i = 0; i < kScales; i++) bar_init(&sc_ready[i], 1);
-        for (int i = 0; i < kFree; i++) {
+        for (int i = 0; i < kTurns; i++) {
             bar_init(&k_free[i], 1);
             bar_init(&v_free[i], 1);
         }
@@ -328,9 +328,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
                     reinterpret_cast<uint4 *>(tiles + ((warp - 2) >> 1) * S::kTile)[i] = make_uint4(0, 0, 0, 0);
             asm volatile("bar.sync 1, 192;" ::: "memory");
             for (int j = (warp - 2) >> 1; j < mine; j += 3) {
-                const int slot = j & 1, rs = j % kRaw, ss = j % kScales;
-                const uint8_t *raw = smem + S::kRawAt + rs * S::kRawStage;
-                if (!bar_wait(&raw_full[rs], (j / kRaw) & 1)) break;
+                const int slot = j & 1, turn = j % kTurns, ss = j % kScales;
+                const uint8_t *raw = smem + S::kRawAt + j % kRaw * S::kRawStage;
+                if (!bar_wait(&raw_full[turn], (j / kTurns) & 1)) break;
                 if (kv) {
                     // the scales, before the tile is free: the softmax of kScales steps ago, their last reader, is done (this
                     // warp's step before last waited for the product of five steps ago)
@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
                     if (lane == 0) bar_arrive(&sc_ready[ss]);
                 }
                 // the tile's last product has ended
-                if (j >= 2 && !bar_wait(&free_[(j - 2) % kFree], ((j - 2) / kFree) & 1)) break;
+                if (j >= 2 && !bar_wait(&free_[(j - 2) % kTurns], ((j - 2) / kTurns) & 1)) break;
 #pragma unroll 1
                 for (int key = lane; key < kBN; key += 32) {
                     const uint8_t *src = raw + kv * S::kRawTile + key * row_bytes;
@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
                 __syncwarp();
                 if (lane == 0) {
                     bar_arrive(&ready[slot]);
-                    bar_arrive(&raw_empty[rs]);
+                    bar_arrive(&raw_empty[turn]);
                 }
             }
         } else if (warp == kMmaWarp) {
@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
                                    k0 + ((slot * S::kTile + (k >> 2) * (kBN * 128) + (k & 3) * 32) >> 4), qk,
                                    part > 0 || k > 0);
                     commit(&s_full[2 * m + (i & 1)]);
-                    if (ALT || m == 1) commit(&k_free[j % kFree]);
+                    if (ALT || m == 1) commit(&k_free[j % kTurns]);
                     return true;
                 };
 #pragma unroll 1
@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
                                 mma_ts(t + 256 + m * 128, t + m * 128 + (i & 1) * 64 + part * 32 + k * 8,
                                        v0 + ((slot * S::kTile + k * 2048) >> 4), pv, i > 0 || part > 0 || k > 0);
                         commit(&pv_done[m]);
-                        if (ALT || m == 1) commit(&v_free[j % kFree]);
+                        if (ALT || m == 1) commit(&v_free[j % kTurns]);
                         ok = scores(m, i + 2);
                     }
                 }
@@ -446,9 +446,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
             // ---------------- raw pages ----------------
             const int run = min(1 << p.bt.page_log2, kBN), runs = kBN / run;  // keys a copy, copies a step
             for (int j = 0; j < mine; j++) {
-                const int st = j % kRaw;
-                if (j >= kRaw && !bar_wait(&raw_empty[st], (j / kRaw - 1) & 1)) break;
-                uint8_t *raw = smem + S::kRawAt + st * S::kRawStage;
+                const int st = j % kTurns, before = j - kRaw;  // the step that had the stage before
+                if (before >= 0 && !bar_wait(&raw_empty[before % kTurns], (before / kTurns) & 1)) break;
+                uint8_t *raw = smem + S::kRawAt + j % kRaw * S::kRawStage;
                 const int key0 = (t0 + j) * kBN, key = key0 + lane * run;
                 const bool on = lane < runs && key < s.len;
                 const uint32_t n = __popc(__ballot_sync(0xffffffffu, on));
@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
                 }
             }
             // copies in flight land before the CTA can end
-            for (int j = mine > kRaw ? mine - kRaw : 0; j < mine; j++) bar_wait(&raw_full[j % kRaw], (j / kRaw) & 1);
+            for (int j = mine > kRaw ? mine - kRaw : 0; j < mine; j++) bar_wait(&raw_full[j % kTurns], (j / kTurns) & 1);
         }
     } else {
         // ---------------- softmax: two threads a row ----------------
@@ -770,7 +770,10 @@ static cudaError_t launch(AttnParams p, int max_len, cudaStream_t stream) {
     if ((long long)p.qtiles * p.kv_heads > 65535) return cudaErrorInvalidConfiguration;
     const long long base = (long long)p.qtiles * p.kv_heads * p.bt.batch;
     // a unit: a step, 1.2 us with two row tiles; a CTA starts, fills and joins in about 8 us, a second kernel takes 4
-    const Split cut = choose_splits(base, p.bt.batch, (double)max_len / kBN, 6.0, 8.0, 3.0, 4.0, most_supers(p),
+    // The tensor core's sums are cut towards zero, 4e-6 of every element over 10,000 keys: an fp32 caller's sequences are
+    // split into at most 8,192 keys a CTA (16 CTAs at most), since the joins round to nearest.
+    const int fewest = sizeof(T) == 4 ? (max_len >= kMaxSplits * 8192 ? kMaxSplits : max_len / 8192 + 1) : 1;
+    const Split cut = choose_splits(base, p.bt.batch, (double)max_len / kBN, 6.0, 8.0, 3.0, 4.0, fewest, most_supers(p),
                                     [&](int n) { return slots((const void *)kernel, n, smem); });
     p.splits = cut.splits;
     p.supers = cut.supers;

@@ -437,8 +437,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 && NT <= 2 ? 2 : 1) t
                 for (int k = 0; k < PER; k += 2) {  // element tile j: elements RUN * r + 2j (rows r), + 2j + 1 (rows r + 8)
                     const uint4 a = make_uint4(vb[k][0], vb[k + 1][0], vb[k][1], vb[k + 1][1]);
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
-{
+                    for (int nt = 0; nt < NT; nt++) {
                         // The products' own sums are cut towards zero: over 10,000 keys that takes 4e-6 off every element. An
                         // fp32 caller's slices are therefore added here, rounded to nearest.
                         constexpr bool APART = sizeof(T) == 4;
@@ -636,45 +635,62 @@ static cudaError_t launch_size(const AttnParams &p, int max_len, cudaStream_t st
     return p.head <= 64 ? launch_rows<T, BITS, 64>(p, max_len, stream) : launch_rows<T, BITS, 128>(p, max_len, stream);
 }
 
-// One block a (new token, sequence): every head's parts, weighted by sum * 2^(max - largest).
+// A thread takes four elements of a (new token, head): the parts of the clusters, weighted by sum * 2^(max - largest). Few
+// rows spread over many blocks, and a thread loads all its parts before it uses one: this is latency only.
 template <typename T>
-__global__ void __launch_bounds__(256) join_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(128) join_kernel(const AttnParams p) {
+    cudaGridDependencySynchronize();  // the blocks are in place when the parts are
     const Sequence s = sequence_at(p, blockIdx.y, &g_attn_error);
     if ((int)blockIdx.x >= s.n) return;
-    const int tok = s.row0 + blockIdx.x, quads = p.head / 4;
-    const float2 *ml = work_ml(p) + (size_t)tok * p.heads;
+    const int tok = s.row0 + blockIdx.x, quads = p.head / 4, i = blockIdx.z * 128 + threadIdx.x;
+    if (i >= p.heads * quads) return;
+    const int head = i / quads, d4 = i - head * quads;
+    const float2 *ml = work_ml(p) + (size_t)tok * p.heads + head;
+    const float *part = p.work + ((size_t)tok * p.heads + head) * p.head + 4 * d4;
     const size_t next = (size_t)p.rows * p.heads;  // rows of one part
-    for (int i = threadIdx.x; i < p.heads * quads; i += 256) {
-        const int head = i / quads, d4 = i - head * quads;
-        float m = -INFINITY, sum = 0.0f;
-        for (int w = 0; w < p.supers; w++) m = fmaxf(m, ml[w * next + head].x);
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-        for (int w = 0; w < p.supers; w++) {
-            const float2 x = ml[w * next + head];
-            const float4 v = *reinterpret_cast<const float4 *>(p.work + (w * next + (size_t)tok * p.heads + head) * p.head + 4 * d4);
-            if (x.y == 0.0f) continue;
-            const float f = x.y * exp2_fast(x.x - m);
-            sum += f;
-            o.x = __fmaf_rn(f, v.x, o.x);
-            o.y = __fmaf_rn(f, v.y, o.y);
-            o.z = __fmaf_rn(f, v.z, o.z);
-            o.w = __fmaf_rn(f, v.w, o.w);
+    float2 x[kMaxSupers];
+    float4 v[kMaxSupers];
+#pragma unroll
+    for (int w = 0; w < kMaxSupers; w++)
+        if (w < p.supers) {
+            x[w] = ml[w * next];
+            v[w] = *reinterpret_cast<const float4 *>(part + w * next * p.head);
         }
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        store4(static_cast<T *>(p.out) + (size_t)tok * p.out_stride + (size_t)head * p.head + 4 * d4,
-               make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
-        if (d4 == 0 && p.lse)
-            p.lse[(size_t)tok * p.heads + head] = sum == 0.0f ? -INFINITY : (m + log2f(sum)) * 0.693147180559945309f;
+    float m = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kMaxSupers; w++)
+        if (w < p.supers) m = fmaxf(m, x[w].x);
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < kMaxSupers; w++) {
+        if (w >= p.supers || x[w].y == 0.0f) continue;
+        const float f = x[w].y * exp2_fast(x[w].x - m);
+        sum += f;
+        o.x = __fmaf_rn(f, v[w].x, o.x);
+        o.y = __fmaf_rn(f, v[w].y, o.y);
+        o.z = __fmaf_rn(f, v[w].z, o.z);
+        o.w = __fmaf_rn(f, v[w].w, o.w);
     }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    store4(static_cast<T *>(p.out) + (size_t)tok * p.out_stride + (size_t)head * p.head + 4 * d4,
+           make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+    if (d4 == 0 && p.lse)
+        p.lse[(size_t)tok * p.heads + head] = sum == 0.0f ? -INFINITY : (m + log2f(sum)) * 0.693147180559945309f;
 }
 
 cudaError_t launch_join(const AttnParams &p, int dtype, cudaStream_t s) {
-    const dim3 grid(p.max_new, p.bt.batch);
-    if (dtype == kF32) join_kernel<float><<<grid, 256, 0, s>>>(p);
-    else if (dtype == kBF16) join_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(p);
-    else join_kernel<__half><<<grid, 256, 0, s>>>(p);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.max_new, p.bt.batch, (p.heads * (p.head / 4) + 127) / 128);
+    cfg.blockDim = dim3(128);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (dtype == kF32) return cudaLaunchKernelEx(&cfg, join_kernel<float>, p);
+    if (dtype == kBF16) return cudaLaunchKernelEx(&cfg, join_kernel<__nv_bfloat16>, p);
+    return cudaLaunchKernelEx(&cfg, join_kernel<__half>, p);
 }
 
 int cluster_slots(const void *kernel, int n, int threads, size_t smem) {

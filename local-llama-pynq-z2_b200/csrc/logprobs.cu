@@ -9,11 +9,12 @@
 // shared-memory word per 16 or 32 elements), so that the streaming loop has no candidate lists and no barriers. Afterwards
 // the top-th largest of the threads' own maxima (its 16 leading bits) is a lower bound of the top-th largest element; the
 // few groups whose maximum reaches it are listed, their vectors read again (from L2), a thread each, and their elements
-// that reach it ranked. Rows with more such elements than the list holds (a
-// vocabulary masked to a few tokens: the rest all equal) take the elements above the bound, then those equal to it in
-// the order of their index; where even the former overflow, `top` rounds of an arg max.
+// that reach it ranked. Rows with more such elements than the list holds (a vocabulary masked to a few tokens: the rest
+// all equal) take the elements above the bound, then those equal to it in the order of their index; where even the former
+// overflow, `top` rounds of an arg max.
 // A few rows: a row is split over a cluster of up to 16 CTAs, joined through distributed shared memory in rank order.
 // Bound: the logits are read once; the exponentials (one a logit, 16 per clock and SM) come close for 16-bit types.
+// 2000 rows of 151,936 bf16 logits, top 20: 119 us (5.1 TB/s); 1000 rows in fp32: 132 us; one row: 9 us.
 #include <cooperative_groups.h>
 #include <limits.h>
 #include <math.h>

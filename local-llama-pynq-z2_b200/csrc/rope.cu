@@ -2,7 +2,8 @@
 // (mvb_rope). The decode step has its rotation inside its attention kernel; this is the operator for callers that keep
 // their own queries and keys.
 //
-// Bound: each element is read and written once; the table row of a token is read once for all its heads.
+// Bound: each element is read and written once; the table row of a token is read once for all its heads (8192 tokens x 40
+// heads of 128, bf16, 64 turned: 5.4 TB/s).
 #include <limits.h>
 
 #include "../../include/matvec_b200.h"
@@ -145,7 +146,7 @@ extern "C" int mvb_rope(const void *x, const int *pos, const float *table, void 
     p.table_rows = table_rows;
     p.pairs = layout;
     // 16 bytes a lane where everything is a multiple of that (8192 tokens x 40 heads of 128, bf16: 43 us with 8 bytes a
-    // lane and 4 heads a warp, 33 us so)
+    // lane and 4 heads a warp, 32 us so)
     const bool wide = dtype != kF32 && rot % 16 == 0 && x_stride % 8 == 0 && out_stride % 8 == 0 &&
                       !(((uintptr_t)x | (uintptr_t)out) & 15);
     const int lane_elems = wide ? 8 : 4, r = 32 / (head <= 8 * lane_elems ? 8 : head <= 16 * lane_elems ? 16 : 32);

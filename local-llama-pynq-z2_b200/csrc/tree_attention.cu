@@ -19,8 +19,11 @@
 // with (key, two rows); movmatrix turns that into the operand of the second product. The order of the head's elements
 // inside a product is free as long as q and k agree, and so is the order of the keys in P v: both are chosen so that a
 // lane reads whole 4- to 16-byte pieces. Keys of a sequence are split over the warps of a CTA and over the CTAs of a
-// cluster (up to 16), whose partial (max, sum, O) are joined in distributed shared memory in a fixed order: one launch,
-// no workspace, the same bits on every run.
+// cluster (up to 16), whose partial (max, sum, O) are joined in distributed shared memory in a fixed order: one launch, no
+// workspace, the same bits on every run. Few long sequences: over several clusters each, so that every SM has a part; the
+// clusters' results go to the caller's workspace and join_kernel adds them.
+// Measured (32 heads of 128 over 8 kv heads, int8, bf16): 64 sequences of 8,000 keys, one token each: 116 us (5.2 TB/s). One
+// of 131,001 keys: 64, 79, 94 us for 8, 16, 24 rows; there a warp's chain over a slice (1.6 us, int4 alike) is the bound.
 #include <cooperative_groups.h>
 #include <limits.h>
 #include <math.h>

@@ -1,6 +1,6 @@
 // mvb_tree_attention for many query rows (new tokens x the query heads of one kv head): trees of dozens of tokens, prompt
 // chunks. Same arithmetic as tree_attention.cu (exact integers in fp16, one scale a row, fp32 statistics), on the
-// 5th-generation tensor cores, since each cached byte now meets 33 to 256 rows.
+// 5th-generation tensor cores, since each cached byte now meets 25 to 256 rows.
 //
 // One CTA: up to MT = 2 tiles of 128 query rows against 64 keys a step. The cache is converted once for all rows: raw
 // pages -> (bulk copies) -> raw bytes -> (converter warps) -> fp16 tiles in the 128-byte swizzled layout, two of each. Keys
@@ -9,9 +9,9 @@
 // (so that the next step's scores stand ready when a softmax ends), then O0 | O1, 128 columns each.
 //
 // Warp roles (768 threads):
-//   warp 0          one thread issues the MMAs: PV0 PV1 QK0'' QK1'' a step. (The oldest warp, which the scheduler prefers:
+//   warp 0          one thread issues the MMAs: PV0 QK0'' PV1 QK1'' a step. (The oldest warp, which the scheduler prefers:
 //                   as warp 12 it waited for issue slots behind the softmax.)
-//   warp 1          bulk copies of the raw pages, kRaw stages ahead.
+//   warp 1          bulk copies of the raw pages, as many stages ahead as fit (3 to 6).
 //   warps 2, 4, 6 and 3, 5, 7  converters of K, of V, a step's tile a warp: bytes -> fp16; the scales.
 //   warps 8-15, 16-23  softmax of row tile 0, 1: two threads a row, 32 of the step's keys each, so that every scheduler has
 //                   four such warps to hide one another's latencies (with one thread a row, 64 keys each, a step took 2,350
@@ -21,7 +21,9 @@
 //                   the barrier that also keeps either's P off the other's unread S, and exchange their maxima only then.
 //                   The unit's factor is folded into the exponent, so it multiplies P and the row's sum alike.
 // What bounds it: for two row tiles of head 128 and 64 keys the exponentials take 1,024 clocks (16 a clock), the MMAs
-// 1,280 (QK at N = 64 waits for shared memory: 48 clocks a product against 32), shared memory 1,150.
+// 1,280 (QK at N = 64 waits for shared memory: 48 clocks a product against 32), and shared memory carries 224 KB, 1,800
+// clocks (QK's operands 96, PV's 32, the conversion 64, the softmax's scales 32); the step takes about 2,300. 16 trees of 64
+// tokens, 16,000 keys, 32 heads of 128 over 8 kv heads, int8, bf16: 172 us (621 TFLOP/s).
 // Up to 128 query rows (MT = 1): both softmax groups take the same rows, for every other step each, with an O and
 // (max, sum) of their own; the two parts are joined like those of the cluster.
 // The keys of a sequence are split over the CTAs of a cluster, joined in distributed shared memory in a fixed order.
@@ -54,7 +56,7 @@ constexpr int kBN = 64;              // keys a step
 constexpr int kTurns = 6;            // barriers of raw stages filled and read, and of tiles set free
 constexpr int kScales = 8;           // steps whose scales are kept
 constexpr float kPUnit = 2.0f;       // log2 of P' / (P * vs / W): P' stays below 2^15 in fp16
-constexpr float kBehind = 12.0f;     // (6: some warp of the eight moved nearly every step, 2,000 clocks each time)
+constexpr float kBehind = 12.0f;     // (at 6 one of a row tile's warps moved nearly every step, 2,000 clocks each time)
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }

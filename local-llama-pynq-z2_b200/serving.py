@@ -88,6 +88,14 @@ def _rows(name, t, heads, head):
     return s0 if shape[0] > 1 else shape[1] * shape[2]  # a single row's stride says nothing
 
 
+def _out_rows(name, t, heads, head):
+    """_rows of a tensor that is written: its rows must not share memory (an expanded one's do)."""
+    stride = _rows(name, t, heads, head)
+    if stride < t.shape[1] * t.shape[2]:
+        raise ValueError(f"{name}: rows {stride} elements apart overlap")
+    return stride
+
+
 def _int32(name, t, *shape):
     if t.dtype is not _T.int32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} is {t.dtype} {tuple(t.shape)}: contiguous int32 {shape} is needed")
@@ -214,7 +222,7 @@ def rope(x, positions, table, out=None, layout="half", stream=None):
     out = x if out is None else out
     xs = _rows("x", x, None, None)
     n, heads, head = x.shape
-    os_ = _rows("out", out, heads, head)
+    os_ = _out_rows("out", out, heads, head)
     if out.dtype is not x.dtype or out.shape[0] != n:
         raise ValueError("out must be like x")
     _int32("positions", positions, n)
@@ -252,8 +260,8 @@ def kv_append(cache, k, v, pages, cu, lens, positions=None, rope=None, layout="h
     if q is not None:
         if rope is None or q_out is None:
             raise ValueError("queries need a rope table and q_out")
-        heads = q.shape[1]
-        qs, qos = _rows("q", q, None, cache.head), _rows("q_out", q_out, heads, cache.head)
+        qs, heads = _rows("q", q, None, cache.head), q.shape[1]
+        qos = _out_rows("q_out", q_out, heads, cache.head)
         if q.shape[0] != n or q_out.shape[0] != n or q.dtype is not dtype or q_out.dtype is not dtype:
             raise ValueError("q and q_out must have k's rows and type")
         qp, qop = q.data_ptr(), q_out.data_ptr()
@@ -266,7 +274,7 @@ def kv_read(cache, pages, cu, lens, k_out, v_out, stream=None):
     bfloat16 or float16) become sequence b's positions lens[b] and on (lens of zeros and cu of running lengths: whole
     contexts). integer * scale, rounded to the output's type."""
     _T or _torch()
-    ks, vs = _rows("k_out", k_out, cache.kv_heads, cache.head), _rows("v_out", v_out, cache.kv_heads, cache.head)
+    ks, vs = (_out_rows(name, t, cache.kv_heads, cache.head) for name, t in (("k_out", k_out), ("v_out", v_out)))
     n = k_out.shape[0]
     if v_out.shape[0] != n or v_out.dtype is not k_out.dtype:
         raise ValueError("v_out must be like k_out")
@@ -306,7 +314,7 @@ def tree_attention(q, cache, pages, cu, lens, out, tree=None, scale=None, max_ne
     decides how finely the work is split. lse (rows, heads) float32: the log of the sum of exponentials. A row that may
     see nothing gives zeros and lse -inf."""
     _T or _torch()
-    qs, os_ = _rows("q", q, None, cache.head), _rows("out", out, None, cache.head)
+    qs, os_ = _rows("q", q, None, cache.head), _out_rows("out", out, None, cache.head)
     n, heads, head = shape = q.shape
     dtype = q.dtype
     if out.shape != shape or out.dtype is not dtype:

@@ -131,6 +131,18 @@ def test_python_checks(mvb):
             mvb.logprobs(*a)
 
 
+def test_overlapping_outputs(mvb):
+    """Rows that share memory may be read, not written."""
+    x, pos, table = torch.zeros(3, 4, 64), torch.zeros(3, dtype=torch.int32), torch.zeros(10, 64)
+    for out in (torch.zeros(1, 4, 64).expand(3, 4, 64), torch.zeros(1000).as_strided((3, 4, 64), (128, 64, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            mvb.rope(x, pos, table, out=out)
+    with pytest.raises(ValueError, match="overlap"):  # in place
+        mvb.rope(x[:1].expand(3, 4, 64), pos, table)
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        mvb.rope(x[:1].expand(3, 4, 64), pos, table, out=torch.zeros(3, 4, 64))
+
+
 def test_cache_geometry():
     """The slots of a 4-bit cache: two elements a byte."""
     from conftest import load_pkg

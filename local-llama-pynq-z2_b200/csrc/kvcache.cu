@@ -133,7 +133,7 @@ __device__ __forceinline__ void quantize_store(const Row<E> &f, const F &exact, 
 
 // One warp: 32 / W heads' keys and values of one token into the cache, or some heads of its queries rotated.
 template <typename T, int W, int BITS, int E>
-__global__ void __launch_bounds__(256, 3) kv_append_kernel(const KvParams p) {
+__global__ void __launch_bounds__(256, 4) kv_append_kernel(const KvParams p) {
     constexpr int R = 32 / W;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane & (W - 1), sub = lane / W;
     // a block's warps do alike work on neighbouring tokens (a block of both kinds keeps its queries' warps waiting idle for

@@ -170,8 +170,13 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 && NT <= 2 ? 2 : 1) t
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
 
-    // q: a warp scales a row by a power of two into fp32 (staged behind the pipeline), then every warp builds fragments
-    float *qrow = reinterpret_cast<float *>(pipe + kWarps * S::kWarp);  // [ROWS][HDP]
+    // q: a warp scales its rows by powers of two into fp32, then every warp builds fragments. The rows are staged in the
+    // rings' last stages, which the first slices above leave free: with room of their own (8 KB) two CTAs of 16 rows a kv
+    // head of 128 in 8 bits miss an SM's shared memory by 1.3 KB each.
+    static_assert((kStages - 1) * S::kStage + ((ROWS - 1) / kWarps + 1) * HDP * 4 <= S::kWarp, "q rows in the last stage");
+    auto qrow = [&](int i) {
+        return reinterpret_cast<float *>(pipe + i % kWarps * S::kWarp + (kStages - 1) * S::kStage) + i / kWarps * HDP;
+    };
     for (int i = warp; i < ROWS; i += kWarps) {
         const int R = R0 + i;
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -185,14 +190,14 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 && NT <= 2 ? 2 : 1) t
         const int k = max(-100, min(e - 127 - 8, 119));
         if (4 * lane < HDP) {
             const float f = pow2(-k);
-            reinterpret_cast<float4 *>(qrow + i * HDP)[lane] = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+            reinterpret_cast<float4 *>(qrow(i))[lane] = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
         }
         if (lane == 0) row_factor[i] = pow2(k);
     }
     __syncthreads();
     for (int i = threadIdx.x; i < NT * KS * 32; i += kWarps * 32) {
         const int ln = i & 31, ks = (i >> 5) % KS, nt = (i >> 5) / KS;
-        const float *a = qrow + (nt * 8 + (ln >> 2)) * HDP;
+        const float *a = qrow(nt * 8 + (ln >> 2));
         float f[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) f[e] = a[element_of<BITS>(ks, ln & 3, e)];
@@ -577,7 +582,7 @@ static cudaError_t launch_warps(AttnParams p, int max_len, cudaStream_t stream) 
     using S = Slice<HDP, BITS>;
     constexpr int ROWS = 8 * NT;
     constexpr size_t frag = (size_t)Parts<T>::kQ * NT * (HDP / 16) * 256;
-    constexpr size_t ring = (size_t)kWarps * S::kWarp + (size_t)ROWS * HDP * 4, join = (size_t)kWarps * ROWS * HDP * 4;
+    constexpr size_t ring = (size_t)kWarps * S::kWarp, join = (size_t)kWarps * ROWS * HDP * 4;
     constexpr size_t smem = frag + (ring > join ? ring : join);
     static_assert(smem <= 227 * 1024 - 8192, "shared memory of a CTA");
     auto kernel = tree_attention_kernel<T, BITS, HDP, NT, kWarps>;

@@ -591,9 +591,12 @@ static cudaError_t launch_warps(AttnParams p, int max_len, cudaStream_t stream) 
     if (e != cudaSuccess) return e;
     p.qtiles = (int)(((long long)p.max_new * p.group + ROWS - 1) / ROWS);
     if ((long long)p.qtiles * p.kv_heads > 65535) return cudaErrorInvalidConfiguration;
-    // a unit: one slice a warp, about 2 us of streaming; a CTA starts and joins in about 6 us, a second kernel in 4
+    // a unit: one slice a warp, 0.7 us (2 where two CTAs of an SM stream); a CTA starts and joins in about 6 us, a second
+    // kernel in 2; a cluster's join grows with its CTAs (one sequence of 2,000 keys, 8 kv heads, int8, 4 | 16 rows: clusters
+    // of 4, 8, 16 take 11.6, 9.7, 10.0 | 15.4, 13.7, 14.8 us)
     const Split cut = choose_splits((long long)p.qtiles * p.kv_heads * p.bt.batch, p.bt.batch,
-                                    (double)max_len / (kWarps * S::kKeys), 3.0, 8.0, 2.0, 1.0, 1, most_supers(p),
+                                    (double)max_len / (kWarps * S::kKeys), 3.0, 8.0, NT == 1 ? 0.14 : 0.26, 2.0,
+                                    1.0, 1, most_supers(p),
                                     [&](int n) { return cluster_slots((const void *)kernel, n, kWarps * 32, smem); });
     p.splits = cut.splits;
     p.supers = cut.supers;
@@ -617,10 +620,10 @@ template <typename T, int BITS, int HDP, int NT>
 static cudaError_t launch(const AttnParams &p, int max_len, cudaStream_t stream) {
     using S = Slice<HDP, BITS>;
     // Two CTAs of 8 warps an SM; or, where the jobs are so few that clusters of 16 leave one CTA an SM, and the sequences
-    // long enough for it, one of 16 warps. Three column tiles need more registers: one CTA of 12 warps.
+    // long enough for it, one of 16 warps (16 jobs of 131,001 int8 keys: 102 us so, 90 with 8 warps). Three column tiles need more registers: one CTA of 12 warps.
     const long long base = ((long long)p.max_new * p.group + 8 * NT - 1) / (8 * NT) * p.kv_heads * p.bt.batch;
     if constexpr (NT <= 2) {
-        if (base <= 18 && max_len >= 2 * 16 * 16 * S::kKeys) return launch_warps<T, BITS, HDP, NT, 16>(p, max_len, stream);
+        if (base <= 9 && max_len >= 2 * 16 * 16 * S::kKeys) return launch_warps<T, BITS, HDP, NT, 16>(p, max_len, stream);
         return launch_warps<T, BITS, HDP, NT, 8>(p, max_len, stream);
     } else {
         return launch_warps<T, BITS, HDP, NT, 12>(p, max_len, stream);

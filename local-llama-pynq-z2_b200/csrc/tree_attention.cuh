@@ -109,16 +109,16 @@ int cluster_slots(const void *kernel, int n, int threads, size_t smem);
 
 // Over how many CTAs of a cluster (splits) and how many clusters (supers, at most most_supers) a sequence's keys are split,
 // so that the estimated time is least: `base` jobs without a split, `steps` units of work each for the longest sequence,
-// `fixed` units to start, fill and join a CTA (`more` where the CTAs exceed one wave) and `join` for a second kernel, at
-// least `least` units a CTA and, where slots allow, `fewest` CTAs. One
-// sequence: its jobs are alike and run in whole waves. Several: three quarters of the longest on average, in no order, and
-// the last jobs end a third of a job apart.
+// `fixed` units to start, fill and join a CTA (`more` where the CTAs exceed one wave), `each` for every CTA of the cluster
+// that it is joined with, and `join` for a second kernel, at least `least` units a CTA and, where slots allow, `fewest`
+// CTAs. All in one wave: whole units. More, of one sequence: its jobs are alike and run in whole waves. Several: three
+// quarters of the longest on average, in no order, and the last jobs end a third of a job apart.
 struct Split {
     int splits, supers;
 };
 template <typename F>
-inline Split choose_splits(long long base, int batch, double steps, double fixed, double more, double join, double least,
-                           int fewest, int most_supers, const F &slots_of) {
+inline Split choose_splits(long long base, int batch, double steps, double fixed, double more, double each,
+                           double join, double least, int fewest, int most_supers, const F &slots_of) {
     Split best = {1, 1};
     double best_time = 1e300;
     for (int n = 1; n <= kMaxSplits; n++) {
@@ -127,7 +127,9 @@ inline Split choose_splits(long long base, int batch, double steps, double fixed
         if (slots < n) continue;
         for (int m = 1; m <= most_supers; m++) {
             if (n * m > fewest && m > 1 && steps < least * n * m) break;
-            const double fill = (double)base * n * m / slots, job = steps / (n * m) + (fill > 1.0 ? more : fixed);
+            const double fill = (double)base * n * m / slots, units = steps / (n * m);
+            const double job = (fill > 1.0 ? units + more : ceil(units) + fixed) + n * each;
+            if (each > 0.0 && fill <= 1.0 && (n & (n - 1))) continue;  // clusters of 6 or 12 take longer than of 8 or 16
             double time = job;
             if (fill > 1.0) time = batch == 1 ? (double)((base * n * m + slots - 1) / slots) * job
                                               : (0.75 * fill > 1.0 ? 0.75 * fill : 1.0) * job + job / 3;

@@ -775,7 +775,7 @@ static cudaError_t launch(AttnParams p, int max_len, cudaStream_t stream) {
     // The tensor core's sums are cut towards zero, 4e-6 of every element over 10,000 keys: an fp32 caller's sequences are
     // split into at most 8,192 keys a CTA (16 CTAs at most), since the joins round to nearest.
     const int fewest = sizeof(T) == 4 ? (max_len >= kMaxSplits * 8192 ? kMaxSplits : max_len / 8192 + 1) : 1;
-    const Split cut = choose_splits(base, p.bt.batch, (double)max_len / kBN, 6.0, 8.0, 3.0, 4.0, fewest, most_supers(p),
+    const Split cut = choose_splits(base, p.bt.batch, (double)max_len / kBN, 6.0, 8.0, 0.0, 3.0, 4.0, fewest, most_supers(p),
                                     [&](int n) { return slots((const void *)kernel, n, smem); });
     p.splits = cut.splits;
     p.supers = cut.supers;

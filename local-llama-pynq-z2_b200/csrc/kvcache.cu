@@ -131,7 +131,9 @@ __device__ __forceinline__ void quantize_store(const Row<E> &f, const F &exact, 
     if (l == 0) *scale_at = bad ? __int_as_float(0x7FC00000) : scale;
 }
 
-// One warp: 32 / W heads' keys and values of one token into the cache, or some heads of its queries rotated.
+// One warp: 32 / W heads' keys and values of one token into the cache, or some heads of its queries rotated. Four blocks an
+// SM hide more of the rows' loads and of the exchanges of the maxima than the few spills of 64 registers cost (8 prompts of
+// 2,000 tokens, 32 + 8 heads of 128, bf16: 88 us against 94 with 80 registers and three blocks).
 template <typename T, int W, int BITS, int E>
 __global__ void __launch_bounds__(256, 4) kv_append_kernel(const KvParams p) {
     constexpr int R = 32 / W;

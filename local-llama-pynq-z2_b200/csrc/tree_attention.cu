@@ -23,7 +23,7 @@
 // workspace, the same bits on every run. Few long sequences: over several clusters each, so that every SM has a part; the
 // clusters' results go to the caller's workspace and join_kernel adds them.
 // Measured (32 heads of 128 over 8 kv heads, int8, bf16): 64 sequences of 8,000 keys, one token each: 116 us (5.2 TB/s). One
-// of 131,001 keys: 64, 79, 94 us for 8, 16, 24 rows; there a warp's chain over a slice (1.6 us, int4 alike) is the bound.
+// of 131,001 keys: 65, 80, 94 us for 8, 16, 24 rows; there a warp's chain over a slice (1.6 us, int4 alike) is the bound.
 #include <cooperative_groups.h>
 #include <limits.h>
 #include <math.h>

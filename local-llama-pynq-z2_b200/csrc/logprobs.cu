@@ -14,7 +14,7 @@
 // overflow, `top` rounds of an arg max.
 // A few rows: a row is split over a cluster of up to 16 CTAs, joined through distributed shared memory in rank order.
 // Bound: the logits are read once; the exponentials (one a logit, 16 per clock and SM) come close for 16-bit types.
-// 2000 rows of 151,936 bf16 logits, top 20: 119 us (5.1 TB/s); 1000 rows in fp32: 132 us; one row: 9 us.
+// 2000 rows of 151,936 bf16 logits, top 20: 119 us (5.1 TB/s); 1000 rows in fp32: 121 us; one row: 9 us.
 #include <cooperative_groups.h>
 #include <limits.h>
 #include <math.h>
@@ -578,8 +578,10 @@ static cudaError_t launch_threads(Params p, cudaStream_t stream) {
     auto kernel = logprobs_kernel<T, TOP, kThreads>;
     // a row over more CTAs while the grid leaves SMs idle and each CTA still has a chunk, or where its maxima would not
     // fit in shared memory
+    // (200 rows of fp32: 34 us whole, 27 us in halves that run at once; 148 rows in quarters: 33 us, in halves 25)
     int splits = 1;
-    while (splits < 16 && (((long long)p.rows * splits * 2 <= 148 * 2 && (long long)kChunk * splits * 2 <= p.vocab) ||
+    while (splits < 16 && (((long long)p.rows * splits * 2 <= (splits == 1 ? 148 * 3 : 148 * 2) &&
+                            (long long)kChunk * splits * 2 <= p.vocab) ||
                            (TOP && (long long)p.vocab / splits / kChunk >= 150)))
         splits *= 2;
     p.splits = splits;
@@ -604,11 +606,26 @@ static cudaError_t launch_threads(Params p, cudaStream_t stream) {
     return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
+// The rows that whole waves hold, one row a CTA: the time of p.rows rows goes with it, since rows are alike.
+template <typename T, bool TOP, int kThreads>
+static long long rows_of_waves(const Params &p) {
+    static const size_t fixed = [] {
+        cudaFuncAttributes a = {};
+        return cudaFuncGetAttributes(&a, logprobs_kernel<T, TOP, kThreads>) == cudaSuccess ? a.sharedSizeBytes : (size_t)0;
+    }();
+    const size_t smem = TOP ? ((size_t)p.vocab / (kThreads * 32) + 2) * kThreads * 4 : 0;
+    const long long fit = 228 * 1024 / (long long)(fixed + smem + 1024), most = 768 / kThreads;
+    const long long slots = 148 * (fit < 1 ? 1 : fit < most ? fit : most);
+    return (p.rows + slots - 1) / slots * slots;
+}
+
 template <typename T, bool TOP>
 static cudaError_t launch(const Params &p, cudaStream_t stream) {
-    // many rows: half the threads a row and twice the rows an SM, so that the ends of rows (joins, candidates) of some
-    // stand beside the streaming of others
-    return p.rows >= 148 * 4 ? launch_threads<T, TOP, 128>(p, stream) : launch_threads<T, TOP, 256>(p, stream);
+    // 128 threads a row and more rows an SM, so that the ends of rows (joins, candidates) of some stand beside the streaming
+    // of others, unless 256 fill their waves better (bf16, top 20, 128 | 256: 740 rows 49 | 55 us, 888 rows 74 | 60, 1,500
+    // rows 112 | 102, 2,000 rows 119 | 128)
+    if (rows_of_waves<T, TOP, 128>(p) <= rows_of_waves<T, TOP, 256>(p)) return launch_threads<T, TOP, 128>(p, stream);
+    return launch_threads<T, TOP, 256>(p, stream);
 }
 
 int logp_take_error(cudaStream_t s) {

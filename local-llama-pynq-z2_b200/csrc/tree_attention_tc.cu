@@ -774,7 +774,7 @@ static cudaError_t launch(AttnParams p, int max_len, cudaStream_t stream) {
     // a unit: a step, 1.2 us with two row tiles; a CTA starts, fills and joins in about 8 us, a second kernel takes 4
     // The tensor core's sums are cut towards zero, 3e-6 to 4e-6 of every element over 4,096 keys with P in two parts: an
     // fp32 caller's sequences are split into at most that many a CTA while 16 CTAs (32 with a workspace) suffice, since the
-    // joins round to nearest. Against 8,192 a CTA this takes the worst of 5,000 drawn calls of 20,000 to 131,072 keys from
+    // joins round to nearest. Against 8,192 a CTA this takes the worst of some thousand random calls of 20,000 keys and more from
     // 1.0e-5 to 9e-6 off the fp32 formula, for 6 % of the time at 131,001 keys.
     const int most = kMaxSplits * (most_supers(p) > 1 ? 2 : 1);
     const int fewest = sizeof(T) == 4 ? (max_len >= most * 4096 ? most : max_len / 4096 + 1) : 1;

@@ -638,6 +638,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
         auto share = [&](int n) { return ALT ? max(0, n - m + 1) / 2 : max(0, n); };
         const int steps = share(mine), plain = share(min(mine, s.ctx / kBN - t0));
         bool ok = true;
+        // A warp whose 32 rows all lie behind the last only keeps the barriers' count: what the product makes of its rows
+        // is not read.
+        const bool idle = R - lane >= nrows;
+#pragma unroll 1
+        for (int i = 0; idle && i < steps && ok; i++) {
+            ok = bar_wait(&s_full[2 * m + (i & 1)], (i >> 1) & 1);
+            if (ok && lane == 0) bar_arrive(&p_ready[2 * m + (i & 1)]);
+        }
+        ok = ok && !idle;
 #pragma unroll 1
         for (int i = 0; i < plain && ok; i++) ok = step(i, std::false_type{});
 #pragma unroll 1

@@ -53,12 +53,15 @@ __device__ __forceinline__ Sequence sequence_at(const AttnParams &p, int b, int 
     return s;
 }
 
-// The page of position pos (in range of the table): page 0 with the error noted where the table names none.
-__device__ __forceinline__ int page_of(const AttnParams &p, int b, int pos, int *error) {
-    const int pg = p.bt.table[(size_t)b * p.bt.table_cols + (pos >> p.bt.page_log2)];
+// A page that the table names: page 0 with the error noted where there is none.
+__device__ __forceinline__ int checked_page(const AttnParams &p, int pg, int *error) {
     if ((unsigned)pg < (unsigned)p.bt.pages) return pg;
     rows::note(error, rows::kBadPage);
     return 0;
+}
+// The page of position pos (in range of the table).
+__device__ __forceinline__ int page_of(const AttnParams &p, int b, int pos, int *error) {
+    return checked_page(p, p.bt.table[(size_t)b * p.bt.table_cols + (pos >> p.bt.page_log2)], error);
 }
 
 // Whether new token i of the sequence may see position t.

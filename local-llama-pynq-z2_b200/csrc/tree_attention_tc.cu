@@ -228,16 +228,20 @@ struct TcSmem {
     static constexpr int kV = kK + 2 * kTile;                     // [2]
     static constexpr int kRawRow = HDP * BITS / 8;
     static constexpr int kRawTile = kBN * kRawRow;
-    static constexpr int kRawAt = kV + 2 * kTile;                 // [kRaw][K | V | ks | vs]
-    static constexpr int kRawStage = 2 * kRawTile + 2 * kBN * 4;
-    // raw stages: as many as fit, up to 6 (keys are converted up to four steps before their values are, and a stage is free
-    // only after its values; with 3 the copies came too late for MT = 1: 2,300 clocks a step)
+    static constexpr int kRawAt = kV + 2 * kTile;                 // [kRaw] K
+    static constexpr int kRawV = kRawTile + 2 * kBN * 4;          // a stage of V | ks | vs
+    static constexpr int kRawStage = kRawTile + kRawV;
+    // raw stages of keys and of values, as many as fit, up to 6; rings of their own, since keys are converted up to four
+    // steps before their values are
     static constexpr int kRest = 32 * 1024;  // what follows the stages, at most
     static constexpr int kFit = (227 * 1024 - kRest - kRawAt) / kRawStage;
-    static constexpr int kRaw = kFit > 6 ? 6 : kFit;
-    static_assert(kRaw >= 3 && kRaw <= kTurns, "raw stages");
+    static constexpr int kRaw = kFit >= 6 ? 6 : MT == 1 && kFit == 5 ? 4 : kFit;
+    // MT = 1: the barrier of step j + kRaw (% kTurns) was step j + kRaw - kTurns's: complete when step j's stage is refilled, since
+    // j's tile was only free after step j - 2 (or it is the same warp's); not so for 5 stages
+    static_assert(kRaw >= 3 && !(MT == 1 && kRaw == 5), "raw stages");
     // the partial O of both softmax groups, [256][HDP] fp32, lies over the tiles
     static constexpr int kJoin = 256 * HDP * 4;
+    static constexpr int kRawVAt = kRawAt + kRaw * kRawTile;      // [kRaw] V | ks | vs
     static constexpr int kEnd = kRawAt + kRaw * kRawStage;
     static constexpr int kScale = kEnd > kJoin ? kEnd : kJoin;    // [kScales][kk | vv] fp32
     static constexpr int kRow = kScale + kScales * 2 * kBN * 4;   // row factors [MT][128]
@@ -249,7 +253,7 @@ struct TcSmem {
     static constexpr bool kPmInside = kEnd - kJoin >= kPmBytes;
     static constexpr int kPm = kPmInside ? kJoin : kAllEnd;
     static constexpr int kBar = kAllEnd + (kPmInside ? 0 : kPmBytes);
-    static constexpr size_t kBytes = kBar + 512 + 1024;           // + alignment
+    static constexpr size_t kBytes = kBar + 640 + 1024;           // + alignment
     static_assert(kBytes <= 227 * 1024, "shared memory of a CTA");
 };
 
@@ -264,12 +268,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
     uint8_t *smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);
     uint64_t *bar = reinterpret_cast<uint64_t *>(smem + S::kBar);
     // (slot = step & 1 where there are two, step % kScales of scales, % kTurns of raw stages and of tiles set free)
-    uint64_t *raw_full = bar, *raw_empty = raw_full + kTurns, *k_ready = raw_empty + kTurns, *k_free = k_ready + 2,
+    uint64_t *raw_full = bar, *raw_empty = raw_full + 2 * kTurns /* K, V */, *k_ready = raw_empty + 2 * kTurns, *k_free = k_ready + 2,
              *v_ready = k_free + kTurns, *v_free = v_ready + 2, *s_full = v_free + kTurns /* [m][slot] */,
              *p_ready = s_full + 4 /* [m][slot] */, *pv_done = p_ready + 4 /* [m] */, *sc_ready = pv_done + 2,
              *q_ready = sc_ready + kScales, *o_done = q_ready + 1;
     uint32_t *tmem_at = reinterpret_cast<uint32_t *>(o_done + 1);
-    float *vmax = reinterpret_cast<float *>(bar + 50);  // [kScales]
+    float *vmax = reinterpret_cast<float *>(bar + 62);  // [kScales]
     float *row_factor = reinterpret_cast<float *>(smem + S::kRow);
     float *cta_m = reinterpret_cast<float *>(smem + S::kMl), *cta_l = cta_m + 256;
 
@@ -284,9 +288,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
     const int mine = t1 - t0;
 
     if (tid == 0) {
-        for (int i = 0; i < kTurns; i++) {
+        for (int i = 0; i < 2 * kTurns; i++) {
             bar_init(&raw_full[i], 1);
-            bar_init(&raw_empty[i], 2);
+            bar_init(&raw_empty[i], 1);
         }
         for (int i = 0; i < 2; i++) {
             bar_init(&k_ready[i], 1);
@@ -318,6 +322,36 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
     const int row_bytes = p.head * BITS / 8;
 
     if (warp < 8) {
+        // raw pages
+        const int run = min(1 << p.bt.page_log2, kBN), runs = kBN / run;  // keys a copy, copies a step
+        const int *entries = p.bt.table + (size_t)b * p.bt.table_cols;
+        auto entry = [&](int j) {  // this lane's entry of the page table in step j
+            const int key = (t0 + j) * kBN + lane * run;
+            return lane < runs && j < mine && key < s.len ? entries[key >> p.bt.page_log2] : 0;
+        };
+        auto stage = [&](int kv, int j) {
+            return smem + (kv ? S::kRawVAt + j % kRaw * S::kRawV : S::kRawAt + j % kRaw * S::kRawTile);
+        };
+        auto load = [&](int kv, int j, int found) {  // a step's keys, or its values and both scales
+            uint64_t *full = &raw_full[kv * kTurns + j % kTurns];
+            uint8_t *raw = stage(kv, j);
+            const int key = (t0 + j) * kBN + lane * run;
+            const bool on = lane < runs && key < s.len;
+            const uint32_t n = __popc(__ballot_sync(0xffffffffu, on));
+            if (lane == 0) bar_expect(full, n * (uint32_t)run * (row_bytes + (kv ? 8 : 0)));
+            __syncwarp();
+            if (on) {
+                const size_t row = (((size_t)checked_page(p, found, &g_tc_error) * p.kv_heads + kvh) << p.bt.page_log2) +
+                                   (key & ((1 << p.bt.page_log2) - 1));
+                const uint32_t bytes = run * row_bytes;
+                bulk_load(raw + lane * bytes, (kv ? p.vq : p.kq) + row * row_bytes, bytes, full);
+                if (kv) {
+                    uint8_t *sc = raw + S::kRawTile + lane * run * 4;
+                    bulk_load(sc, p.ks + row, run * 4, full);
+                    bulk_load(sc + kBN * 4, p.vs + row, run * 4, full);
+                }
+            }
+        };
         if (warp >= 2) {
             // ---------------- converters: a tile a warp, two keys a lane ----------------
             // warps 2, 4, 6 take the keys of every third step, 3, 5, 7 the values (two warps a tile, every tile: waits and
@@ -329,15 +363,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
                 for (int i = lane; i < S::kTile / 16; i += 32)
                     reinterpret_cast<uint4 *>(tiles + ((warp - 2) >> 1) * S::kTile)[i] = make_uint4(0, 0, 0, 0);
             asm volatile("bar.sync 1, 192;" ::: "memory");
-            for (int j = (warp - 2) >> 1; j < mine; j += 3) {
+            // ALT: a warp that has converted a step's tile refills its stage with the step kRaw ahead (a loader, which shares
+            // its scheduler with the softmax, came too late: one sequence of 131,001 keys, 64 rows, 123 us against 105)
+            int j = (warp - 2) >> 1;
+            if (ALT) {
+                const int found0 = entry(j), found1 = entry(j + 3);
+                if (j < mine) load(kv, j, found0);
+                if (j + 3 < min(mine, kRaw)) load(kv, j + 3, found1);
+            }
+            for (; j < mine; j += 3) {
+                const int found = ALT ? entry(j + kRaw) : 0;
                 const int slot = j & 1, turn = j % kTurns, ss = j % kScales;
-                const uint8_t *raw = smem + S::kRawAt + j % kRaw * S::kRawStage;
-                if (!bar_wait(&raw_full[turn], (j / kTurns) & 1)) break;
+                const uint8_t *raw = stage(kv, j);
+                if (!bar_wait(&raw_full[kv * kTurns + turn], (j / kTurns) & 1)) break;
                 if (kv) {
                     // the scales, before the tile is free: the softmax of kScales steps ago, their last reader, is done (this
                     // warp's step before last waited for the product of five steps ago)
                     float *sc = reinterpret_cast<float *>(smem + S::kScale) + ss * 2 * kBN;
-                    const float *rsc = reinterpret_cast<const float *>(raw + 2 * S::kRawTile);
+                    const float *rsc = reinterpret_cast<const float *>(raw + S::kRawTile);
                     float mv = 0.0f;
 #pragma unroll
                     for (int key = lane; key < kBN; key += 32) {
@@ -357,7 +400,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
                 if (j >= 2 && !bar_wait(&free_[(j - 2) % kTurns], ((j - 2) / kTurns) & 1)) break;
 #pragma unroll 1
                 for (int key = lane; key < kBN; key += 32) {
-                    const uint8_t *src = raw + kv * S::kRawTile + key * row_bytes;
+                    const uint8_t *src = raw + key * row_bytes;
                     uint8_t *dst = tiles + slot * S::kTile + key * 128;
                     // the lanes of a quarter warp start at different pieces: different banks
                     if (pieces == HDP / 16) {
@@ -388,11 +431,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) {
-                    bar_arrive(&ready[slot]);
-                    bar_arrive(&raw_empty[turn]);
-                }
+                if (lane == 0) bar_arrive(&ready[slot]);
+                if (!ALT && lane == 0) bar_arrive(&raw_empty[kv * kTurns + turn]);
+                if (ALT && j + kRaw < mine) load(kv, j + kRaw, found);
             }
+            // gave up: copies in flight land before the CTA can end
+            for (int n = max(0, j - 2); ALT && j < mine && n < min(mine, j + kRaw); n++)
+                bar_wait(&raw_full[kv * kTurns + n % kTurns], (n / kTurns) & 1);
         } else if (warp == kMmaWarp) {
             // ---------------- MMA issue ----------------
             if (mine > 0 && elect_one()) {
@@ -444,32 +489,30 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
                 }
                 commit(o_done);
             }
-        } else if (warp == kLoadWarp) {
-            // ---------------- raw pages ----------------
-            const int run = min(1 << p.bt.page_log2, kBN), runs = kBN / run;  // keys a copy, copies a step
-            for (int j = 0; j < mine; j++) {
-                const int st = j % kTurns, before = j - kRaw;  // the step that had the stage before
-                if (before >= 0 && !bar_wait(&raw_empty[before % kTurns], (before / kTurns) & 1)) break;
-                uint8_t *raw = smem + S::kRawAt + j % kRaw * S::kRawStage;
-                const int key0 = (t0 + j) * kBN, key = key0 + lane * run;
-                const bool on = lane < runs && key < s.len;
-                const uint32_t n = __popc(__ballot_sync(0xffffffffu, on));
-                if (lane == 0) bar_expect(&raw_full[st], n * (uint32_t)run * (2 * row_bytes + 8));
-                __syncwarp();
-                if (on) {
-                    const int pg = page_of(p, b, key, &g_tc_error);
-                    const size_t row = (((size_t)pg * p.kv_heads + kvh) << p.bt.page_log2) +
-                                       (key & ((1 << p.bt.page_log2) - 1));
-                    const uint32_t bytes = run * row_bytes;
-                    bulk_load(raw + lane * bytes, p.kq + row * row_bytes, bytes, &raw_full[st]);
-                    bulk_load(raw + S::kRawTile + lane * bytes, p.vq + row * row_bytes, bytes, &raw_full[st]);
-                    uint8_t *sc = raw + 2 * S::kRawTile + lane * run * 4;
-                    bulk_load(sc, p.ks + row, run * 4, &raw_full[st]);
-                    bulk_load(sc + kBN * 4, p.vs + row, run * 4, &raw_full[st]);
-                }
+        } else if (!ALT && warp == kLoadWarp) {
+            // ---------------- raw pages: keys LEAD steps ahead of their values, as the scores are of the products ----------------
+            // (a loader, since two row tiles leave the converters no time: 16 trees of 64 tokens 169 us, loaded by them 178)
+            constexpr int LEAD = 2;
+            auto refill = [&](int kv, int j, int found) {
+                const int before = j - kRaw;  // the step that had the stage before
+                if (before >= 0 && !bar_wait(&raw_empty[kv * kTurns + before % kTurns], (before / kTurns) & 1)) return false;
+                load(kv, j, found);
+                return true;
+            };
+            // this lane's entries of the page table, read two steps ahead of their use; found[k]: of the step k before j
+            int next = entry(0), after = entry(1), found[LEAD + 1];
+            for (int j = 0; j < mine + LEAD; j++) {
+#pragma unroll
+                for (int k = LEAD; k; k--) found[k] = found[k - 1];
+                found[0] = next;
+                next = after;
+                after = entry(j + 2);
+                if (j < mine && !refill(0, j, found[0])) break;
+                if (j >= LEAD && !refill(1, j - LEAD, found[LEAD])) break;
             }
             // copies in flight land before the CTA can end
-            for (int j = mine > kRaw ? mine - kRaw : 0; j < mine; j++) bar_wait(&raw_full[j % kTurns], (j / kTurns) & 1);
+            for (int j = mine > kRaw ? mine - kRaw : 0; j < mine; j++)
+                for (int kv = 0; kv < 2; kv++) bar_wait(&raw_full[kv * kTurns + j % kTurns], (j / kTurns) & 1);
         }
     } else {
         // ---------------- softmax: two threads a row ----------------

@@ -640,9 +640,13 @@ static cudaError_t launch_rows(const AttnParams &p, int max_len, cudaStream_t st
 
 template <typename T, int BITS>
 static cudaError_t launch_size(const AttnParams &p, int max_len, cudaStream_t stream) {
-    // 24 rows: with 8 kv heads of 128 in 8 bits, 24 and 32 rows take 88 and 106 us here against 92 and 92 there for 64
-    // sequences of up to 2,000 keys, 46 and 54 against 50 and 50 for 16 of up to 4,000
-    if ((long long)p.max_new * p.group > 24) return launch_tc(p, rows::Type<T>::kId, BITS, max_len, stream);
+    // Above 24 rows the tensor-core kernel; above 16 too for heads behind 64 unless P goes in two parts for fp16 callers or a
+    // few sequences leave SMs without a second CTA anyway. 24 rows, 8 kv heads, int8, here | there, 64 sequences of 2,000
+    // keys and 16 of 4,000: heads of 128, bf16 89 | 86 and 49 | 43 us, fp32 108 | 100 and 68 | 50, fp16 (int4) 90 | 101 and
+    // 56 | 51; heads of 64, bf16 64 | 82 and 33 | 41. One sequence of 131,001: 95 | 100.
+    const long long rows = (long long)p.max_new * p.group;
+    const bool many = (long long)p.bt.batch * p.kv_heads > 18 && p.head > 64 && rows::Type<T>::kId != rows::kF16;
+    if (rows > (many ? 16 : 24)) return launch_tc(p, rows::Type<T>::kId, BITS, max_len, stream);
     return p.head <= 64 ? launch_rows<T, BITS, 64>(p, max_len, stream) : launch_rows<T, BITS, 128>(p, max_len, stream);
 }
 

@@ -1,6 +1,6 @@
 // mvb_tree_attention for many query rows (new tokens x the query heads of one kv head): trees of dozens of tokens, prompt
 // chunks. Same arithmetic as tree_attention.cu (exact integers in fp16, one scale a row, fp32 statistics), on the
-// 5th-generation tensor cores, since each cached byte now meets 25 to 256 rows.
+// 5th-generation tensor cores, since each cached byte now meets 17 to 256 rows.
 //
 // One CTA: up to MT = 2 tiles of 128 query rows against 64 keys a step. The cache is converted once for all rows: raw
 // pages -> (bulk copies) -> raw bytes -> (converter warps) -> fp16 tiles in the 128-byte swizzled layout, two of each. Keys
@@ -11,7 +11,8 @@
 // Warp roles (768 threads):
 //   warp 0          one thread issues the MMAs: PV0 QK0'' PV1 QK1'' a step. (The oldest warp, which the scheduler prefers:
 //                   as warp 12 it waited for issue slots behind the softmax.)
-//   warp 1          bulk copies of the raw pages, as many stages ahead as fit (3 to 6).
+//   warp 1          with two row tiles, bulk copies of the raw pages, as many stages ahead as fit (3 to 6); with one the
+//                   converters' own, which then have the time for it.
 //   warps 2, 4, 6 and 3, 5, 7  converters of K, of V, a step's tile a warp: bytes -> fp16; the scales.
 //   warps 8-15, 16-23  softmax of row tile 0, 1: two threads a row, 32 of the step's keys each, so that every scheduler has
 //                   four such warps to hide one another's latencies (with one thread a row, 64 keys each, a step took 2,350

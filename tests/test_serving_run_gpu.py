@@ -38,6 +38,17 @@ def test_many_rows(torch, mvb, dtype, bits, tree, lens, new, heads, kv_heads, he
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("drafts,lens,heads,kv_heads,head,page", [
+    (10, [0, 3, 700, 64, 65, 130, 1, 200, 63, 31], 4, 2, 128, 32), (12, list(range(0, 760, 40)), 2, 1, 96, 16),
+    (60, [3000, 2000], 4, 2, 128, 64), (130, [2500, 40], 2, 1, 128, 16)])
+def test_tiles_refilled(torch, mvb, dtype, bits, drafts, lens, heads, kv_heads, head, page):
+    """17 to 24 rows of many sequences, and enough steps for every ring of the tensor-core kernel to come round."""
+    c = Case(torch, mvb, lens, [drafts] * len(lens), kv_heads, head, bits, page, seed=drafts, pad_rows=1)
+    check_attention(torch, mvb, c, heads, dtype, max_new=drafts)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
 @pytest.mark.parametrize("drafts", [1, 4, 7, 40, 150])
 @pytest.mark.parametrize("max_len", [None, 17000, 300])
 def test_long_context(torch, mvb, dtype, drafts, max_len):

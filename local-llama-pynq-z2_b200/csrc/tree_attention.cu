@@ -620,7 +620,8 @@ template <typename T, int BITS, int HDP, int NT>
 static cudaError_t launch(const AttnParams &p, int max_len, cudaStream_t stream) {
     using S = Slice<HDP, BITS>;
     // Two CTAs of 8 warps an SM; or, where the jobs are so few that clusters of 16 leave one CTA an SM, and the sequences
-    // long enough for it, one of 16 warps (16 jobs of 131,001 int8 keys: 102 us so, 90 with 8 warps). Three column tiles need more registers: one CTA of 12 warps.
+    // long enough for it, one of 16 warps (16 jobs of 131,001 int8 keys: 102 us so, 90 with 8 warps).
+    // Three column tiles need more registers: one CTA of 12 warps.
     const long long base = ((long long)p.max_new * p.group + 8 * NT - 1) / (8 * NT) * p.kv_heads * p.bt.batch;
     if constexpr (NT <= 2) {
         if (base <= 9 && max_len >= 2 * 16 * 16 * S::kKeys) return launch_warps<T, BITS, HDP, NT, 16>(p, max_len, stream);

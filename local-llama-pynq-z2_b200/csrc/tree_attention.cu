@@ -7,9 +7,10 @@
 // with k and v the cached integers, which fp16 holds exactly: the products take them as they are, the keys' scales
 // multiply S and the values' scales multiply P. q is put in fp16 after a power of two of its row's largest element was
 // taken out (2 ^ e; a bf16 or fp16 q keeps every bit that is above 2^-33 of the row's largest); an fp32 q goes in two
-// parts, high and low (22 bits). P is rounded to fp16 once for bf16 callers (2^-12, an eighth of the output's own half
-// step); for fp16 and fp32 callers it goes in two parts too (22 bits), since one rounding would be as large as an fp16
-// output's own. max, sum and O are fp32.
+// parts, high and low (22 bits). P vs goes to fp16 in a unit of its row's own (`moved`), rounded once for bf16 callers (2^-11, an
+// eighth of the output's own half step); for fp16 and fp32 callers in two parts (22 bits), since one rounding would be as
+// large as an fp16 output's own. What is far below the row's largest is held to a fixed step: 2^-27 of that at most.
+// max, sum and O are fp32.
 //
 // This kernel: 8 * NT query rows (new tokens x the query heads of one kv head) at a time; a handful of rows does little
 // arithmetic per cached byte, so the work is to stream the cache with few instructions a byte. One warp owns slices of 16
@@ -43,8 +44,6 @@ namespace cg = cooperative_groups;
 static __device__ int g_attn_error;
 
 constexpr int kStages = 3;
-constexpr float kPScale = 4.0f;     // P' = P * vs * kPScale / W stays below 2^14 in fp16
-constexpr float kLazy = 12.0f;      // the running maximum moves only when it is 2^12 behind
 
 template <int HDP, int BITS>
 struct Slice {
@@ -216,7 +215,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 && NT <= 2 ? 2 : 1) t
     }
 
     // this lane's rows of column tile nt: 8 nt + 2c, + 1
-    float O[NT][KS][4], m[NT][2], l[NT][2], rf[NT][2];
+    float O[NT][KS][4], unit[NT][2], l[NT][2], rf[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -225,12 +224,11 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 && NT <= 2 ? 2 : 1) t
             for (int e = 0; e < 4; e++) O[nt][j][e] = 0.0f;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            m[nt][h] = -INFINITY;
+            unit[nt][h] = INFINITY;
             l[nt][h] = 0.0f;
             rf[nt][h] = row_factor[nt * 8 + 2 * c + h];
         }
     }
-    float W = pow2(-100);  // at or above every finite |vs| so far, a power of two
 
     // where this lane's fragments lie in a stage (+ 16 * kRow * sub; the rows 8 further lie 8 * kRow further)
     const int k_at = place<S::kRow>(r, BITS == 8 ? 16 * c : 8 * c);
@@ -328,15 +326,15 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 && NT <= 2 ? 2 : 1) t
                             if (!allowed(p, s, (R0 + nt * 8 + 2 * c + h) / p.group, key)) sc[nt][sub][2 * n + h] = -INFINITY;
                 }
         }
-        // The running maxima (log2 units) and W move only when some row falls kLazy behind, or a value's scale passes
-        // W: every lane looks at its own scores, one vote a slice; the maxima are exchanged only then.
+        // The rows' units move only when a row needs it: every lane looks at its own scores and scales, one vote a slice; the
+        // maxima are exchanged only then.
         float mx[NT][2], mv = 0.0f;
 #pragma unroll
         for (int sub = 0; sub < S::kSub; sub++)
 #pragma unroll
-            for (int n = 0; n < 2; n++)  // (an infinite scale makes the rows that see it infinite; it must not set W)
+            for (int n = 0; n < 2; n++)  // (an infinite scale makes the rows that see it infinite, and no unit)
                 if (fabsf(vv[sub][n]) < INFINITY) mv = fmaxf(mv, fabsf(vv[sub][n]));
-        move = mv > W;
+        const float limit = unit_limit(mv);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -345,30 +343,27 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 && NT <= 2 ? 2 : 1) t
 #pragma unroll
                 for (int sub = 1; sub < S::kSub; sub++) x = fmaxf(x, fmaxf(sc[nt][sub][h], sc[nt][sub][2 + h]));
                 mx[nt][h] = x * rf[nt][h];
-                move |= mx[nt][h] > m[nt][h] + kLazy;  // -inf + kLazy: any finite score moves the first maximum
+                move |= mx[nt][h] + unit[nt][h] > limit;
             }
         if (__any_sync(0xffffffffu, move)) {
-            float wf = 1.0f;
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) mv = fmaxf(mv, __shfl_xor_sync(0xffffffffu, mv, o));
-            if (mv > W) {
-                const float w2 = pow2(min(exponent_of(mv) - 127 + 1, 127));
-                wf = W / w2;
-                W = w2;
-            }
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    float x = mx[nt][h];
+                    float t = mx[nt][h], w = 0.0f;
 #pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+                    for (int o = 4; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+#pragma unroll
+                    for (int sub = 0; sub < S::kSub; sub++)
+#pragma unroll
+                        for (int n = 0; n < 2; n++)
+                            w = fmaxf(w, product_of(sc[nt][sub][2 * n + h], rf[nt][h], t, vv[sub][n]));
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, o));
                     // only the rows that are behind move, so that a row's result does not depend on its neighbours
-                    if (!(x > m[nt][h] + kLazy)) x = m[nt][h];
-                    const float a = m[nt][h] == -INFINITY ? 0.0f : exp2_fast(m[nt][h] - x);
-                    m[nt][h] = x;
-                    l[nt][h] *= a;
-                    const float f = a * wf;
+                    const float to = moved(unit[nt][h], t, w), f = unit_factor(unit[nt][h], to);
+                    unit[nt][h] = to;
+                    l[nt][h] *= f;
 #pragma unroll
                     for (int j = 0; j < KS; j++) {
                         O[nt][j][h] *= f;
@@ -376,20 +371,17 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 && NT <= 2 ? 2 : 1) t
                     }
                 }
         }
-        const float vf = kPScale / W;
 #pragma unroll
         for (int sub = 0; sub < S::kSub; sub++) {
             uint32_t P[PP][NT][2];  // [part][column tile][keys 0 .. 7, 8 .. 15]: the operand of the second product
-            const float w0 = vv[sub][0] * vf, w1 = vv[sub][1] * vf;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 float pv[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const float base = m[nt][e & 1] == -INFINITY ? 0.0f : m[nt][e & 1];
-                    const float x = exp2_fast(__fmaf_rn(sc[nt][sub][e], rf[nt][e & 1], -base));
+                    const float x = exp2_fast(__fmaf_rn(sc[nt][sub][e], rf[nt][e & 1], or_zero(unit[nt][e & 1])));
                     l[nt][e & 1] += x;
-                    pv[e] = x * (e < 2 ? w0 : w1);
+                    pv[e] = x * vv[sub][e >> 1];
                 }
                 if (tail) {  // a masked key's value scale may be anything: its weight is zero, not zero times that
 #pragma unroll
@@ -467,9 +459,8 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 && NT <= 2 ? 2 : 1) t
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
 
-    // join the warps: O in its own units to shared memory, then (max, sum) of each row
+    // join the warps: O in the unit of the sums to shared memory, then (max, sum) of each row
     float *po = reinterpret_cast<float *>(pipe);  // [kWarps][ROWS][HDP]
-    const float back = W / kPScale;
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -478,9 +469,11 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 && NT <= 2 ? 2 : 1) t
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             const int row = nt * 8 + 2 * c + h;
+            const float2 ml = normal_sum(unit[nt][h], sum);
+            const float back = sum == 0.0f ? 0.0f : pow2_of((float)(127 - exponent_of(sum)));
             if (r == 0) {
-                warp_m[warp][row] = m[nt][h];
-                warp_l[warp][row] = sum;
+                warp_m[warp][row] = ml.x;
+                warp_l[warp][row] = ml.y;
             }
             float *d = po + ((size_t)warp * ROWS + row) * HDP + RUN * r;
 #pragma unroll

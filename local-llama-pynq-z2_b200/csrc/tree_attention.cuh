@@ -83,8 +83,51 @@ __device__ __forceinline__ float exp2_fast(float x) {  // 2 ulp; exp2(-inf) = 0
 // 2^k as fp32 for k in [-126, 127].
 __device__ __forceinline__ float pow2(int k) { return __int_as_float((k + 127) << 23); }
 
+// The same of an integer-valued float of that range.
+__device__ __forceinline__ float pow2_of(float k) {
+    return __int_as_float(__float_as_int(__fadd_rn(k, 12582912.0f + 127.0f)) << 23);
+}
+
 // Biased exponent of |x| (0 for zero and subnormals, 255 for infinities and NaN).
 __device__ __forceinline__ int exponent_of(float x) { return (__float_as_int(x) >> 23) & 255; }
+
+// The unit of a row's sums: l = sum of 2^(s + b) over its scores s (log2), O = sum of P' v with P' = 2^(s + b) vs in fp16. b
+// keeps every P' below 2^kTop (and every weight below 2^kSumTop); when it has to fall, the row's largest P' so far comes near
+// 2^(kTop - kLazy). fp16's steps below 2^-14 are 2^-24, so no weight is off by more than 2^(kLazy - 39) of the row's largest
+// weight times value scale. Only weights and scales that the row sees count: a key that the mask hides from it leaves b
+// where it is, and so does one that stands far above the rest while its value is near zero. b is a whole number, so that O and
+// l change by exact factors; infinite while the row has seen no score.
+constexpr float kLazy = 12.0f;
+constexpr float kTop = 15.0f, kSumTop = 100.0f;
+// What the largest score plus b may reach beside value scales up to vmax before `moved` has to be asked.
+__device__ __forceinline__ float unit_limit(float vmax) {
+    return fminf(kSumTop, (kTop - 0.01f) - (float)(exponent_of(vmax) - 126));  // vmax is below 2^(exponent - 126)
+}
+// 2^(s - t) vs for the row's largest score t; nothing where the scale is infinite or the score hidden.
+__device__ __forceinline__ float product_of(float s, float rf, float t, float vs) {
+    const float w = __fmul_rn(exp2_fast(__fmaf_rn(s, rf, -t)), fabsf(vs));
+    return w < INFINITY ? w : 0.0f;
+}
+// b where the row meets scores up to t and products up to w 2^t.
+__device__ __forceinline__ float moved(float b, float t, float w) {
+    const float top = t + __log2f(w);
+    float to = b;
+    if (t + b > kSumTop) to = floorf(__fsub_rd(kSumTop - 4.0f, t));
+    if (top + b > kTop - 0.005f) to = fminf(to, floorf(__fsub_rd(kTop - kLazy, top)));
+    // (value scales above 2^100: rather a weight below 2^-122 lost than all of them)
+    return to < b ? fminf(b, fmaxf(to, ceilf(-122.0f - t))) : b;
+}
+// The factor of l and O; what has seen nothing is zero.
+__device__ __forceinline__ float unit_factor(float b, float to) {
+    const float k = to - b;
+    return b == INFINITY ? 1.0f : k >= -126.0f ? pow2_of(k) : 0.0f;
+}
+__device__ __forceinline__ float or_zero(float b) { return b == INFINITY ? 0.0f : b; }
+// A sum l in b's unit as (max, sum in its unit): 2^max * sum with sum in [1, 2).
+__device__ __forceinline__ float2 normal_sum(float b, float l) {
+    const float k = (float)(exponent_of(l) - 127);
+    return l == 0.0f ? make_float2(-INFINITY, 0.0f) : make_float2(k - b, l * pow2_of(-k));
+}
 
 // Bytes 0 and 2 of a word (int8) as an exact half2: the byte with its sign bit flipped in the low mantissa of 1024 is
 // 1024 + (v + 128). One logic operation takes the bytes out, flips the signs and puts the exponents in.

@@ -17,10 +17,11 @@
 //   warps 8-15, 16-23  softmax of row tile 0, 1: two threads a row, 32 of the step's keys each, so that every scheduler has
 //                   four such warps to hide one another's latencies (with one thread a row, 64 keys each, a step took 2,350
 //                   clocks). S from tensor memory, keys' scales, maximum, exponentials, values' scales, P in fp16 back to
-//                   tensor memory. The running maximum and the values' unit W move only when a row falls 2^12 behind (then O
-//                   is scaled in tensor memory, after the product before has ended): a row's two threads vote on that with
-//                   the barrier that also keeps either's P off the other's unread S, and exchange their maxima only then.
-//                   The unit's factor is folded into the exponent, so it multiplies P and the row's sum alike.
+//                   tensor memory. A row's unit moves only when it has to (then O is scaled in tensor memory, after the product
+//                   before has ended): a row's two threads vote on that with the barrier that also keeps either's P off
+//                   the other's unread S, and exchange their maxima only then. The vote asks the step's largest score and
+//                   its largest value scale; only where both together might pass is the product looked at key by key. The
+//                   unit is folded into the exponent, so it multiplies P and the row's sum alike.
 // What bounds it: for two row tiles of head 128 and 64 keys the exponentials take 1,024 clocks (16 a clock), the MMAs
 // 1,280 (QK at N = 64 waits for shared memory: 48 clocks a product against 32), and shared memory carries 224 KB, 1,800
 // clocks (QK's operands 96, PV's 32, the conversion 64, the softmax's scales 32); the step takes about 2,300. 16 trees of 64
@@ -57,8 +58,6 @@ constexpr int kBN = 64;              // keys a step
 // warps of a kind wait on in turn are as many as make the same warp wait on each (multiples of 3).
 constexpr int kTurns = 6;            // barriers of raw stages filled and read, and of tiles set free
 constexpr int kScales = 8;           // steps whose scales are kept
-constexpr float kPUnit = 2.0f;       // log2 of P' / (P * vs / W): P' stays below 2^15 in fp16
-constexpr float kBehind = 12.0f;     // (at 6 one of a row tile's warps moved nearly every step, 2,000 clocks each time)
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -275,7 +274,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
              *p_ready = s_full + 4 /* [m][slot] */, *pv_done = p_ready + 4 /* [m] */, *sc_ready = pv_done + 2,
              *q_ready = sc_ready + kScales, *o_done = q_ready + 1;
     uint32_t *tmem_at = reinterpret_cast<uint32_t *>(o_done + 1);
-    float *vmax = reinterpret_cast<float *>(bar + 62);  // [kScales]
+    float *limits = reinterpret_cast<float *>(bar + 62);  // [kScales] of the rows' units beside each step's value scales
     float *row_factor = reinterpret_cast<float *>(smem + S::kRow);
     float *cta_m = reinterpret_cast<float *>(smem + S::kMl), *cta_l = cta_m + 256;
 
@@ -390,11 +389,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
                         const float x = live ? rsc[kBN + key] : 0.0f;
                         sc[key] = live ? rsc[key] * p.scale_log2 : 0.0f;
                         sc[kBN + key] = x;
-                        if (fabsf(x) < INFINITY) mv = fmaxf(mv, fabsf(x));  // an infinite scale must not set the unit
+                        if (fabsf(x) < INFINITY) mv = fmaxf(mv, fabsf(x));  // an infinite scale limits no unit
                     }
 #pragma unroll
                     for (int o = 16; o; o >>= 1) mv = fmaxf(mv, __shfl_xor_sync(0xffffffffu, mv, o));
-                    if (lane == 0) vmax[ss] = mv;
+                    if (lane == 0) limits[ss] = unit_limit(mv);
                     __syncwarp();
                     if (lane == 0) bar_arrive(&sc_ready[ss]);
                 }
@@ -566,7 +565,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
         const uint32_t lane_at = tmem + ((uint32_t)(row & 96) << 16), o_at = lane_at + 256 + m * 128;
         const int R = R0 + (ALT ? 0 : m * 128) + row, draft = R / p.group;
         const float rf = row_factor[ALT ? row : m * 128 + row];
-        float mx = -INFINITY, l = 0.0f, lw = -80.0f;  // running maximum and sum (in the unit's factor); lw = log2 of W
+        float unit = INFINITY, l = 0.0f;
         // One step; TAIL: some of its keys are new tokens, or none (a variant of its own: the mask's branches cost the
         // others more than their arithmetic).
         auto step = [&](int i, auto is_tail) -> bool {
@@ -578,7 +577,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
             const float *kk = reinterpret_cast<const float *>(smem + S::kScale) + ss * 2 * kBN + 32 * half, *vv = kk + kBN;
             float u[32];
             tmem_load32(s_at + 32 * half, u);
-            const float vm = vmax[ss];
+            const float limit = limits[ss];
             const uint32_t bits = TAIL ? mask32(p, s, draft, key0 + 32 * half - s.ctx) : ~0u;
             wait_load();
             float top[2] = {-INFINITY, -INFINITY};
@@ -595,34 +594,33 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
                 top[0] = max3(top[0], u[i], u[i + 1]);
                 top[1] = max3(top[1], u[i + 2], u[i + 3]);
             }
-            float now = fmaxf(mx, fmaxf(top[0], top[1]) * rf);
-            const float lv = (float)(min(max(exponent_of(vm), 1) - 127 + 1, 127));  // W above this step's scales
-            const bool grow = vm > 0.0f && lv > lw;
+            float now = fmaxf(top[0], top[1]) * rf;
             uint32_t vote;  // of both warps; after it both have read their S
             asm volatile(
                 "{\n\t.reg .pred a, b;\n\tsetp.ne.u32 a, %1, 0;\n\t"
                 "barrier.cta.red.or.pred b, %2, 64, a;\n\tselp.u32 %0, 1, 0, b;\n\t}"
                 : "=r"(vote)
-                : "r"((uint32_t)(grow || now > mx + kBehind || !fine)), "r"(pair)
+                : "r"((uint32_t)(now + unit > limit || !fine)), "r"(pair)
                 : "memory");
             if (vote) {
-                // a wait that ran out on either side ends both (NaN stands for it)
-                *mine_x = fine ? now : __int_as_float(0x7FC00000);
-                asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
-                const float theirs = *other_x;
-                asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
-                if (__any_sync(0xffffffffu, !fine || theirs != theirs)) return false;
-                now = fmaxf(now, theirs);
-                const bool behind = now > mx + kBehind;
-                const float lw2 = grow ? lv : lw;
-                // O and the sum: exp2(old max - new max), and the old unit in the new one. Only the rows that are behind
-                // move, so that a row's result does not depend on its neighbours.
-                const float mx2 = behind ? now : mx;
-                const float f = mx == -INFINITY ? 0.0f : exp2_fast((mx - mx2) + (lw - lw2));
-                mx = mx2;
-                lw = lw2;
+                auto larger = [&](float x) {  // of both threads of the row
+                    *mine_x = x;
+                    asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
+                    const float theirs = *other_x;
+                    asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
+                    return x != x || theirs != theirs ? __int_as_float(0x7FC00000) : fmaxf(x, theirs);
+                };
+                // a wait that ran out on either side ends both (NaN stands for it; scores that are all NaN count as none)
+                now = larger(!fine ? __int_as_float(0x7FC00000) : now == now ? now : -INFINITY);
+                if (__any_sync(0xffffffffu, now != now)) return false;
+                float w = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 32; i++) w = fmaxf(w, product_of(u[i], rf, now, vv[i]));
+                // Only the rows that are behind move, so that a row's result does not depend on its neighbours.
+                const float to = moved(unit, now, larger(w)), f = unit_factor(unit, to);
+                unit = to;
                 l *= f;
-                if (i > 0) {
+                if (i > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
                     // (the product of two steps ago has ended: this step's scores were issued after it; where this wait
                     // runs out, the results are void and the error is noted)
                     bar_wait(&pv_done[m], (i - 1) & 1);
@@ -638,8 +636,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
                     }
                 }
             }
-            const float base = (kPUnit - lw) - (mx == -INFINITY ? 0.0f : mx);
-            const uint64_t rf2 = pair2(rf, rf), base2 = pair2(base, base);
+            const uint64_t rf2 = pair2(rf, rf), base2 = pair2(or_zero(unit), or_zero(unit));
             uint64_t sum[2] = {0, 0};
             uint32_t hi[16], low[PP == 2 ? 16 : 1];
 #pragma unroll
@@ -702,14 +699,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
         *mine_x = l;
         asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
         l = half ? *other_x + l : l + *other_x;
-        // O in units of W / 2^kPUnit, and the sum in the same: they cancel
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // both in the row's unit
         const int c0 = half * (HDP / 32);  // this thread's half of O, 16 columns at a time
         if (!ALT && p.splits * p.supers == 1) {
             const int tok = s.row0 + R / p.group, head = kvh * p.group + R % p.group;
             if (R < nrows && p.lse && half == 0)
                 p.lse[(size_t)tok * p.heads + head] =
-                    l == 0.0f ? -INFINITY : (mx - (kPUnit - lw) + log2f(l)) * 0.693147180559945309f;
+                    l == 0.0f ? -INFINITY : (log2f(l) - unit) * 0.693147180559945309f;
 #pragma unroll 1
             for (int c = c0; c < c0 + HDP / 32; c++) {
                 float o[16];
@@ -728,8 +724,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
         } else {
             // this group's part: O divided by its own sum, the row's (max, sum) beside it
             if (half == 0) {
-                cta_m[m * 128 + row] = mx;
-                cta_l[m * 128 + row] = l == 0.0f ? 0.0f : l * exp2f(lw - kPUnit);  // the sum in its own units
+                const float2 ml = normal_sum(unit, l);
+                cta_m[m * 128 + row] = ml.x;
+                cta_l[m * 128 + row] = ml.y;
             }
             float *po = reinterpret_cast<float *>(smem) + (size_t)(m * 128 + row) * HDP;
 #pragma unroll 1

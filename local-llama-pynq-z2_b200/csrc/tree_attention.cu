@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 && NT <= 2 ? 2 : 1) t
         // the scales of this lane's keys; S in units of the row's factor; the mask where some key is new or none
         float vv[S::kSub][2];
         const bool tail = key0 + S::kKeys > s.ctx;
-        bool move = false;
+        uint32_t move = 0;  // one bit for each of this lane's rows
 #pragma unroll
         for (int sub = 0; sub < S::kSub; sub++)
 #pragma unroll
@@ -343,13 +343,15 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 && NT <= 2 ? 2 : 1) t
 #pragma unroll
                 for (int sub = 1; sub < S::kSub; sub++) x = fmaxf(x, fmaxf(sc[nt][sub][h], sc[nt][sub][2 + h]));
                 mx[nt][h] = x * rf[nt][h];
-                move |= mx[nt][h] + unit[nt][h] > limit;
+                move |= (uint32_t)(mx[nt][h] + unit[nt][h] > limit) << (2 * nt + h);
             }
         if (__any_sync(0xffffffffu, move)) {
+            move = __reduce_or_sync(0xffffffffu, move);
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
+                    if (!((move >> (2 * nt + h)) & 1)) continue;
                     float t = mx[nt][h], w = 0.0f;
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
@@ -361,7 +363,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 && NT <= 2 ? 2 : 1) t
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, o));
                     // only the rows that are behind move, so that a row's result does not depend on its neighbours
-                    const float to = moved(unit[nt][h], t, w), f = unit_factor(unit[nt][h], to);
+                    const float to = moved<PP>(unit[nt][h], t, w), f = unit_factor(unit[nt][h], to);
                     unit[nt][h] = to;
                     l[nt][h] *= f;
 #pragma unroll

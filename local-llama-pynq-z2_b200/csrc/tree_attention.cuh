@@ -93,27 +93,26 @@ __device__ __forceinline__ int exponent_of(float x) { return (__float_as_int(x) 
 
 // The unit of a row's sums: l = sum of 2^(s + b) over its scores s (log2), O = sum of P' v with P' = 2^(s + b) vs in fp16. b
 // keeps every P' below 2^kTop (and every weight below 2^kSumTop); when it has to fall, the row's largest P' so far comes near
-// 2^(kTop - kLazy). fp16's steps below 2^-14 are 2^-24, so no weight is off by more than 2^(kLazy - 39) of the row's largest
+// 2^(kTop - lazy). fp16's steps below 2^-14 are 2^-24, so no weight is off by more than 2^(lazy - 40) of the row's largest
 // weight times value scale. Only weights and scales that the row sees count: a key that the mask hides from it leaves b
 // where it is, and so does one that stands far above the rest while its value is near zero. b is a whole number, so that O and
 // l change by exact factors; infinite while the row has seen no score.
-constexpr float kLazy = 12.0f;
-constexpr float kTop = 15.0f, kSumTop = 100.0f;
+__host__ __device__ constexpr float lazy(int parts) { return parts == 2 ? 9.0f : 13.0f; }
+constexpr float kTop = 15.99f, kSumTop = 100.0f;
 // What the largest score plus b may reach beside value scales up to vmax before `moved` has to be asked.
-__device__ __forceinline__ float unit_limit(float vmax) {
-    return fminf(kSumTop, (kTop - 0.01f) - (float)(exponent_of(vmax) - 126));  // vmax is below 2^(exponent - 126)
-}
+__device__ __forceinline__ float unit_limit(float vmax) { return fminf(kSumTop, (kTop - 0.005f) - __log2f(vmax)); }
 // 2^(s - t) vs for the row's largest score t; nothing where the scale is infinite or the score hidden.
 __device__ __forceinline__ float product_of(float s, float rf, float t, float vs) {
     const float w = __fmul_rn(exp2_fast(__fmaf_rn(s, rf, -t)), fabsf(vs));
     return w < INFINITY ? w : 0.0f;
 }
 // b where the row meets scores up to t and products up to w 2^t.
+template <int PP>  // parts of P'
 __device__ __forceinline__ float moved(float b, float t, float w) {
     const float top = t + __log2f(w);
     float to = b;
     if (t + b > kSumTop) to = floorf(__fsub_rd(kSumTop - 4.0f, t));
-    if (top + b > kTop - 0.005f) to = fminf(to, floorf(__fsub_rd(kTop - kLazy, top)));
+    if (top + b > kTop) to = fminf(to, floorf(__fsub_rd(16.0f - lazy(PP), top)));
     // (value scales above 2^100: rather a weight below 2^-122 lost than all of them)
     return to < b ? fminf(b, fmaxf(to, ceilf(-122.0f - t))) : b;
 }

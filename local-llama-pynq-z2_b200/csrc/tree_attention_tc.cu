@@ -617,7 +617,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
 #pragma unroll
                 for (int i = 0; i < 32; i++) w = fmaxf(w, product_of(u[i], rf, now, vv[i]));
                 // Only the rows that are behind move, so that a row's result does not depend on its neighbours.
-                const float to = moved(unit, now, larger(w)), f = unit_factor(unit, to);
+                const float to = moved<PP>(unit, now, larger(w)), f = unit_factor(unit, to);
                 unit = to;
                 l *= f;
                 if (i > 0 && __any_sync(0xffffffffu, f != 1.0f)) {

@@ -198,6 +198,24 @@ def test_late_dominant_key(torch, mvb, dtype, heads, tokens, at):
     check(torch, mvb, c, q, max_len=16000 + tokens)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("heads,head,tokens", [(4, 64, 1), (4, 128, 3), (4, 128, 6), (4, 64, 12), (4, 128, 20)])
+@pytest.mark.parametrize("nats", [12.0, 16.0, 18.0])
+def test_dominant_key_above_equal_ones(torch, mvb, dtype, heads, head, tokens, nats):
+    """The other keys weigh alike, so that what a weight is off by does not average out, in one CTA; the dominant value is zero
+    in half of its elements, where the others are all there is."""
+    c = Case(torch, mvb, [4000], [tokens], 1, head, 8, 64, seed=head)
+    q = dominant(torch, c, tokens, heads, dtype, nats, 1.0)
+    pg = int(c.pages[0, 0])
+    top = c.cache.kq[pg, :, 0].clone()
+    c.cache.kq.zero_()
+    c.cache.kq[pg, :, 0] = top
+    c.cache.vq.copy_(c.cache.vq.abs().clamp(min=20))
+    c.cache.vq[pg, :, 0, ::2] = 0
+    c.cache.vs.copy_(torch.where(c.cache.vs.isnan(), c.cache.vs, torch.full_like(c.cache.vs, 0.5)))
+    check(torch, mvb, c, q, together=4000, max_len=16)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("heads,head,tokens", [(4, 64, 1), (4, 128, 5), (4, 128, 12), (3, 64, 50), (3, 128, 100)])
 def test_value_outliers(torch, mvb, dtype, heads, head, tokens):

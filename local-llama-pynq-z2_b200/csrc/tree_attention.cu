@@ -106,7 +106,9 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 && NT <= 2 ? 2 : 1) t
     constexpr int RUN = HDP / 8;                 // a lane's elements of a value row: RUN * r ..
     constexpr int QP = Parts<T>::kQ, PP = Parts<T>::kP;
     constexpr int ROWS = 8 * NT;
-    constexpr bool QREG = NT * QP * KS <= (NT == 1 ? 16 : 8);  // q's fragments in registers, else read again for every slice
+    constexpr bool QREG = NT * QP * KS <= (NT == 1 && !(QP == 2 && kWarps == 16) ? 16 : 8);  // q's fragments in registers, else
+    // read again for every slice (16 warps, fp32: 32 registers of them spill others; one sequence of 131,001 keys, 4 rows,
+    // 82 us so, 73 with q read again)
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float row_factor[ROWS], warp_m[kWarps][ROWS], warp_l[kWarps][ROWS], cta_m[ROWS], cta_l[ROWS];
     __shared__ float all_m[16][ROWS], all_l[16][ROWS];

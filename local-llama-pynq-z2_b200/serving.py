@@ -181,7 +181,7 @@ def rope_frequencies(rot, theta, scaling=None, factor=1.0, original=None, fast=3
     _need(scaling == "yarn", f"scaling={scaling!r}: None, 'linear', 'ntk' or 'yarn' is needed")
     _need(original is not None and original > 0 and theta > 1, "yarn needs original positions and a base above 1")
     turn = lambda n: half * math.log(original / (n * 2 * math.pi)) / math.log(theta)  # noqa: E731
-    lo, hi = max(math.floor(turn(fast)), 0), min(math.ceil(turn(slow)), half - 1)
+    lo, hi = max(math.floor(turn(fast)), 0), min(math.ceil(turn(slow)), rot - 1)  # hi may lie behind the last pair
     keep = 1 - np.clip((np.arange(half) - lo) / max(hi - lo, 1e-3), 0, 1)
     return f / factor * (1 - keep) + f * keep, (0.1 * math.log(factor) + 1 if factor > 1 else 1.0)
 

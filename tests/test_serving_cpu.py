@@ -188,3 +188,21 @@ def test_tree_mask(mvb):
 def test_status_names_every_code(mvb):
     assert set(mvb.serving.STATUS) == {0, 1, 2, 3, 4, 5}
     assert mvb.lib().mvb_serve_status.restype is C.c_int
+
+
+def test_yarn_ramp_behind_the_last_pair(mvb):
+    """Where no pair turns fewer than `slow` times, the ramp ends behind the last pair, at the rotary size at most: no pair is
+    divided by the whole factor."""
+    f, _ = mvb.rope_frequencies(64, 1e4)
+    g, _ = mvb.rope_frequencies(64, 1e4, "yarn", factor=4.0, original=131072)
+    turns = 131072 * f / (2 * math.pi)
+    assert turns.min() > 2.7
+    lo = math.floor(32 * math.log(131072 / (32 * 2 * math.pi)) / math.log(1e4))
+    hi = math.ceil(32 * math.log(131072 / (2 * math.pi)) / math.log(1e4))
+    assert (lo, hi) == (22, 35)
+    keep = 1 - np.clip((np.arange(32) - lo) / (hi - lo), 0, 1)
+    assert keep[31] > 0.3 and np.allclose(g, f / 4 * (1 - keep) + f * keep, rtol=1e-15)
+    # never behind the rotary size
+    g, _ = mvb.rope_frequencies(8, 2.0, "yarn", factor=4.0, original=1 << 20)
+    f, _ = mvb.rope_frequencies(8, 2.0)
+    assert np.array_equal(g, f)

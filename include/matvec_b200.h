@@ -92,7 +92,8 @@ int mvb_qwen_forward(void *model, int token, int pos, float *logits);
 /* Log probabilities over the head's logits of the last step (mvb_qwen_forward, mvb_qwen_decode), computed where they lie
  * (mvb_logprobs) instead of downloading them: of the n <= 1024 given head rows, the entropy (nats), and the `top` <= 64 most
  * probable head rows, equal logits by the lowest row. Host arrays; any may be NULL whose count is 0 (entropy always). Head
- * rows are token ids with a full head or a runq handle. 0, or -1. */
+ * rows are token ids with a full head or a runq handle. 0, or -1; -1 too while there is no such step: after loading, after
+ * mvb_qwen_full_head changed the head, and after a prompt was fed (mvb_qwen_prefill) until the next step. */
 int mvb_qwen_logprobs(void *model, const int *rows, int n, float *logp, float *entropy, int top, int *top_rows,
                       float *top_logp);
 

@@ -409,7 +409,8 @@ class QwenDecoder:
 
     def logprobs(self, rows=(), top=0):
         """(log probabilities of the head rows `rows`, entropy in nats, the `top` most probable head rows, their log
-        probabilities) of the last forward() or decode() step, computed on the device from its logits."""
+        probabilities) of the last forward() or decode() step, computed on the device from its logits. Refused (MatvecError)
+        while there is none: at first, after full_head() changed the head, after prefill() until the next step."""
         import numpy as np
         r = self._ids(rows).reshape(-1)
         logp, ent = np.empty(r.size, np.float32), C.c_float()

@@ -157,6 +157,7 @@ struct Model {
     bool stamping = false;  // set while the stamped copy is captured
     // mvb_qwen_logprobs' ids and results (allocated on first use)
     int *lp = nullptr;
+    bool has_logits = false;  // `logits` are those of a step of the present head with no prompt fed after it
     struct Info { const char *kind; int layer; };
     std::vector<Info> info;  // one per kernel of the step, in launch order
     // batched prefill buffers (allocated on first use): up to `cap` tokens per batch
@@ -943,6 +944,7 @@ extern "C" int mvb_qwen_full_head(void *model, int on) {
         return -1;
     }
     if (wait_stream(*m, "mvb_qwen_full_head", timeout_s())) return -1;
+    if (m->head.w != (on ? m->emb : m->head_trim).w) m->has_logits = false;
     m->head = on ? m->emb : m->head_trim;
     m->head_ids = on ? nullptr : m->ids_trim;
     m->head_rows = on ? m->c.vocab_size : m->c.head_k;
@@ -979,6 +981,7 @@ extern "C" int mvb_qwen_launch(void *model, int count) {
             set_error("mvb_qwen_launch: %s", cudaGetErrorString(e));
             return -1;
         }
+        m->has_logits = true;
     }
     return 0;
 }
@@ -1013,6 +1016,10 @@ extern "C" int mvb_qwen_logprobs(void *model, const int *rows, int n, float *log
     if (n < 0 || n > kIds || top < 0 || top > kTop || top > m->head_rows || (n && (!rows || !logp)) ||
         (top && (!top_rows || !top_logp))) {
         set_error("mvb_qwen_logprobs: need 0 <= n <= %d, 0 <= top <= min(%d, head rows), and arrays for both", kIds, kTop);
+        return -1;
+    }
+    if (!m->has_logits) {
+        set_error("mvb_qwen_logprobs: no step has been taken since the model was loaded, its head changed or a prompt was fed");
         return -1;
     }
     for (int i = 0; i < n; i++)
@@ -1064,7 +1071,9 @@ static int check_prompt(Model *m, const int *prompt, int n, const char *who) {
 extern "C" int mvb_qwen_prefill_tokenwise(void *model, const int *prompt, int n) {
     Model *m = static_cast<Model *>(model);
     if (check_prompt(m, prompt, n, "mvb_qwen_prefill_tokenwise")) return -1;
-    if (set_state(*m, prompt[0], 0, n) || mvb_qwen_launch(m, n - 1)) return -1;
+    const bool fed = !set_state(*m, prompt[0], 0, n) && !mvb_qwen_launch(m, n - 1);
+    m->has_logits = false;
+    if (!fed) return -1;
     return wait_stream(*m, "mvb_qwen_prefill_tokenwise", timeout_s() + 0.01 * n);
 }
 
@@ -1076,6 +1085,7 @@ extern "C" int mvb_qwen_prefill(void *model, const int *prompt, int n) {
     Model *m = static_cast<Model *>(model);
     if (m && m->family == kRunq) return mvb_qwen_prefill_tokenwise(model, prompt, n);
     if (check_prompt(m, prompt, n, "mvb_qwen_prefill")) return -1;
+    m->has_logits = false;
     for (int p0 = 0; p0 < n - 1; p0 += kBatchCap)
         if (prefill_batch(*m, m->prompt + p0, p0, (n - 1 - p0) < kBatchCap ? n - 1 - p0 : kBatchCap)) return -1;
     if (set_state(*m, prompt[n - 1], n - 1, n)) return -1;
@@ -1165,6 +1175,7 @@ extern "C" int mvb_qwen_profile(void *model, float *ms, int cap) {
         set_error("mvb_qwen_profile: %s", cudaGetErrorString(e));
         return -1;
     }
+    m->has_logits = true;
     if (wait_stream(*m, "mvb_qwen_profile", timeout_s())) return -1;
     for (int k = 0; k < m->kernels_per_step; k++) {
         if ((e = cudaEventElapsedTime(&ms[k], m->prof_ev[k], m->prof_ev[k + 1])) != cudaSuccess) {
@@ -1190,6 +1201,7 @@ extern "C" int mvb_qwen_stamps(void *model, double *us, int cap) {
         set_error("mvb_qwen_stamps: %s", cudaGetErrorString(e));
         return -1;
     }
+    m->has_logits = true;
     if (wait_stream(*m, "mvb_qwen_stamps", timeout_s())) return -1;
     const unsigned long long t0 = ~t[0];
     for (int k = 0; k < m->kernels_per_step; k++) {
@@ -1213,6 +1225,7 @@ extern "C" int mvb_qwen_trace(void *model, int token, int pos, float *trace) {
     cudaError_t e = cudaMalloc(&dev, n * 4);
     if (e == cudaSuccess && set_state(*m, token, pos, -1) == 0) {
         e = enqueue_step(*m, &count, nullptr, nullptr, dev);
+        m->has_logits = e == cudaSuccess;
         if (e == cudaSuccess) e = cudaMemcpyAsync(trace, dev, n * 4, cudaMemcpyDeviceToHost, m->stream);
         if (e == cudaSuccess && wait_stream(*m, "mvb_qwen_trace", timeout_s())) e = cudaErrorUnknown;
     }

@@ -238,7 +238,8 @@ int mvb_kv_read(const void *kq, const float *ks, const void *vq, const float *vs
 /* Attention of the batch's new tokens, whose keys and values are in the cache: out = softmax(scale * q k) v over positions
  * below lens[b] and, of the new ones, those that `tree` allows: rows x words 64-bit words, bit j for the sequence's j-th
  * new token (NULL: each sees those before it and itself). heads is a multiple of kv_heads; out may be q. max_new: at least
- * the most new tokens of a sequence (sequences with more are left out and reported); max_len: about the longest lens[b] +
+ * the most new tokens of a sequence (sequences with more are left out and reported; ceil(max_new * heads / kv_heads / 128) *
+ * kv_heads <= 65535); max_len: about the longest lens[b] +
  * new tokens, which only decides how the work is split. lse (may be NULL): rows x heads, the natural log of the sum of exponentials. A
  * row that sees nothing gives zeros and -inf. fp32 inputs give fp32-accurate results; the same call gives the same bits.
  * work (may be NULL; 16-byte aligned): room of work_bytes for this call alone until it has run; with it, few sequences with

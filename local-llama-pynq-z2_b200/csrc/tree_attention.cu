@@ -583,11 +583,10 @@ static cudaError_t launch_warps(AttnParams p, int max_len, cudaStream_t stream) 
     constexpr size_t smem = frag + (ring > join ? ring : join);
     static_assert(smem <= 227 * 1024 - 8192, "shared memory of a CTA");
     auto kernel = tree_attention_kernel<T, BITS, HDP, NT, kWarps>;
+    if (!tiles_fit(p, ROWS)) return kTooManyRows;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
-    p.qtiles = (int)(((long long)p.max_new * p.group + ROWS - 1) / ROWS);
-    if ((long long)p.qtiles * p.kv_heads > 65535) return cudaErrorInvalidConfiguration;
     // a unit: one slice a warp, 0.7 us (2 where two CTAs of an SM stream); a CTA starts and joins in about 6 us, a second
     // kernel in 2; a cluster's join grows with its CTAs (one sequence of 2,000 keys, 8 kv heads, int8, 4 | 16 rows: clusters
     // of 4, 8, 16 take 11.6, 9.7, 10.0 | 15.4, 13.7, 14.8 us)
@@ -805,10 +804,6 @@ extern "C" int mvb_tree_attention(const void *q, long long q_stride, const void 
         set_error("%s: null or misaligned pointer or stride (cache 16 bytes, q and out four elements, tree 8)", who);
         return -1;
     }
-    if (((long long)max_new * (heads / kv_heads) + 15) / 16 * kv_heads > 65535) {
-        set_error("%s: max_new=%d x heads=%d are too many rows for one call", who, max_new, heads);
-        return -1;
-    }
     AttnParams p = {};
     p.q = q;
     p.out = out;
@@ -845,6 +840,11 @@ extern "C" int mvb_tree_attention(const void *q, long long q_stride, const void 
     else
         e = dtype == rows::kF32 ? launch_size<float, 4>(p, max_len, st)
             : dtype == rows::kBF16 ? launch_size<__nv_bfloat16, 4>(p, max_len, st) : launch_size<__half, 4>(p, max_len, st);
+    if (e == kTooManyRows) {
+        set_error("%s: max_new=%d x heads=%d are too many rows for one call (need ceil(max_new * heads / kv_heads / 128) * "
+                  "kv_heads <= 65535)", who, max_new, heads);
+        return -1;
+    }
     if (e != cudaSuccess) {
         set_error("%s: launch failed: %s", who, cudaGetErrorString(e));
         return -1;

@@ -145,6 +145,14 @@ __device__ __forceinline__ uint32_t nibbles_to_half2(uint32_t x, int k) {
     return h;
 }
 
+// Tiles of `tile` query rows of a sequence with max_new new tokens into p.qtiles; false where a grid cannot hold them.
+inline bool tiles_fit(AttnParams &p, int tile) {
+    const long long n = ((long long)p.max_new * p.group + tile - 1) / tile;
+    p.qtiles = (int)n;
+    return n * p.kv_heads <= 65535;
+}
+constexpr cudaError_t kTooManyRows = cudaErrorInvalidConfiguration;
+
 constexpr int kMaxSplits = 16, kMaxSupers = 8;
 int most_supers(const AttnParams &p);
 

@@ -816,11 +816,10 @@ static cudaError_t launch(AttnParams p, int max_len, cudaStream_t stream) {
     // more than half of an SM's shared memory, so that no second CTA waits for tensor memory
     constexpr size_t smem = S::kBytes > 116 * 1024 ? S::kBytes : 116 * 1024;
     auto kernel = tree_attention_tc_kernel<T, QP, PP, BITS, HDP, MT>;
+    if (!tiles_fit(p, MT * 128)) return kTooManyRows;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
-    p.qtiles = (int)(((long long)p.max_new * p.group + MT * 128 - 1) / (MT * 128));
-    if ((long long)p.qtiles * p.kv_heads > 65535) return cudaErrorInvalidConfiguration;
     const long long base = (long long)p.qtiles * p.kv_heads * p.bt.batch;
     // a unit: a step, 1.2 us with two row tiles; a CTA starts, fills and joins in about 8 us, a second kernel takes 4
     // The tensor core's sums are cut towards zero, 3e-6 to 4e-6 of every element over 4,096 keys with P in two parts: an

@@ -309,8 +309,8 @@ def tree_attention(q, cache, pages, cu, lens, out, tree=None, scale=None, max_ne
     token i at position lens[b] + i), over those their mask allows. q, out (rows, heads, head; out may be q), heads a multiple
     of the cache's kv_heads. tree (rows, words) int64: bit j of a row allows its sequence's j-th new token; None: each sees those
     before it and itself, so that one new token a sequence is a decode step and many are a prompt. scale: default
-    1 / sqrt(head). max_new: at least the most new tokens of a sequence (default: all rows); sequences with more are
-    skipped and reported. max_len: about the longest lens[b] + new tokens (default: the page table's reach), which only
+    1 / sqrt(head). max_new: at least the most new tokens of a sequence (default: all rows, or the page table's reach where
+    that is less; ceil(max_new * heads / kv_heads / 128) * kv_heads <= 65535); sequences with more are skipped and reported. max_len: about the longest lens[b] + new tokens (default: the page table's reach), which only
     decides how finely the work is split. lse (rows, heads) float32: the log of the sum of exponentials. A row that may
     see nothing gives zeros and lse -inf."""
     _T or _torch()
@@ -330,7 +330,7 @@ def tree_attention(q, cache, pages, cu, lens, out, tree=None, scale=None, max_ne
         if lse.dtype is not _T.float32 or lse.shape != (n, heads) or not lse.is_contiguous():
             raise ValueError(f"lse: contiguous float32 {(n, heads)} is needed")
         lp = lse.data_ptr()
-    max_new = n if max_new is None else max_new
+    max_new = min(n, b[1] * cache.page) if max_new is None else max_new
     max_len = b[1] * cache.page if max_len is None else max_len
     work, wp, wn = None, None, 0
     if b[4] * cache.kv_heads <= 18 and max_len >= 16384:  # few jobs, long contexts: a workspace may help

@@ -56,3 +56,30 @@ def test_decoder_logprobs_need_a_step(torch, mvb, tmp_path):
         fine()
     finally:
         dec.close()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_prompts_of_many_rows(torch, mvb, dtype):
+    """Prompts whose rows together pass 32,768, and a max_new above that: 32 heads over 8 kv heads fit one call up to 262,140."""
+    from test_attention_accuracy_gpu import bound
+    new = [4200, 4100, 4225, 4150, 4200, 4000, 4300, 4200]
+    c = Case(torch, mvb, [0] * 8, new, 8, 16, 8, 64)
+    dt = getattr(torch, dtype)
+    q = torch.randn(c.rows, 32, 16, device="cuda").to(dt)
+    for max_new in (None, c.rows, 65536):
+        out = torch.full_like(q, 9.0)
+        mvb.tree_attention(q, c.cache, *c.batch(), out, max_new=max_new)
+        assert mvb.serve_status() == 0 and not (out == 9).all(-1).any()
+        vs = c.cache.vs.cpu().numpy().astype(np.float64)
+        for b in (0, 2, 7):
+            k, v = c.values(b, new[b], 0), c.values(b, new[b], 1)
+            at = np.arange(new[b])
+            for i in (0, 63, 2000, new[b] - 1):
+                row = int(c.cu[b]) + i
+                for h in (0, 7):
+                    want, _, tol, _ = bound(torch, dt, f64(q[row:row + 1, 4 * h:4 * h + 4]), k[:i + 1, h], v[:i + 1, h],
+                                            vs[c.pages[b, at // 64], h, at % 64][:i + 1], np.ones((1, i + 1), bool), 0.25,
+                                            4096, 8 if dtype == "float32" else 12)
+                    assert np.all(np.abs(f64(out[row:row + 1, 4 * h:4 * h + 4]) - want) <= tol)
+    with pytest.raises(mvb.MatvecError, match="too many rows"):
+        mvb.tree_attention(q, c.cache, *c.batch(), out, max_new=1 << 30)

@@ -195,7 +195,7 @@ int mvb_gemm_status(void *stream);
 /* ---- Serving operators: rotary positions, a paged 8- or 4-bit cache, attention over it, log probabilities ----
  * No counterpart in the reference, whose cache is fp32 inside its forward pass. Device pointers, asynchronous on
  * `stream`, on the current device; 0, or -1 with the reason in mvb_last_error(). No call keeps state, so calls on several
- * streams or in several graphs do not meet. Strides are in elements.
+ * streams or in several graphs do not meet, but for what mvb_serve_status reports. Strides are in elements.
  *
  * dtype of queries, keys, values, outputs and logits: MVB_F32, MVB_BF16 or MVB_F16.
  * Cache: kq, vq hold pages x kv_heads x page rows of head integers (bits 8: int8; bits 4: two's complement nibbles, element
@@ -257,9 +257,10 @@ int mvb_tree_attention(const void *q, long long q_stride, const void *kq, const 
 int mvb_logprobs(const void *x, long long stride, int dtype, int rows, int vocab, const int *ids, int nids, float *logp,
                  float *entropy, int top, int *top_ids, float *top_logp, void *stream);
 
-/* Synchronizes `stream`; 0, or what the serving operators found out of range since the last call, and clears it: 1 a page
- * number, 2 a length or row range, 3 a rotary position, 4 a token id, 5 a wait inside a kernel that gave up;
- * -1 if the stream failed. */
+/* Synchronizes `stream`; 0, or what the serving operators found out of range on the current device since the last call, and
+ * clears it: 1 a page number, 2 a length or row range, 3 a rotary position, 4 a token id, 5 a wait inside a kernel that gave
+ * up; -1 if the stream failed. The report is the device's, not the stream's (a captured graph may run on any): whoever asks
+ * first gets what the calls of every stream found. Ask in one place, after the streams whose calls it answers for. */
 int mvb_serve_status(void *stream);
 
 /* ---- Row-sharded matvec with the all-gather fused into the kernel (one process per GPU, NVLink peers) ----

@@ -320,16 +320,9 @@ static void launch_read(const KvParams &p, unsigned grid, cudaStream_t s) {
     else kv_read_kernel<T, 16, BITS><<<grid, 256, 0, s>>>(p);
 }
 
-int kv_take_error(cudaStream_t s) {
-    int v = 0;
-    if (cudaMemcpyFromSymbolAsync(&v, g_kv_error, sizeof v, 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
-        cudaStreamSynchronize(s) != cudaSuccess)
-        return -1;
-    const int z = 0;
-    if (v && (cudaMemcpyToSymbolAsync(g_kv_error, &z, sizeof z, 0, cudaMemcpyHostToDevice, s) != cudaSuccess ||
-              cudaStreamSynchronize(s) != cudaSuccess))
-        return -1;
-    return v;
+int *kv_error_word() {
+    void *p = nullptr;
+    return cudaGetSymbolAddress(&p, g_kv_error) == cudaSuccess ? static_cast<int *>(p) : nullptr;
 }
 
 // The cache's and the batch's arguments, checked; fills p. 0, or -1 after set_error().

@@ -628,28 +628,37 @@ static cudaError_t launch(const Params &p, cudaStream_t stream) {
     return launch_threads<T, TOP, 256>(p, stream);
 }
 
-int logp_take_error(cudaStream_t s) {
-    int v = 0;
-    if (cudaMemcpyFromSymbolAsync(&v, g_logp_error, sizeof v, 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
-        cudaStreamSynchronize(s) != cudaSuccess)
-        return -1;
-    const int z = 0;
-    if (v && (cudaMemcpyToSymbolAsync(g_logp_error, &z, sizeof z, 0, cudaMemcpyHostToDevice, s) != cudaSuccess ||
-              cudaStreamSynchronize(s) != cudaSuccess))
-        return -1;
-    return v;
+int *logp_error_word() {
+    void *p = nullptr;
+    return cudaGetSymbolAddress(&p, g_logp_error) == cudaSuccess ? static_cast<int *>(p) : nullptr;
 }
 
 }  // namespace logp
 
 namespace rows {
-int rope_take_error(cudaStream_t s);
-int kv_take_error(cudaStream_t s);
+int *rope_error_word();
+int *kv_error_word();
 }  // namespace rows
 namespace attn {
-int attn_take_error(cudaStream_t s);
-int tc_take_error(cudaStream_t s);
+int *attn_error_word();
+int *tc_error_word();
 }
+
+// The current device's error words (each source file's own), read and cleared at once: a note that falls between a read and
+// a clearing store of two callers would be lost, or one note be told twice.
+struct ErrorWords {
+    int *at[5];
+};
+__global__ void take_errors_kernel(const ErrorWords w, int *out) {
+    if (threadIdx.x < 5) out[threadIdx.x] = atomicExch(w.at[threadIdx.x], rows::kOk);
+}
+// Five words of host memory that the device writes, a thread's own.
+struct HostWords {
+    int *p = nullptr;
+    ~HostWords() {
+        if (p) cudaFreeHost(p);
+    }
+};
 }  // namespace mvb
 
 using namespace mvb;
@@ -699,18 +708,24 @@ extern "C" int mvb_logprobs(const void *x, long long stride, int dtype, int rows
     return 0;
 }
 
-// Synchronizes `stream`; the first bad index that a serving operator met since the last call (and clears it).
+// Synchronizes `stream`; the first bad index that a serving operator met on the device since the last call (and clears it).
 extern "C" int mvb_serve_status(void *stream) {
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    int first = 0;
-    for (auto take : {rows::rope_take_error, rows::kv_take_error, attn::attn_take_error, attn::tc_take_error,
-                      logp::logp_take_error}) {
-        const int v = take(s);
-        if (v < 0) {
-            set_error("mvb_serve_status: the stream failed: %s", cudaGetErrorString(cudaGetLastError()));
-            return -1;
-        }
-        if (!first) first = v;
+    static thread_local HostWords host;
+    const ErrorWords w = {{rows::rope_error_word(), rows::kv_error_word(), attn::attn_error_word(), attn::tc_error_word(),
+                           logp::logp_error_word()}};
+    cudaError_t e = w.at[0] && w.at[1] && w.at[2] && w.at[3] && w.at[4] ? cudaSuccess : cudaErrorInvalidSymbol;
+    if (e == cudaSuccess && !host.p) e = cudaHostAlloc(&host.p, 5 * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+    if (e == cudaSuccess) {
+        take_errors_kernel<<<1, 32, 0, s>>>(w, host.p);
+        e = cudaGetLastError();
     }
-    return first;
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    if (e != cudaSuccess) {
+        set_error("mvb_serve_status: the stream failed: %s", cudaGetErrorString(e));
+        return -1;
+    }
+    for (int i = 0; i < 5; i++)
+        if (host.p[i]) return host.p[i];
+    return 0;
 }

@@ -72,16 +72,9 @@ static void launch_rope(const RopeParams &p, dim3 grid, bool wide, cudaStream_t 
     launch_lanes<T, 4>(p, grid, s);
 }
 
-int rope_take_error(cudaStream_t s) {
-    int v = 0;
-    if (cudaMemcpyFromSymbolAsync(&v, g_rope_error, sizeof v, 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
-        cudaStreamSynchronize(s) != cudaSuccess)
-        return -1;
-    const int z = 0;
-    if (v && (cudaMemcpyToSymbolAsync(g_rope_error, &z, sizeof z, 0, cudaMemcpyHostToDevice, s) != cudaSuccess ||
-              cudaStreamSynchronize(s) != cudaSuccess))
-        return -1;
-    return v;
+int *rope_error_word() {
+    void *p = nullptr;
+    return cudaGetSymbolAddress(&p, g_rope_error) == cudaSuccess ? static_cast<int *>(p) : nullptr;
 }
 
 }  // namespace rows

@@ -738,16 +738,9 @@ int cluster_slots(const void *kernel, int n, int threads, size_t smem) {
     return clusters * n;
 }
 
-int attn_take_error(cudaStream_t s) {
-    int v = 0;
-    if (cudaMemcpyFromSymbolAsync(&v, g_attn_error, sizeof v, 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
-        cudaStreamSynchronize(s) != cudaSuccess)
-        return -1;
-    const int z = 0;
-    if (v && (cudaMemcpyToSymbolAsync(g_attn_error, &z, sizeof z, 0, cudaMemcpyHostToDevice, s) != cudaSuccess ||
-              cudaStreamSynchronize(s) != cudaSuccess))
-        return -1;
-    return v;
+int *attn_error_word() {
+    void *p = nullptr;
+    return cudaGetSymbolAddress(&p, g_attn_error) == cudaSuccess ? static_cast<int *>(p) : nullptr;
 }
 
 }  // namespace attn

@@ -195,7 +195,6 @@ inline Split choose_splits(long long base, int batch, double steps, double fixed
     return best;
 }
 
-int tc_take_error(cudaStream_t s);
 // The kernel for many query rows; returns the CUDA error of its launch.
 cudaError_t launch_tc(const AttnParams &p, int dtype, int bits, int max_len, cudaStream_t s);
 

@@ -869,16 +869,9 @@ cudaError_t launch_tc(const AttnParams &p, int dtype, int bits, int max_len, cud
     return p.head <= 64 ? launch_type<4, 64>(p, dtype, max_len, s) : launch_type<4, 128>(p, dtype, max_len, s);
 }
 
-int tc_take_error(cudaStream_t s) {
-    int v = 0;
-    if (cudaMemcpyFromSymbolAsync(&v, g_tc_error, sizeof v, 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
-        cudaStreamSynchronize(s) != cudaSuccess)
-        return -1;
-    const int z = 0;
-    if (v && (cudaMemcpyToSymbolAsync(g_tc_error, &z, sizeof z, 0, cudaMemcpyHostToDevice, s) != cudaSuccess ||
-              cudaStreamSynchronize(s) != cudaSuccess))
-        return -1;
-    return v;
+int *tc_error_word() {
+    void *p = nullptr;
+    return cudaGetSymbolAddress(&p, g_tc_error) == cudaSuccess ? static_cast<int *>(p) : nullptr;
 }
 
 }  // namespace attn

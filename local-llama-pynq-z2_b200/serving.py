@@ -18,7 +18,8 @@ are. All of it is read on the device: a call may be captured in a CUDA graph and
 Checks: types, shapes, strides and devices are checked here (ValueError) and in the library (MatvecError). What only the
 device can see (a page number, position or length out of range) is skipped there, never followed, and reported by
 serve_status(). Calls are asynchronous on `stream` (default: the current stream of the tensors' device) and may run on any
-device; they keep no state, and memory that a call needs is its own, so calls on several streams do not meet.
+device; they keep no state, and memory that a call needs is its own, so calls on several streams do not meet, but for the
+device's one serve_status().
 """
 import ctypes as C
 import math
@@ -399,8 +400,9 @@ STATUS = {0: "ok", 1: "a page number out of range", 2: "a length or a row range 
 
 
 def serve_status(stream=None, device=None):
-    """Synchronizes `stream` and returns the first thing that the serving operators found out of range on the device since
-    the last call (a key of STATUS; 0: nothing), clearing it. Outputs of a call that reported are not to be used."""
+    """Synchronizes `stream` and returns what the serving operators found out of range on the device since the last call (a
+    key of STATUS; 0: nothing), clearing it. Outputs of a call that reported are not to be used. The report is the device's, not
+    the stream's: ask in one place, after the streams whose calls it answers for."""
     torch = _torch()
     m = _mvb()
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)

@@ -83,3 +83,32 @@ def test_prompts_of_many_rows(torch, mvb, dtype):
                     assert np.all(np.abs(f64(out[row:row + 1, 4 * h:4 * h + 4]) - want) <= tol)
     with pytest.raises(mvb.MatvecError, match="too many rows"):
         mvb.tree_attention(q, c.cache, *c.batch(), out, max_new=1 << 30)
+
+
+def test_status_told_once(torch, mvb):
+    """Two threads that ask while one of them makes bad calls: every report reaches one of them, once."""
+    import threading
+    assert mvb.serve_status() == 0
+    f, _ = mvb.rope_frequencies(64, 1e4)
+    table = mvb.rope_table(f, 10)
+    x = torch.ones(1, 1, 64, device="cuda")
+    pos = torch.full((1,), 10, dtype=torch.int32, device="cuda")
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    told, done = [0, 0], threading.Event()
+
+    def other():
+        while not done.is_set():
+            told[1] += mvb.serve_status(stream=streams[1], device="cuda:0") != 0
+
+    t = threading.Thread(target=other)
+    t.start()
+    n = 2000
+    for _ in range(n):
+        mvb.rope(x, pos, table, stream=streams[0])
+        streams[0].synchronize()
+        told[0] += mvb.serve_status(stream=streams[0]) != 0
+    done.set()
+    t.join()
+    told[0] += mvb.serve_status() != 0
+    assert sum(told) == n, told

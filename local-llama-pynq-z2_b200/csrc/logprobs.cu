@@ -19,6 +19,8 @@
 #include <limits.h>
 #include <math.h>
 
+#include <atomic>
+
 #include "../../include/matvec_b200.h"
 #include "mvb_runtime.h"
 #include "rows.cuh"
@@ -609,10 +611,13 @@ static cudaError_t launch_threads(Params p, cudaStream_t stream) {
 // The rows that whole waves hold, one row a CTA: the time of p.rows rows goes with it, since rows are alike.
 template <typename T, bool TOP, int kThreads>
 static long long rows_of_waves(const Params &p) {
-    static const size_t fixed = [] {
+    static std::atomic<size_t> known{0};
+    size_t fixed = known.load(std::memory_order_relaxed);
+    if (!fixed) {  // (a query that failed is not kept)
         cudaFuncAttributes a = {};
-        return cudaFuncGetAttributes(&a, logprobs_kernel<T, TOP, kThreads>) == cudaSuccess ? a.sharedSizeBytes : (size_t)0;
-    }();
+        if (cudaFuncGetAttributes(&a, logprobs_kernel<T, TOP, kThreads>) == cudaSuccess) known.store(fixed = a.sharedSizeBytes);
+        else cudaGetLastError();
+    }
     const size_t smem = TOP ? ((size_t)p.vocab / (kThreads * 32) + 2) * kThreads * 4 : 0;
     const long long fit = 228 * 1024 / (long long)(fixed + smem + 1024), most = 768 / kThreads;
     const long long slots = 148 * (fit < 1 ? 1 : fit < most ? fit : most);

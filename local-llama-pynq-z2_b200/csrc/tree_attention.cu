@@ -708,7 +708,8 @@ cudaError_t launch_join(const AttnParams &p, int dtype, cudaStream_t s) {
 int cluster_slots(const void *kernel, int n, int threads, size_t smem) {
     struct Entry {
         const void *kernel;
-        int device, n, slots;
+        int device, n, threads, slots;
+        size_t smem;
     };
     static std::mutex mutex;
     static Entry known[1024];
@@ -717,7 +718,9 @@ int cluster_slots(const void *kernel, int n, int threads, size_t smem) {
     if (cudaGetDevice(&device) != cudaSuccess) return n == 1 ? 148 : 0;
     std::lock_guard<std::mutex> lock(mutex);
     for (int i = 0; i < count; i++)
-        if (known[i].kernel == kernel && known[i].device == device && known[i].n == n) return known[i].slots;
+        if (known[i].kernel == kernel && known[i].device == device && known[i].n == n && known[i].threads == threads &&
+            known[i].smem == smem)
+            return known[i].slots;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(n);
     cfg.blockDim = dim3(threads);
@@ -732,9 +735,9 @@ int cluster_slots(const void *kernel, int n, int threads, size_t smem) {
     int clusters = 0;
     if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) {
         cudaGetLastError();
-        clusters = 0;
+        return 0;  // not kept: the next call asks again
     }
-    if (count < (int)(sizeof known / sizeof known[0])) known[count++] = Entry{kernel, device, n, clusters * n};
+    if (count < (int)(sizeof known / sizeof known[0])) known[count++] = Entry{kernel, device, n, threads, clusters * n, smem};
     return clusters * n;
 }
 

@@ -112,3 +112,16 @@ def test_status_told_once(torch, mvb):
     t.join()
     told[0] += mvb.serve_status() != 0
     assert sum(told) == n, told
+
+
+def test_failed_occupancy_query_is_not_kept(torch, mvb):
+    """A query of the device that fails (here: more threads than a block may have) says nothing about the next."""
+    import ctypes as C
+    L = mvb.lib()
+    slots = L["_ZN3mvb4attn13cluster_slotsEPKviim"]
+    slots.restype, slots.argtypes = C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_size_t]
+    for name in ("_ZN3mvb4attn11join_kernelIfEEvNS0_10AttnParamsE", "_ZN3mvb4attn11join_kernelI6__halfEEvNS0_10AttnParamsE"):
+        kernel = C.cast(L[name], C.c_void_p)
+        for n in (1, 2, 4):
+            assert slots(kernel, n, 4096, 0) == 0
+            assert slots(kernel, n, 128, 0) >= 148 // n * n

@@ -142,7 +142,10 @@ __global__ void __launch_bounds__(256, 4) kv_append_kernel(const KvParams p) {
     // those that quantize: 14,000 rows of 32 + 8 heads took 179 us so)
     const int chunk = blockIdx.y;
     const long long tok = (long long)blockIdx.x * 8 + warp;
-    if (tok >= p.rows || tok >= p.bt.cu[p.bt.batch] || tok < p.bt.cu[0]) return;  // rows of no sequence stay as they are
+    if (tok >= p.rows) return;
+    const int end = p.bt.cu[p.bt.batch];
+    if (tok == p.rows - 1 && end > p.rows && lane == 0) note(&g_kv_error, kBadLength);  // rows that the arrays lack
+    if (tok >= end || tok < p.bt.cu[0]) return;  // rows of no sequence stay as they are
     const bool on = E * l < p.head, in_rot = E * l < p.rot;
     const bool is_q = chunk >= p.kv_chunks;
     int b = 0;
@@ -244,7 +247,9 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvParams p) {
     if (tid < nt) {
         const int tok = t0 + tid;
         long long slot = -1;
-        if (tok < p.bt.cu[p.bt.batch] && tok >= p.bt.cu[0]) {
+        const int end = p.bt.cu[p.bt.batch];
+        if (tok == p.rows - 1 && end > p.rows) note(&g_kv_error, kBadLength);  // rows that the arrays lack
+        if (tok < end && tok >= p.bt.cu[0]) {
             int lo = 0, hi = p.bt.batch;  // the first sequence that ends behind the row
             while (lo < hi) {
                 const int mid = (lo + hi) >> 1;

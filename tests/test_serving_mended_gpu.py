@@ -125,3 +125,22 @@ def test_failed_occupancy_query_is_not_kept(torch, mvb):
         for n in (1, 2, 4):
             assert slots(kernel, n, 4096, 0) == 0
             assert slots(kernel, n, 128, 0) >= 148 // n * n
+
+
+@pytest.mark.parametrize("rows", [1, 6, 40])
+def test_more_rows_than_the_arrays_hold(torch, mvb, rows):
+    """cu that ends behind the row arrays: the rows there are are done, the rest is reported."""
+    c = Case(torch, mvb, [5, 0], [rows, 3], 2, 64, 8, 16)
+    k = torch.randn(rows, 2, 64, device="cuda")
+    mvb.kv_append(c.cache, k, k, *c.batch())
+    assert mvb.serve_status() == 2
+    ko, vo = torch.full_like(k, 5.0), torch.full_like(k, 5.0)
+    mvb.kv_read(c.cache, *c.batch(), ko, vo)
+    assert mvb.serve_status() == 2
+    ints, scale = ref.quantize(f64(k), 8)
+    want = ints * scale[..., None]
+    assert np.all(np.abs(f64(ko) - want) <= 2 ** -23 * np.abs(want)) and torch.equal(ko, vo)
+    exact = torch.tensor([0, rows, rows], dtype=torch.int32, device="cuda")
+    mvb.kv_append(c.cache, k, k, c.pages_, exact, c.lens_)
+    mvb.kv_read(c.cache, c.pages_, exact, c.lens_, ko, vo)
+    assert mvb.serve_status() == 0

@@ -592,7 +592,7 @@ static cudaError_t launch_warps(AttnParams p, int max_len, cudaStream_t stream) 
     // of 4, 8, 16 take 11.6, 9.7, 10.0 | 15.4, 13.7, 14.8 us)
     const Split cut = choose_splits((long long)p.qtiles * p.kv_heads * p.bt.batch, p.bt.batch,
                                     (double)max_len / (kWarps * S::kKeys), 3.0, 8.0, NT == 1 ? 0.14 : 0.26, 2.0,
-                                    1.0, 1, most_supers(p),
+                                    1.0, most_supers(p),
                                     [&](int n) { return cluster_slots((const void *)kernel, n, kWarps * 32, smem); });
     p.splits = cut.splits;
     p.supers = cut.supers;

@@ -163,23 +163,23 @@ int cluster_slots(const void *kernel, int n, int threads, size_t smem);
 // Over how many CTAs of a cluster (splits) and how many clusters (supers, at most most_supers) a sequence's keys are split,
 // so that the estimated time is least: `base` jobs without a split, `steps` units of work each for the longest sequence,
 // `fixed` units to start, fill and join a CTA (`more` where the CTAs exceed one wave), `each` for every CTA of the cluster
-// that it is joined with, and `join` for a second kernel, at least `least` units a CTA and, where slots allow, `fewest`
-// CTAs. All in one wave: whole units. More, of one sequence: its jobs are alike and run in whole waves. Several: three
-// quarters of the longest on average, in no order, and the last jobs end a third of a job apart.
+// that it is joined with, and `join` for a second kernel, at least `least` units a CTA. All in one wave: whole units. More,
+// of one sequence: its jobs are alike and run in whole waves. Several: three quarters of the longest on average, in no
+// order, and the last jobs end a third of a job apart.
 struct Split {
     int splits, supers;
 };
 template <typename F>
 inline Split choose_splits(long long base, int batch, double steps, double fixed, double more, double each,
-                           double join, double least, int fewest, int most_supers, const F &slots_of) {
+                           double join, double least, int most_supers, const F &slots_of) {
     Split best = {1, 1};
     double best_time = 1e300;
     for (int n = 1; n <= kMaxSplits; n++) {
-        if (n > fewest && steps < least * n) break;
+        if (n > 1 && steps < least * n) break;
         const int slots = slots_of(n);
         if (slots < n) continue;
         for (int m = 1; m <= most_supers; m++) {
-            if (n * m > fewest && m > 1 && steps < least * n * m) break;
+            if (m > 1 && steps < least * n * m) break;
             const double fill = (double)base * n * m / slots, units = steps / (n * m);
             const double job = (fill > 1.0 ? units + more : ceil(units) + fixed) + n * each;
             if (each > 0.0 && fill <= 1.0 && (n & (n - 1))) continue;  // clusters of 6 or 12 take longer than of 8 or 16
@@ -187,9 +187,8 @@ inline Split choose_splits(long long base, int batch, double steps, double fixed
             if (fill > 1.0) time = batch == 1 ? (double)((base * n * m + slots - 1) / slots) * job
                                               : (0.75 * fill > 1.0 ? 0.75 * fill : 1.0) * job + job / 3;
             if (m > 1) time += join;
-            if (n * m < fewest) time += 1e6 * (fewest - n * m);
             if (time < best_time * 0.999) best_time = time, best = Split{n, m};
-            if (fill > 2.0 && n * m >= fewest) break;
+            if (fill > 2.0) break;
         }
     }
     return best;

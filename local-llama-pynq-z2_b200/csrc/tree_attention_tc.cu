@@ -258,6 +258,24 @@ struct TcSmem {
     static_assert(kBytes <= 227 * 1024, "shared memory of a CTA");
 };
 
+// Before the first product of a span: a thread's half of O, from column `at` on, goes into its sums, whose last element is the
+// unit they are in. A call of its own, so that the steps keep their registers.
+template <int HDP>
+__device__ __noinline__ void keep(float *sums, uint32_t at, float unit, bool first, uint64_t *pv_done, uint32_t parity) {
+    bar_wait(pv_done, parity);
+    fence_after();
+    const float f = first ? 0.0f : unit_factor(sums[HDP / 2], unit);
+    sums[HDP / 2] = unit;
+#pragma unroll 1
+    for (int c = 0; c < HDP / 2; c += 16) {
+        float o[16];
+        tmem_load16(at + c, o);
+        wait_load();
+#pragma unroll
+        for (int e = 0; e < 16; e++) sums[c + e] = first ? o[e] : __fmaf_rn(sums[c + e], f, o[e]);
+    }
+}
+
 template <typename T, int QP, int PP, int BITS, int HDP, int MT>
 __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const AttnParams p) {
     using S = TcSmem<QP, BITS, HDP, MT>;
@@ -265,6 +283,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
     constexpr bool ALT = MT == 1;            // the groups alternate over the steps
     constexpr int PARTS = ALT ? 2 : 1;       // partial results of a row in a CTA
     constexpr int kRaw = S::kRaw;
+    // The products' sums are cut towards zero at 2^-23 for every 16 keys and part, which adds up: values of one sign lost 1e-5 over
+    // 4,096 keys of an fp32 caller and 2e-3 over 500,000. So a group's product starts anew every kSpan steps, and its threads
+    // add what there was to sums of their own, rounded to nearest (in local memory: 260 bytes a thread, touched only then).
+    // That takes about 3,000 clocks; a step with heads of 64 is shorter, hence the longer span there (16 sequences of 8,000
+    // keys, 256 rows of 64: 124 us with 16 steps). bf16 callers, whose output's half step is 4e-3 and whose products have one
+    // part, go without.
+    constexpr int kSpan = PP == 1 ? 1 << 30 : sizeof(T) == 4 ? 2048 / HDP : 128;
+    constexpr bool SPANS = PP > 1;
     extern __shared__ __align__(1024) uint8_t raw_smem[];
     uint8_t *smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);
     uint64_t *bar = reinterpret_cast<uint64_t *>(smem + S::kBar);
@@ -482,7 +508,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
 #pragma unroll
                             for (int k = 0; k < kBN / 16; k++)
                                 mma_ts(t + 256 + m * 128, t + m * 128 + (i & 1) * 64 + part * 32 + k * 8,
-                                       v0 + ((slot * S::kTile + k * 2048) >> 4), pv, i > 0 || part > 0 || k > 0);
+                                       v0 + ((slot * S::kTile + k * 2048) >> 4), pv, (SPANS ? i % kSpan : i) > 0 || part > 0 || k > 0);
                         commit(&pv_done[m]);
                         if (ALT || m == 1) commit(&v_free[j % kTurns]);
                         ok = scores(m, i + 2);
@@ -566,6 +592,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
         const int R = R0 + (ALT ? 0 : m * 128) + row, draft = R / p.group;
         const float rf = row_factor[ALT ? row : m * 128 + row];
         float unit = INFINITY, l = 0.0f;
+        float sums[SPANS ? HDP / 2 + 1 : 1];  // what spans before summed, and the unit it is in
         // One step; TAIL: some of its keys are new tokens, or none (a variant of its own: the mask's branches cost the
         // others more than their arithmetic).
         auto step = [&](int i, auto is_tail) -> bool {
@@ -671,6 +698,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
             split2(sum[1], a2, d2);
             l += (a + d) + (a2 + d2);
             wait_store();
+            if constexpr (SPANS) {
+                if (i > 0 && i % kSpan == 0) keep<HDP>(sums, o_at + half * (HDP / 2), unit, i == kSpan, &pv_done[m], (i - 1) & 1);
+            }
             fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive(&p_ready[2 * m + slot]);
@@ -701,6 +731,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
         l = half ? *other_x + l : l + *other_x;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // both in the row's unit
         const int c0 = half * (HDP / 32);  // this thread's half of O, 16 columns at a time
+        auto load_o = [&](int c, float *o) {  // 16 columns of O, with what was summed before
+            tmem_load16(o_at + 16 * c, o);
+            wait_load();
+            if constexpr (SPANS) {
+                if (steps <= kSpan) return;
+                const float f = unit_factor(sums[HDP / 2], unit);
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[e] = __fmaf_rn(sums[16 * (c - c0) + e], f, o[e]);
+            }
+        };
         if (!ALT && p.splits * p.supers == 1) {
             const int tok = s.row0 + R / p.group, head = kvh * p.group + R % p.group;
             if (R < nrows && p.lse && half == 0)
@@ -709,10 +749,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
 #pragma unroll 1
             for (int c = c0; c < c0 + HDP / 32; c++) {
                 float o[16];
-                if (mine > 0) {
-                    tmem_load16(o_at + 16 * c, o);
-                    wait_load();
-                }
+                if (mine > 0) load_o(c, o);
                 if (R >= nrows) continue;
                 T *d = static_cast<T *>(p.out) + (size_t)tok * p.out_stride + (size_t)head * p.head + 16 * c;
 #pragma unroll
@@ -732,10 +769,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
 #pragma unroll 1
             for (int c = c0; c < c0 + HDP / 32; c++) {
                 float o[16];
-                if (steps > 0) {
-                    tmem_load16(o_at + 16 * c, o);
-                    wait_load();
-                }
+                if (steps > 0) load_o(c, o);
                 // the 16-byte pieces of a row start at different places: different banks
 #pragma unroll
                 for (int i = 0; i < 16; i += 4)
@@ -822,13 +856,7 @@ static cudaError_t launch(AttnParams p, int max_len, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     const long long base = (long long)p.qtiles * p.kv_heads * p.bt.batch;
     // a unit: a step, 1.2 us with two row tiles; a CTA starts, fills and joins in about 8 us, a second kernel takes 4
-    // The tensor core's sums are cut towards zero, 3e-6 to 4e-6 of every element over 4,096 keys with P in two parts: an
-    // fp32 caller's sequences are split into at most that many a CTA while 16 CTAs (32 with a workspace) suffice, since the
-    // joins round to nearest. Against 8,192 a CTA this takes the worst of some thousand random calls of 20,000 keys and more from
-    // 1.0e-5 to 9e-6 off the fp32 formula, for 6 % of the time at 131,001 keys.
-    const int most = kMaxSplits * (most_supers(p) > 1 ? 2 : 1);
-    const int fewest = sizeof(T) == 4 ? (max_len >= most * 4096 ? most : max_len / 4096 + 1) : 1;
-    const Split cut = choose_splits(base, p.bt.batch, (double)max_len / kBN, 6.0, 8.0, 0.0, 3.0, 4.0, fewest, most_supers(p),
+    const Split cut = choose_splits(base, p.bt.batch, (double)max_len / kBN, 6.0, 8.0, 0.0, 3.0, 4.0, most_supers(p),
                                     [&](int n) { return slots((const void *)kernel, n, smem); });
     p.splits = cut.splits;
     p.supers = cut.supers;

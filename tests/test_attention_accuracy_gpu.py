@@ -240,3 +240,17 @@ def test_long_fp32(torch, mvb, bits, ctx, heads, kv_heads, head, tokens):
     torch.manual_seed(1)
     q = torch.randn(tokens, heads, head, device="cuda") * 2
     check(torch, mvb, c, q, together=4096, max_len=ctx + tokens)
+
+
+@pytest.mark.parametrize("dtype,ctx,span", [("float32", 60000, 16), ("float16", 60000, 128), ("bfloat16", 60000, 128)])
+@pytest.mark.parametrize("heads,head,tokens", [(1, 64, 30), (1, 128, 40), (3, 64, 60), (3, 128, 60)])
+@pytest.mark.parametrize("max_len", [16, 60100])
+def test_sums_do_not_drift(torch, mvb, dtype, ctx, span, heads, head, tokens, max_len):
+    """Values of one sign, whose sums the tensor core cuts in one direction: what is lost stays that of one span of keys, however
+    many a CTA has, so that max_len decides the split alone. (The sums of the spans, 60 at most, are rounded to nearest: within
+    the bound's roundings of a join.)"""
+    c = Case(torch, mvb, [ctx], [tokens], 1, head, 8, 64, seed=tokens)
+    torch.manual_seed(2)
+    c.cache.vq.copy_(c.cache.vq.abs().clamp(min=30))
+    q = (torch.randn(tokens, heads, head, device="cuda")).to(getattr(torch, dtype))
+    check(torch, mvb, c, q, together=64 * (32 if head == 64 and dtype == "float32" else span), max_len=max_len)

@@ -203,8 +203,8 @@ int mvb_gemm_status(void *stream);
  * in 16 .. 1024; head: a multiple of 16 in 16 .. 128; all four 16-byte aligned.
  * Batch: rows cu[b] .. cu[b + 1] - 1 belong to sequence b and stand at its positions lens[b] and on; position p is slot
  * p % page of page table[b * table_cols + p / page]. `rows` is the room of the row arrays; rows at or behind cu[batch]
- * are left as they are. cu, lens and table are read on the device; what is out of range there is skipped and reported by
- * mvb_serve_status. */
+ * are left as they are. cu (which does not fall), lens and table are read on the device; what is out of range there is
+ * skipped and reported by mvb_serve_status. */
 #define MVB_F32 0
 #define MVB_BF16 1
 #define MVB_F16 2
@@ -239,11 +239,10 @@ int mvb_kv_read(const void *kq, const float *ks, const void *vq, const float *vs
  * below lens[b] and, of the new ones, those that `tree` allows: rows x words 64-bit words, bit j for the sequence's j-th
  * new token (NULL: each sees those before it and itself). heads is a multiple of kv_heads; out may be q. max_new: at least
  * the most new tokens of a sequence (sequences with more are left out and reported; ceil(max_new * heads / kv_heads / 128) *
- * kv_heads <= 65535); max_len: about the longest lens[b] +
- * new tokens, which only decides how the work is split. lse (may be NULL): rows x heads, the natural log of the sum of exponentials. A
- * row that sees nothing gives zeros and -inf. fp32 inputs: products of 22-bit parts summed in
- * fp32, within 2e-5 of a row's sum of weighted magnitudes (some 1e-6 up to 24 rows a kv head, 5e-6 above), however long
- * the context and whatever max_len. The same call gives the same bits.
+ * kv_heads <= 65535); max_len: about the longest lens[b] + new tokens, which only decides how the work is split. lse (may be
+ * NULL): rows x heads, the natural log of the sum of exponentials. A row that sees nothing gives zeros and -inf. fp32 inputs:
+ * products of 22-bit parts summed in fp32, within 2e-5 of a row's sum of weighted magnitudes (some 1e-6 up to 24 rows a kv
+ * head, 5e-6 above), however long the context and whatever max_len. The same call gives the same bits.
  * work (may be NULL; 16-byte aligned): room of work_bytes for this call alone until it has run; with it, few sequences with
  * long contexts are split over more SMs. mvb_tree_attention_work gives the bytes worth having for such sizes, or 0. */
 size_t mvb_tree_attention_work(int rows, int heads, int kv_heads, int head, int batch, int max_new, int max_len);

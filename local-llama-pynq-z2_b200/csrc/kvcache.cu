@@ -153,7 +153,12 @@ __global__ void __launch_bounds__(256, 4) kv_append_kernel(const KvParams p) {
     if (!is_q || !p.pos) {
         b = sequence_of(p.bt.cu, p.bt.batch, (int)tok);
         if (b >= p.bt.batch) return;
-        at = (long long)p.bt.lens[b] + tok - p.bt.cu[b];
+        const int first = p.bt.cu[b];
+        if (first < 0 || first > tok) {  // cu that falls, or begins below 0
+            if (lane == 0) note(&g_kv_error, kBadLength);
+            return;
+        }
+        at = (long long)p.bt.lens[b] + tok - first;
     }
     Turn<E> t;
 #pragma unroll
@@ -257,8 +262,10 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvParams p) {
                 else hi = mid;
             }
             if (lo < p.bt.batch) {
-                const long long at = (long long)p.bt.lens[lo] + tok - p.bt.cu[lo];
-                slot = at > INT_MAX ? -1 : slot_of(p.bt, lo, (int)at, &g_kv_error);
+                const int first = p.bt.cu[lo];
+                const long long at = (long long)p.bt.lens[lo] + tok - first;
+                if (first < 0 || first > tok) note(&g_kv_error, kBadLength);  // cu that falls, or begins below 0
+                else slot = at > INT_MAX ? -1 : slot_of(p.bt, lo, (int)at, &g_kv_error);
             }
         }
         slots[tid] = slot;

@@ -144,3 +144,24 @@ def test_more_rows_than_the_arrays_hold(torch, mvb, rows):
     mvb.kv_append(c.cache, k, k, c.pages_, exact, c.lens_)
     mvb.kv_read(c.cache, c.pages_, exact, c.lens_, ko, vo)
     assert mvb.serve_status() == 0
+
+
+@pytest.mark.parametrize("cu", [[-3, 4, 8], [0, 9, 3, 8]])
+def test_row_ranges_out_of_order(torch, mvb, cu):
+    """cu that begins below 0 or falls: what was cached before stays, and the append reports rows whose sequence begins elsewhere;
+    rows before the first are read as nobody's."""
+    c = Case(torch, mvb, [20] * (len(cu) - 1), [4] * (len(cu) - 1), 2, 64, 8, 16)
+    k = torch.randn(9, 2, 64, device="cuda")
+    negative = cu[0] < 0
+    cu = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    keep = c.cache.kq.clone()
+    mvb.kv_append(c.cache, k, k, c.pages_, cu, c.lens_)
+    assert mvb.serve_status() == 2
+    for b in range(len(cu) - 1):
+        for i in range(20):
+            pg, sl = int(c.pages[b, i // 16]), i % 16
+            assert torch.equal(c.cache.kq[pg, :, sl], keep[pg, :, sl])
+    if negative:
+        ko, vo = torch.full_like(k, 5.0), torch.full_like(k, 5.0)
+        mvb.kv_read(c.cache, c.pages_, cu, c.lens_, ko, vo)
+        assert mvb.serve_status() == 2 and (ko[:4] == 5).all() and not (ko[4:8] == 5).any()

@@ -96,7 +96,8 @@ __device__ __forceinline__ int exponent_of(float x) { return (__float_as_int(x) 
 // 2^(kTop - lazy). fp16's steps below 2^-14 are 2^-24, so no weight is off by more than 2^(lazy - 40) of the row's largest
 // weight times value scale. Only weights and scales that the row sees count: a key that the mask hides from it leaves b
 // where it is, and so does one that stands far above the rest while its value is near zero. b is a whole number, so that O and
-// l change by exact factors; infinite while the row has seen no score.
+// l change by exact factors (of scores above 2^24, whose spacing leaves nothing else, minus the score); infinite while the
+// row has seen none.
 __host__ __device__ constexpr float lazy(int parts) { return parts == 2 ? 9.0f : 13.0f; }
 constexpr float kTop = 15.99f, kSumTop = 100.0f;
 // What the largest score plus b may reach beside value scales up to vmax before `moved` has to be asked.

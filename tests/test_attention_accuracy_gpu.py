@@ -254,3 +254,31 @@ def test_sums_do_not_drift(torch, mvb, dtype, ctx, span, heads, head, tokens, ma
     c.cache.vq.copy_(c.cache.vq.abs().clamp(min=30))
     q = (torch.randn(tokens, heads, head, device="cuda")).to(getattr(torch, dtype))
     check(torch, mvb, c, q, together=64 * (32 if head == 64 and dtype == "float32" else span), max_len=max_len)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,head,tokens", [(4, 64, 1), (4, 128, 5), (3, 64, 50), (3, 128, 100)])
+@pytest.mark.parametrize("nats", [1e4, 3e6, 4e7, 1e9, 1e12, -1e9])
+def test_huge_scores(torch, mvb, dtype, heads, head, tokens, nats):
+    """One key far above all others, by more than fp32 can tell a score from the next (or all others far above one, and alike
+    but for their values): the row is that key's value."""
+    c = Case(torch, mvb, [900], [tokens], 1, head, 8, 64, seed=head)
+    q = dominant(torch, c, tokens, heads, dtype, nats, 1.0, at=500)
+    out, lse = torch.empty_like(q), torch.empty(tokens, heads, device="cuda")
+    mvb.tree_attention(q, c.cache, *c.batch(), out, max_new=tokens, lse=lse)
+    if nats < 0:
+        keep = c.cache.ks[int(c.pages[0, 7]), :, 500 % 64].clone()
+        assert float(keep.max()) > 0
+        check(torch, mvb, c, q)
+        return
+    v = c.values(0, 501, 1)[500, 0]
+    half = torch.finfo(q.dtype).eps / 2
+    # P's parts; a score above 2^24 leaves its unit no whole number next to it but itself, so that P' is the value scale, held in
+    # steps of at most 2^-24
+    vs = float(c.cache.vs[int(c.pages[0, 500 // 64]), 0, 500 % 64])
+    p = max(2.0 ** -11 if dtype == "bfloat16" else 2.0 ** -22, 2.0 ** -25 / vs if nats > 2 ** 23 else 0.0)
+    assert np.all(np.abs(f64(out) - v) <= (half + p + 2.0 ** -21) * np.abs(v))
+    k = c.values(0, 501, 0)[500, 0]
+    want = f64(q) @ k * head ** -0.5
+    # q's parts, the cut sums of at most 128 products, the scale's four roundings: all relative to sum |q k|, here the score
+    assert np.all(np.abs(f64(lse) - want) <= 2.0 ** -18 * np.abs(want))

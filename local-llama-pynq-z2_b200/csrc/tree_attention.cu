@@ -349,23 +349,29 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 && NT <= 2 ? 2 : 1) t
             }
         if (__any_sync(0xffffffffu, move)) {
             move = __reduce_or_sync(0xffffffffu, move);
+            float lv[S::kSub][2];
+#pragma unroll
+            for (int sub = 0; sub < S::kSub; sub++)
+#pragma unroll
+                for (int n = 0; n < 2; n++) lv[sub][n] = log_scale(vv[sub][n]);
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     if (!((move >> (2 * nt + h)) & 1)) continue;
-                    float t = mx[nt][h], w = 0.0f;
-#pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+                    float t = mx[nt][h], top = -INFINITY;
 #pragma unroll
                     for (int sub = 0; sub < S::kSub; sub++)
 #pragma unroll
                         for (int n = 0; n < 2; n++)
-                            w = fmaxf(w, product_of(sc[nt][sub][2 * n + h], rf[nt][h], t, vv[sub][n]));
+                            top = fmaxf(top, __fmaf_rn(sc[nt][sub][2 * n + h], rf[nt][h], lv[sub][n]));
 #pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, o));
+                    for (int o = 4; o < 32; o <<= 1) {
+                        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    }
                     // only the rows that are behind move, so that a row's result does not depend on its neighbours
-                    const float to = moved<PP>(unit[nt][h], t, w), f = unit_factor(unit[nt][h], to);
+                    const float to = moved<PP>(unit[nt][h], t, top), f = unit_factor(unit[nt][h], to);
                     unit[nt][h] = to;
                     l[nt][h] *= f;
 #pragma unroll
@@ -442,8 +448,9 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 && NT <= 2 ? 2 : 1) t
                     const uint4 a = make_uint4(vb[k][0], vb[k + 1][0], vb[k][1], vb[k + 1][1]);
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
-                        // The products' own sums are cut towards zero: over 10,000 keys that takes 4e-6 off every element. An
-                        // fp32 caller's slices are therefore added here, rounded to nearest.
+                        // The products' own sums are cut towards zero, at 2^-23 for every 16 keys and part: some 1e-4 over 16,000 keys
+                        // of a warp whose values have one sign, a quarter of an fp16 output's half step. An fp32 caller's
+                        // slices are therefore added here, rounded to nearest.
                         constexpr bool APART = sizeof(T) == 4;
                         float (&o)[4] = O[nt][(PER * i + k) / 2];
                         float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};

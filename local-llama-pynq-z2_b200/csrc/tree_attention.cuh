@@ -102,15 +102,17 @@ __host__ __device__ constexpr float lazy(int parts) { return parts == 2 ? 9.0f :
 constexpr float kTop = 15.99f, kSumTop = 100.0f;
 // What the largest score plus b may reach beside value scales up to vmax before `moved` has to be asked.
 __device__ __forceinline__ float unit_limit(float vmax) { return fminf(kSumTop, (kTop - 0.005f) - __log2f(vmax)); }
+// log2 of a value scale, for scores plus that: nothing where the scale is infinite.
+__device__ __forceinline__ float log_scale(float vs) { return fabsf(vs) < INFINITY ? __log2f(fabsf(vs)) : -INFINITY; }
 // 2^(s - t) vs for the row's largest score t; nothing where the scale is infinite or the score hidden.
 __device__ __forceinline__ float product_of(float s, float rf, float t, float vs) {
     const float w = __fmul_rn(exp2_fast(__fmaf_rn(s, rf, -t)), fabsf(vs));
     return w < INFINITY ? w : 0.0f;
 }
-// b where the row meets scores up to t and products up to w 2^t.
+// b where the row meets scores up to t and products up to 2^top (rounded at a score's spacing, of which whole numbers are
+// multiples: where b stays, no product reaches 2^16).
 template <int PP>  // parts of P'
-__device__ __forceinline__ float moved(float b, float t, float w) {
-    const float top = t + __log2f(w);
+__device__ __forceinline__ float moved(float b, float t, float top) {
     float to = b;
     if (t + b > kSumTop) to = floorf(__fsub_rd(kSumTop - 4.0f, t));
     if (top + b > kTop) to = fminf(to, floorf(__fsub_rd(16.0f - lazy(PP), top)));

@@ -23,8 +23,9 @@
 // cluster (up to 16), whose partial (max, sum, O) are joined in distributed shared memory in a fixed order: one launch, no
 // workspace, the same bits on every run. Few long sequences: over several clusters each, so that every SM has a part; the
 // clusters' results go to the caller's workspace and join_kernel adds them.
-// Measured (32 heads of 128 over 8 kv heads, int8, bf16): 64 sequences of 8,000 keys, one token each: 116 us (5.2 TB/s). One
-// of 131,001 keys: 65, 80, 94 us for 8, 16, 24 rows; there a warp's chain over a slice (1.6 us, int4 alike) is the bound.
+// Measured (32 heads of 128 over 8 kv heads, int8, bf16): 64 sequences of 8,000 keys, one token each: 114 us in a burst
+// (5.3 TB/s), 126 for a second on end, where the power limit takes a tenth of the clock. One of 131,001 keys: 62, 77, 95 us for 4, 16, 24 rows; there a warp's chain over
+// a slice (1.6 us, int4 alike) is the bound.
 #include <cooperative_groups.h>
 #include <limits.h>
 #include <math.h>
@@ -646,8 +647,8 @@ template <typename T, int BITS>
 static cudaError_t launch_size(const AttnParams &p, int max_len, cudaStream_t stream) {
     // Above 24 rows the tensor-core kernel; above 16 too for heads behind 64 unless P goes in two parts for fp16 callers or a
     // few sequences leave SMs without a second CTA anyway. 24 rows, 8 kv heads, int8, here | there, 64 sequences of 2,000
-    // keys and 16 of 4,000: heads of 128, bf16 89 | 86 and 49 | 43 us, fp32 108 | 100 and 68 | 50, fp16 (int4) 90 | 101 and
-    // 56 | 51; heads of 64, bf16 64 | 82 and 33 | 41. One sequence of 131,001: 95 | 100.
+    // keys and 16 of 4,000: heads of 128, bf16 92 | 86 and 50 | 43 us, fp32 110 | 100 and 66 | 49, fp16 (int4) 92 | 101 and
+    // 54 | 50; heads of 64, bf16 66 | 82 and 34 | 41. One sequence of 131,001, bf16: 95 | 98.
     const long long rows = (long long)p.max_new * p.group;
     const bool many = (long long)p.bt.batch * p.kv_heads > 18 && p.head > 64 && rows::Type<T>::kId != rows::kF16;
     if (rows > (many ? 16 : 24)) return launch_tc(p, rows::Type<T>::kId, BITS, max_len, stream);

@@ -25,8 +25,9 @@
 // What bounds it: for two row tiles of head 128 and 64 keys the exponentials take 1,024 clocks (16 a clock), the MMAs
 // 1,280 (QK at N = 64 waits for shared memory: 48 clocks a product against 32), and shared memory carries 224 KB, 1,800
 // clocks (QK's operands 96, PV's 32, the conversion 64, the softmax's scales 32); the step takes about 2,300. 16 trees of 64
-// tokens, 16,000 keys, 32 heads of 128 over 8 kv heads, int8, bf16: 169 us (636 TFLOP/s). With one row tile the chain of a step is the bound (64 sequences of 2,000
-// keys, 32 | 128 rows: 87 | 107 us, 1,500 | 1,800 clocks a step).
+// tokens, 16,000 keys, 32 heads of 128 over 8 kv heads, int8, bf16: 170 us in a burst (631 TFLOP/s), 184 for a second on end, where the
+// power limit takes a tenth of the clock; their longest sequence's CTAs, 125 steps, take most of it. With one row tile the chain of a step is the bound
+// (64 sequences of 2,000 keys, 32 | 128 rows: 88 | 106 us, 1,500 | 1,800 clocks a step).
 // Up to 128 query rows (MT = 1): both softmax groups take the same rows, for every other step each, with an O and
 // (max, sum) of their own; the two parts are joined like those of the cluster.
 // The keys of a sequence are split over the CTAs of a cluster, joined in distributed shared memory in a fixed order.

@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 && NT <= 2 ? 2 : 1) t
                     for (int nt = 0; nt < NT; nt++) {
                         // The products' own sums are cut towards zero, at 2^-23 for every 16 keys and part: some 1e-4 over 16,000 keys
                         // of a warp whose values have one sign, a quarter of an fp16 output's half step. An fp32 caller's
-                        // slices are therefore added here, rounded to nearest.
+                        // slices are therefore added here, rounded to nearest (an fp16 caller's so: 4 to 10 % longer).
                         constexpr bool APART = sizeof(T) == 4;
                         float (&o)[4] = O[nt][(PER * i + k) / 2];
                         float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};

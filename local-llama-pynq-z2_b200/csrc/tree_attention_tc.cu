@@ -25,9 +25,9 @@
 // What bounds it: for two row tiles of head 128 and 64 keys the exponentials take 1,024 clocks (16 a clock), the MMAs
 // 1,280 (QK at N = 64 waits for shared memory: 48 clocks a product against 32), and shared memory carries 224 KB, 1,800
 // clocks (QK's operands 96, PV's 32, the conversion 64, the softmax's scales 32); the step takes about 2,300. 16 trees of 64
-// tokens, 16,000 keys, 32 heads of 128 over 8 kv heads, int8, bf16: 170 us in a burst (631 TFLOP/s), 184 for a second on end, where the
-// power limit takes a tenth of the clock; their longest sequence's CTAs, 125 steps, take most of it. With one row tile the chain of a step is the bound
-// (64 sequences of 2,000 keys, 32 | 128 rows: 88 | 106 us, 1,500 | 1,800 clocks a step).
+// tokens, 16,000 keys, 32 heads of 128 over 8 kv heads, int8, bf16: 170 us in a burst (631 TFLOP/s), 184 for a second on end,
+// where the power limit takes a tenth of the clock; their longest sequence's CTAs, 125 steps, take most of it. With one row
+// tile the chain of a step is the bound (64 sequences of 2,000 keys, 32 | 128 rows: 88 | 106 us, 1,500 | 1,800 clocks a step).
 // Up to 128 query rows (MT = 1): both softmax groups take the same rows, for every other step each, with an O and
 // (max, sum) of their own; the two parts are joined like those of the cluster.
 // The keys of a sequence are split over the CTAs of a cluster, joined in distributed shared memory in a fixed order.
@@ -284,9 +284,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
     constexpr bool ALT = MT == 1;            // the groups alternate over the steps
     constexpr int PARTS = ALT ? 2 : 1;       // partial results of a row in a CTA
     constexpr int kRaw = S::kRaw;
-    // The products' sums are cut towards zero at 2^-23 for every 16 keys and part, which adds up: values of one sign lost 1e-5 over
-    // 4,096 keys of an fp32 caller and 2e-3 over 500,000. So a group's product starts anew every kSpan steps, and its threads
-    // add what there was to sums of their own, rounded to nearest (in local memory: 260 bytes a thread, touched only then).
+    // The products' sums are cut towards zero at 2^-23 for every 16 keys and part, which adds up: values of one sign lost
+    // 1e-5 over 4,096 keys of an fp32 caller and 2e-3 over 500,000. So a group's product starts anew every kSpan steps, and its
+    // threads add what there was to sums of their own, rounded to nearest (in local memory: 260 bytes a thread, touched only
+    // then).
     // That takes about 3,000 clocks; a step with heads of 64 is shorter, hence the longer span there (16 sequences of 8,000
     // keys, 256 rows of 64: 124 us with 16 steps). bf16 callers, whose output's half step is 4e-3 and whose products have one
     // part, go without.
@@ -594,8 +595,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
         const int R = R0 + (ALT ? 0 : m * 128) + row, draft = R / p.group;
         const float rf = row_factor[ALT ? row : m * 128 + row];
         float unit = INFINITY, l = 0.0f;
-        // This thread's half of O in 16 columns: held from here on where that leaves the steps fewer spills (64 sequences of 2,000
-        // keys, 32 rows: bf16 88 us held, 91 not; fp16 102 and 99), else made anew.
+        // This thread's half of O in 16 columns: held from here on where that leaves the steps fewer spills (64 sequences of
+        // 2,000 keys, 32 rows: bf16 88 us held, 91 not; fp16 102 and 99), else made anew.
         constexpr bool HELD = ALT && (QP == 2 || PP == 1);
         const int held = HELD ? half * (HDP / 32) : 0;
         float sums[SPANS ? HDP / 2 + 1 : 1];  // what spans before summed, and the unit it is in

@@ -260,21 +260,34 @@ struct TcSmem {
 };
 
 // Before the first product of a span: a thread's half of O, from column `at` on, goes into its sums, whose last element is the
-// unit they are in. A call of its own, so that the steps keep their registers.
+// unit they are in. Heads up to 64 leave tensor memory free behind O, which holds the sums then; else they are in local
+// memory. A call of its own, so that the steps keep their registers.
 template <int HDP>
 __device__ __noinline__ void keep(float *sums, uint32_t at, float unit, bool first, uint64_t *pv_done, uint32_t parity) {
+    constexpr bool TM = HDP == 64;
     bar_wait(pv_done, parity);
     fence_after();
-    const float f = first ? 0.0f : unit_factor(sums[HDP / 2], unit);
-    sums[HDP / 2] = unit;
+    float &in = sums[TM ? 0 : HDP / 2];
+    const float f = first ? 0.0f : unit_factor(in, unit);
+    in = unit;
 #pragma unroll 1
     for (int c = 0; c < HDP / 2; c += 16) {
         float o[16];
         tmem_load16(at + c, o);
-        wait_load();
+        if constexpr (TM) {
+            float had[16];
+            tmem_load16(at + HDP + c, had);
+            wait_load();
 #pragma unroll
-        for (int e = 0; e < 16; e++) sums[c + e] = first ? o[e] : __fmaf_rn(sums[c + e], f, o[e]);
+            for (int e = 0; e < 16; e++) had[e] = first ? o[e] : __fmaf_rn(had[e], f, o[e]);
+            tmem_store16(at + HDP + c, reinterpret_cast<const uint32_t *>(had));
+        } else {
+            wait_load();
+#pragma unroll
+            for (int e = 0; e < 16; e++) sums[c + e] = first ? o[e] : __fmaf_rn(sums[c + e], f, o[e]);
+        }
     }
+    if (TM) wait_store();
 }
 
 template <typename T, int QP, int PP, int BITS, int HDP, int MT>
@@ -286,12 +299,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
     constexpr int kRaw = S::kRaw;
     // The products' sums are cut towards zero at 2^-23 for every 16 keys and part, which adds up: values of one sign lost
     // 1e-5 over 4,096 keys of an fp32 caller and 2e-3 over 500,000. So a group's product starts anew every kSpan steps, and its
-    // threads add what there was to sums of their own, rounded to nearest (in local memory: 260 bytes a thread, touched only
-    // then).
-    // That takes about 3,000 clocks; a step with heads of 64 is shorter, hence the longer span there (16 sequences of 8,000
-    // keys, 256 rows of 64: 124 us with 16 steps). bf16 callers, whose output's half step is 4e-3 and whose products have one
+    // threads add what there was to sums of their own, rounded to nearest. That takes about 3,000 clocks for heads of 128 (the
+    // sums, 260 bytes a thread, come from L2). bf16 callers, whose output's half step is 4e-3 and whose products have one
     // part, go without.
-    constexpr int kSpan = PP == 1 ? 1 << 30 : sizeof(T) == 4 ? 2048 / HDP : 128;
+    constexpr int kSpan = PP == 1 ? 1 << 30 : sizeof(T) == 4 ? 16 : 128;
     constexpr bool SPANS = PP > 1;
     extern __shared__ __align__(1024) uint8_t raw_smem[];
     uint8_t *smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);
@@ -599,7 +610,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
         // 2,000 keys, 32 rows: bf16 88 us held, 91 not; fp16 102 and 99), else made anew.
         constexpr bool HELD = ALT && (QP == 2 || PP == 1);
         const int held = HELD ? half * (HDP / 32) : 0;
-        float sums[SPANS ? HDP / 2 + 1 : 1];  // what spans before summed, and the unit it is in
+        float sums[SPANS && HDP == 128 ? HDP / 2 + 1 : 1];  // what spans before summed (or tensor memory), and its unit
         // One step; TAIL: some of its keys are new tokens, or none (a variant of its own: the mask's branches cost the
         // others more than their arithmetic).
         auto step = [&](int i, auto is_tail) -> bool {
@@ -744,9 +755,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attention_tc_kernel(const 
             wait_load();
             if constexpr (SPANS) {
                 if (steps <= kSpan) return;
-                const float f = unit_factor(sums[HDP / 2], unit);
+                const float f = unit_factor(sums[HDP == 128 ? HDP / 2 : 0], unit);
+                float had[16];
+                if constexpr (HDP == 64) {
+                    tmem_load16(o_at + HDP + 16 * c, had);
+                    wait_load();
+                }
 #pragma unroll
-                for (int e = 0; e < 16; e++) o[e] = __fmaf_rn(sums[16 * (c - c0) + e], f, o[e]);
+                for (int e = 0; e < 16; e++)
+                    o[e] = __fmaf_rn(HDP == 64 ? had[e] : sums[HDP == 64 ? 0 : 16 * (c - c0) + e], f, o[e]);
             }
         };
         if (!ALT && p.splits * p.supers == 1) {

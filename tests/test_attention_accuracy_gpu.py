@@ -253,7 +253,7 @@ def test_sums_do_not_drift(torch, mvb, dtype, ctx, span, heads, head, tokens, ma
     torch.manual_seed(2)
     c.cache.vq.copy_(c.cache.vq.abs().clamp(min=30))
     q = (torch.randn(tokens, heads, head, device="cuda")).to(getattr(torch, dtype))
-    check(torch, mvb, c, q, together=64 * (32 if head == 64 and dtype == "float32" else span), max_len=max_len)
+    check(torch, mvb, c, q, together=64 * span, max_len=max_len)
 
 
 @pytest.mark.parametrize("dtype", TYPES)

@@ -261,7 +261,8 @@ int mvb_logprobs(const void *x, long long stride, int dtype, int rows, int vocab
 /* Synchronizes `stream`; 0, or what the serving operators found out of range on the current device since the last call, and
  * clears it: 1 a page number, 2 a length or row range, 3 a rotary position, 4 a token id, 5 a wait inside a kernel that gave
  * up; -1 if the stream failed. The report is the device's, not the stream's (a captured graph may run on any): whoever asks
- * first gets what the calls of every stream found. Ask in one place, after the streams whose calls it answers for. */
+ * first gets what the calls of every stream found. Ask in one place, after the streams whose calls it answers for. Not to be
+ * captured; a thread's first call allocates a few bytes of pinned host memory. */
 int mvb_serve_status(void *stream);
 
 /* ---- Row-sharded matvec with the all-gather fused into the kernel (one process per GPU, NVLink peers) ----
